@@ -129,6 +129,11 @@ def _cumulative(lens):
     return torch.tensor(c, dtype=torch.int32)
 
 
+def _scales(amax, fmt):
+    """fp32 quotients, rounded once (a division by a number becomes a product with its reciprocal)."""
+    return (amax / torch.full_like(amax, QMAX[fmt])).clamp_min(2.0 ** -126)
+
+
 # ---- inputs --------------------------------------------------------------------------------------
 def _cache_of(case, pool, g, dev, filled):
     """Codes and scales of a pool of pages; ``filled`` holds values of unit deviation quantised row by row."""
@@ -139,7 +144,7 @@ def _cache_of(case, pool, g, dev, filled):
         if filled:
             x = torch.randn(shape, generator=g, device=dev)
             x[..., case["dim"]:] = 0
-            scale = (x.abs().amax(-1) / QMAX[case["format"]]).clamp_min(2.0 ** -126)
+            scale = _scales(x.abs().amax(-1), case["format"])
             q = x / scale[..., None]
             q = q.clamp(-127, 127).round() if case["format"] == "int8" else q.clamp(-448, 448)
             parts[name + "_codes"], parts[name + "_scale"] = q.to(CODE[case["format"]]), scale
@@ -273,7 +278,7 @@ def _plain_slots(st):
 
 def _plain_codes(x, fmt):
     """(values of the codes in 64 bits, scales in 32): the quotient is rounded once, in 64 bits."""
-    scale = (x.float().abs().amax(-1) / QMAX[fmt]).clamp_min(2.0 ** -126)
+    scale = _scales(x.float().abs().amax(-1), fmt)
     y = x.double() / scale.double()[..., None]
     if fmt == "int8":
         return y.round().clamp(-127, 127), scale
@@ -423,7 +428,7 @@ def _exact_places(case, table):
 
 def _exact_codes(x, fmt):
     """Nearest code of x / scale, ties to the even code, found among the sorted values of all codes."""
-    scale = torch.clamp(x.abs().amax(-1).float() / QMAX[fmt], min=2.0 ** -126)
+    scale = torch.clamp((x.abs().amax(-1) / QMAX[fmt]).float(), min=2.0 ** -126)
     if fmt == "int8":
         values = torch.arange(-127, 128, dtype=torch.float64, device=x.device)
         even = torch.arange(-127, 128, device=x.device) % 2 == 0
