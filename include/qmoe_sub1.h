@@ -407,6 +407,98 @@ int qmoe_decode_attention_ex(const void *qkv_dev, void *k_cache_dev, void *v_cac
                              void *out_dev, int heads, int head_dim, int max_len, float scale, const float *bias_dev,
                              int32_t *status_dev, int device, void *stream);
 
+/* ---- serving a batch of sequences ---------------------------------------------------------------
+ * No counterpart in the reference, which leaves attention, caches and sampling to HuggingFace behind
+ * model.generate (sub1.py:373-379).  Activations are bf16 or fp16 (QMOE_BF16 / QMOE_FP16); strides are
+ * in elements, the last axis of every tensor is contiguous.  A packed batch holds the rows of its
+ * sequences one after another: sequence s owns rows [cu[s], cu[s + 1]) of an int32 device array of
+ * n_seqs + 1 non-decreasing entries (entries outside the tensor are clamped to it).  Rows behind the
+ * last sequence are neither read nor written. */
+#define QMOE_BF16 0
+#define QMOE_FP16 1
+#define QMOE_FP32 2
+#define QMOE_CACHE_E4M3 0
+#define QMOE_CACHE_INT8 1
+
+typedef struct qmoe_prompt_shape {
+  int64_t total_q, total_k;                     /* rows of q / out and of k / v */
+  int64_t q_row, q_head, k_row, k_head;         /* strides */
+  int64_t v_row, v_head, out_row, out_head;
+  int32_t n_seqs, heads, kv_heads, head_dim;    /* heads a multiple of kv_heads, head_dim <= 256 */
+  int32_t dtype;
+  int32_t n_dist;                               /* columns of the relative bias (0: none) */
+  float scale;                                  /* <= 0: 1 / sqrt(head_dim) */
+} qmoe_prompt_shape;
+
+/* Causal attention over a packed batch of prompts.  Sequence s has n = cu_q[s + 1] - cu_q[s] queries
+ * and m = cu_k[s + 1] - cu_k[s] keys; query i sees keys 0 .. i + m - n (its own position when n = m;
+ * with m > n the first m - n keys are an earlier part of the sequence; with m < n the first n - m
+ * queries see nothing and their output is 0).  Query head h reads key head h / (heads / kv_heads).
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j] + bias) v[j]
+ * with bias = rel_bias_dev[h * n_dist + min(distance, n_dist - 1)] (fp32, may be NULL), the distance
+ * being i + m - n - j: the one-directional relative bias of T5 / Switch (scale 1).  Statistics and
+ * sums are fp32. */
+int qmoe_prompt_attention(const void *q_dev, const void *k_dev, const void *v_dev, void *out_dev,
+                          const int32_t *cu_q_dev, const int32_t *cu_k_dev, const float *rel_bias_dev,
+                          const qmoe_prompt_shape *shape, int device, void *stream);
+
+/* A paged cache whose keys and values are held in 8 bits.  codes: [n_pages][kv_heads][page_size]
+ * [row_bytes], row_bytes = head_dim rounded up to 16, the padding zero, 16-byte aligned; scales: fp32
+ * [n_pages][kv_heads][page_size].  Value = code * scale, with scale = max(amax / 448, 2^-126) (e4m3) or
+ * max(amax / 127, 2^-126) (int8) over the head's row and the code nearest to value / scale, ties to
+ * the even code.  A row with a value that is not finite is stored with scale NaN: it reads back as NaN.
+ * A page table int32 [n_seqs][max_pages] gives the pages of every sequence in order; entries behind a
+ * sequence's last page are not looked at.  page_size is a power of two in [16, 1024], head_dim <= 256. */
+typedef struct qmoe_quant_cache {
+  void *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  int32_t n_pages, page_size, kv_heads, head_dim, format;
+} qmoe_quant_cache;
+
+/* append: row r = cu[s] + i of k / v becomes position start[s] + i of sequence s.  read: the inverse,
+ * into contiguous [n_rows][kv_heads][head_dim] tensors.  A position outside the table (negative, or
+ * >= max_pages * page_size) or on a page number outside [0, n_pages) is refused: *status_dev is
+ * incremented once per row, nothing is written to the cache, and a row read from there is zero.  Pages
+ * that are written must belong to one sequence; pages that are only read may be shared. */
+int qmoe_cache_append(const qmoe_quant_cache *cache, const void *k_dev, const void *v_dev, int64_t k_row,
+                      int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *cu_dev,
+                      const int32_t *start_dev, const int32_t *page_table_dev, int32_t *status_dev, int n_seqs,
+                      int max_pages, int64_t n_rows, int dtype, int device, void *stream);
+int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_dev, const int32_t *cu_dev,
+                    const int32_t *start_dev, const int32_t *page_table_dev, int32_t *status_dev, int n_seqs,
+                    int max_pages, int64_t n_rows, int dtype, int device, void *stream);
+
+/* Attention of one new token per sequence over such a cache: q_dev [n_seqs][heads][head_dim], out_dev
+ * contiguous of the same shape, lengths_dev int32 [n_seqs] = positions to attend to (the new token's
+ * included; 0: the output is 0).  Scale and bias as in qmoe_prompt_attention, the distance being
+ * length - 1 - position.  Positions without a valid page are left out and counted in *status_dev: once
+ * per 16 positions and key head on a bad page number, once per sequence and key head for all positions
+ * behind max_pages * page_size.  work_dev: qmoe_decode_paged_work_bytes bytes, 16-byte
+ * aligned, not shared by calls that may overlap. */
+int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int head_dim, int max_pages, int page_size,
+                                     int device);
+int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev, int64_t q_row, int64_t q_head,
+                                void *out_dev, const int32_t *page_table_dev, const int32_t *lengths_dev,
+                                const float *rel_bias_dev, int n_dist, int32_t *status_dev, void *work_dev, int n_seqs,
+                                int heads, int max_pages, float scale, int dtype, int device, void *stream);
+
+/* One token per row of logits [rows][vocab] (fp32, bf16 or fp16, rows row_stride apart), vocab <=
+ * 262144.  Per row, all device arrays of `rows` entries, each may be NULL but uniform:
+ *   temperature  fp32, NULL: 1; 0: the first index of the largest logit
+ *   top_k        int32, NULL or <= 0: all; else the k largest logits, ties to the lower index
+ *   top_p        fp32, NULL or >= 1: all; else the tokens of what top_k left, in falling order, before
+ *                which less than top_p of its mass lies (one at least)
+ *   min_p        fp32, NULL or <= 0: all; else tokens of at least min(min_p, 1) times the largest probability
+ *   uniform      fp32 in [0, 1): the first token, in index order, up to which the kept mass exceeds
+ *                uniform times the whole of it (values outside are clamped)
+ * tokens int64; logprob fp32 (may be NULL): log of the token's share of the kept mass.  Probabilities
+ * are exp((l - max) / temperature) held as 64-bit multiples of 2^-45, so that sums do not depend on
+ * their order.  A row without a distribution (a NaN or +inf among the logits, all of them -inf, a
+ * temperature that is negative or not finite) gives token -1 and logprob NaN. */
+int qmoe_sample(const void *logits_dev, int64_t row_stride, int rows, int vocab, int dtype, const float *temperature_dev,
+                const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev, const float *uniform_dev,
+                int64_t *tokens_dev, float *logprob_dev, int device, void *stream);
+
 /* Number of kernels this library has launched in the calling process (all devices, all entry points). */
 int64_t qmoe_launch_count(void);
 

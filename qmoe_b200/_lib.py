@@ -55,6 +55,22 @@ class InterleavedStore(ctypes.Structure):
                 ("dec", ctypes.c_void_p), ("rows", ctypes.c_void_p)]
 
 
+class PromptShape(ctypes.Structure):
+    """Mirror of ``qmoe_prompt_shape``."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in
+                ("total_q", "total_k", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")] \
+        + [(name, ctypes.c_int32) for name in ("n_seqs", "heads", "kv_heads", "head_dim", "dtype", "n_dist")] \
+        + [("scale", ctypes.c_float)]
+
+
+class QuantCacheDesc(ctypes.Structure):
+    """Mirror of ``qmoe_quant_cache``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k_codes", "v_codes", "k_scale", "v_scale")] \
+        + [(name, ctypes.c_int32) for name in ("n_pages", "page_size", "kv_heads", "head_dim", "format")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
@@ -104,6 +120,12 @@ SIGNATURES = {
     "qmoe_gemv": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_float, _I, _I, _P]),
     "qmoe_decode_attention": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "qmoe_decode_attention_ex": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, ctypes.c_float, _P, _P, _I, _P]),
+    "qmoe_prompt_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
+    "qmoe_cache_append": (_I, [_P, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P]),
+    "qmoe_cache_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P]),
+    "qmoe_decode_paged_work_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I]),
+    "qmoe_decode_attention_paged": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, ctypes.c_float, _I, _I, _P]),
+    "qmoe_sample": (_I, [_P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
     "qmoe_sub1_code_histogram": (_I, [_P, _L, _P, _I, _P]),
     "qmoe_sub1_remap_tables": (_I, [_P, _P, _P, _P, _I, _P]),
     "qmoe_moe_combine": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),

@@ -1,0 +1,50 @@
+// Shared pieces of the serving kernels: 16-bit activations, packed batches, 8-bit cache codes.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <float.h>
+
+#include "common.cuh"
+
+namespace qmoe {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32(float v) { return v; }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+
+// Rows [begin, end) of sequence s of a packed batch, clamped to the tensor's `total` rows.
+__device__ __forceinline__ int2 packed_rows(const int32_t *__restrict__ cu, int s, long long total) {
+  const int lim = (int)(total > 0x7fffffffLL ? 0x7fffffffLL : total);
+  const int b = min(max(cu[s], 0), lim);
+  return make_int2(b, min(max(cu[s + 1], b), lim));
+}
+
+// Sequence that owns `row`: the last s with cu[s] <= row; -1 when the row lies before the first or
+// behind the last sequence.
+__device__ __forceinline__ int packed_seq(const int32_t *__restrict__ cu, int n_seqs, int row) {
+  if (row < cu[0] || row >= cu[n_seqs]) return -1;
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__host__ __device__ constexpr int cache_row_bytes(int head_dim) { return (head_dim + 15) & ~15; }
+
+}  // namespace qmoe

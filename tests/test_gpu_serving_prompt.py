@@ -1,0 +1,205 @@
+"""Prompt attention against a plain 64-bit statement: head layouts, lengths, strides, masks."""
+import math
+
+import pytest
+import torch
+
+from qmoe_b200 import serving
+from tests import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _cu(lens, first=0):
+    c = [first]
+    for n in lens:
+        c.append(c[-1] + n)
+    return torch.tensor(c, dtype=torch.int32, device=DEV)
+
+
+def _case(lens_q, lens_k, heads, kv_heads, d, dtype, seed=0, small=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    mk = lambda n, h, s: (torch.randn(n, h, d, generator=g, device=DEV) * s).to(dtype)  # noqa: E731
+    return mk(sum(lens_q), heads, small), mk(sum(lens_k), kv_heads, small), mk(sum(lens_k), kv_heads, 1.0)
+
+
+def _check(got, q, k, v, lens_q, lens_k, scale, bias=None, exact_fn=ref.attention_fast):
+    a = b = 0
+    for n, m in zip(lens_q, lens_k):
+        out, size = exact_fn(q[a:a + n].double(), k[b:b + m].double(), v[b:b + m].double(), scale, bias, m - n)
+        err = (got[a:a + n].double() - out).abs()
+        bound = ref.attention_bound(out, size, q.dtype)
+        worst = float((err - bound).max()) if n else 0.0
+        assert worst <= 0, (n, m, worst, float(err.max()))
+        a, b = a + n, b + m
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 65), (8, 2, 128), (3, 1, 64), (2, 2, 1), (6, 3, 40), (2, 1, 127),
+                                              (2, 2, 200), (1, 1, 256), (4, 2, 80), (2, 1, 16)])
+def test_packed_prompts(heads, kv_heads, d, dtype):
+    lens = [1, 130, 0, 257, 64, 2, 33]
+    q, k, v = _case(lens, lens, heads, kv_heads, d, dtype)
+    got = serving.prompt_attention(q, k, v, _cu(lens))
+    _check(got, q, k, v, lens, lens, d ** -0.5)
+
+
+@pytest.mark.parametrize("n", [1, 2, 127, 128, 129, 255, 256, 257, 511, 640, 1000])
+def test_lengths_at_tile_edges(n):
+    q, k, v = _case([n], [n], 2, 1, 64, torch.bfloat16, seed=n)
+    _check(serving.prompt_attention(q, k, v, _cu([n])), q, k, v, [n], [n], 0.125)
+
+
+@pytest.mark.parametrize("d", [64, 65, 128])
+def test_earlier_keys_and_queries_that_see_nothing(d):
+    lens_q, lens_k = [5, 100, 300, 1, 7, 4], [200, 100, 450, 999, 3, 0]       # the last two: queries before any key
+    q, k, v = _case(lens_q, lens_k, 4, 2, d, torch.bfloat16, seed=2)
+    got = serving.prompt_attention(q, k, v, _cu(lens_q), _cu(lens_k))
+    _check(got, q, k, v, lens_q, lens_k, d ** -0.5)
+    assert bool((got[-4:] == 0).all()) and bool((got[-11:-7] == 0).all())
+
+
+@pytest.mark.parametrize("n_dist", [1, 2, 33, 128, 700])
+def test_relative_bias_unscaled(n_dist):
+    lens_q, lens_k = [300, 17, 129], [300, 400, 700]
+    q, k, v = _case(lens_q, lens_k, 4, 4, 64, torch.float16, seed=3, small=64 ** -0.25)
+    bias = torch.randn(4, n_dist, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4)) * 2
+    got = serving.prompt_attention(q, k, v, _cu(lens_q), _cu(lens_k), scale=1.0, rel_bias=bias)
+    _check(got, q, k, v, lens_q, lens_k, 1.0, bias)
+
+
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min])
+def test_bias_that_masks(low):
+    """Distances of 40 and more are masked (a window), or everything is."""
+    lens = [200, 1, 90]
+    q, k, v = _case(lens, lens, 2, 1, 64, torch.bfloat16, seed=5)
+    bias = torch.zeros(2, 41, device=DEV)
+    bias[:, 40] = low
+    got = serving.prompt_attention(q, k, v, _cu(lens), rel_bias=bias)
+    _check(got, q, k, v, lens, lens, 0.125, bias, ref.attention)
+    got = serving.prompt_attention(q, k, v, _cu(lens), rel_bias=torch.full((2, 1), low, device=DEV))
+    if low == -math.inf:
+        assert bool((got == 0).all())
+    else:                                   # the lowest finite value swallows every score: plain averages
+        _check(got, q, k, v, lens, lens, 0.125, torch.full((2, 1), low, device=DEV), ref.attention)
+
+
+def test_strides_of_a_fused_projection_and_odd_offsets():
+    lens = [70, 200]
+    g = torch.Generator(device=DEV).manual_seed(6)
+    for d in (64, 65, 128):
+        rows = torch.randn(270, 3, 4, d, generator=g, device=DEV).bfloat16()
+        q, k, v = rows[:, 0], rows[:, 1], rows[:, 2]
+        want = serving.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), _cu(lens))
+        assert torch.equal(serving.prompt_attention(q, k, v, _cu(lens)), want)
+        # head-major storage, as a cache keeps it
+        kt, vt = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (k, v))
+        assert torch.equal(serving.prompt_attention(q, kt, vt, _cu(lens)), want)
+        # tensors that begin in the middle of a 16-byte unit, rows of odd pitch
+        wide = torch.zeros(270, 4, d + 3, device=DEV).bfloat16()
+        odd = []
+        for t in (q, k, v):
+            w = wide.clone()
+            w[:, :, 1:d + 1] = t
+            odd.append(w[:, :, 1:d + 1])
+        out = wide.clone()[:, :, 2:d + 2]
+        assert torch.equal(serving.prompt_attention(*odd, _cu(lens), out=out), want)
+        # one key head broadcast to all query heads by a stride of 0
+        one = serving.prompt_attention(q, k[:, :1].expand(-1, 4, -1), v[:, :1].expand(-1, 4, -1), _cu(lens))
+        assert torch.equal(one, serving.prompt_attention(q, k[:, :1], v[:, :1], _cu(lens)))
+
+
+@pytest.mark.parametrize("d", [64, 65])
+def test_rows_behind_the_last_sequence_and_before_the_first(d):
+    lens = [40, 133]
+    q, k, v = _case([5 + 173 + 90], [5 + 173 + 90], 2, 2, d, torch.bfloat16, seed=7)
+    for t in (q, k, v):                                   # rows of nobody hold NaN
+        t[:5] = math.nan
+        t[178:] = math.nan
+    out = torch.full_like(q, 7.0)
+    serving.prompt_attention(q, k, v, _cu(lens, 5), out=out)
+    assert bool((out[:5] == 7).all()) and bool((out[178:] == 7).all())
+    _check(out[5:178], q[5:178], k[5:178], v[5:178], lens, lens, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 65, 128])
+@pytest.mark.parametrize("what", ["k", "v", "kv"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_non_finite_later_keys_do_not_reach_earlier_queries(d, what, value):
+    n, at = 300, 201
+    q, k, v = _case([n, 50], [n, 50], 2, 1, d, torch.bfloat16, seed=8)
+    clean = serving.prompt_attention(q, k, v, _cu([n, 50]))
+    if "k" in what:
+        k[at] = value
+    if "v" in what:
+        v[at] = value
+    got = serving.prompt_attention(q, k, v, _cu([n, 50]))
+    assert torch.equal(got[n:], clean[n:])                # another sequence
+    k2, v2 = k.clone(), v.clone()
+    k2[at:n], v2[at:n] = 0, 0
+    _check(got[:at], q[:at], k2[:at], v2[:at], [at], [at], d ** -0.5)
+    if what != "k" or not math.isinf(value):              # an infinite key may also get weight 0
+        assert not bool(torch.isfinite(got[at:n]).any())
+
+
+def test_large_scores_and_constant_rows():
+    q, k, v = _case([260], [260], 2, 2, 64, torch.bfloat16, seed=9)
+    got = serving.prompt_attention(q * 100, k * 100, v, _cu([260]))          # weights are nearly one-hot
+    assert bool(torch.isfinite(got).all())
+    # the score's own error grows with it: 2^-24 * |s| on the exponent, |s| up to 8e4, for near ties
+    out, _ = ref.attention_fast((q * 100).double(), (k * 100).double(), v.double(), 0.125, None, 0)
+    assert float(((got.double() - out).abs() > 0.05).float().mean()) < 1e-3
+    got = serving.prompt_attention(torch.zeros_like(q), k, v, _cu([260]))     # plain averages
+    _check(got, torch.zeros_like(q), k, v, [260], [260], 0.125)
+
+
+def test_many_short_sequences():
+    lens = [(7 * i) % 19 for i in range(700)]
+    q, k, v = _case(lens, lens, 2, 1, 64, torch.bfloat16, seed=10)
+    got = serving.prompt_attention(q, k, v, _cu(lens))
+    whole = torch.cat([ref.attention_fast(q[a:a + n].double(), k[a:a + n].double(), v[a:a + n].double(), 0.125, None, 0)[0]
+                       for a, n in zip(_cu(lens).tolist(), lens)])
+    assert float((got.double() - whole).abs().max()) < 2.0 ** -5             # |v| < 6, weights and output at 2^-8 each
+
+
+def test_empty_batches():
+    q, k, v = _case([4], [4], 2, 1, 64, torch.bfloat16)
+    out = torch.full_like(q, 3.0)
+    assert torch.equal(serving.prompt_attention(q, k, v, _cu([]), out=out), torch.full_like(q, 3.0))
+    assert torch.equal(serving.prompt_attention(q, k, v, _cu([0, 0]), out=out), torch.full_like(q, 3.0))
+    assert serving.prompt_attention(q[:0], k[:0], v[:0], _cu([0])).shape == (0, 2, 64)
+    got = serving.prompt_attention(q, k[:0], v[:0], _cu([4]), _cu([0]))
+    assert bool((got == 0).all())
+
+
+def test_offsets_outside_the_tensors_are_clamped():
+    q, k, v = _case([64], [64], 2, 1, 64, torch.bfloat16, seed=11)
+    want = serving.prompt_attention(q, k, v, _cu([64]))
+    bad = torch.tensor([-50, 1 << 30], dtype=torch.int32, device=DEV)
+    assert torch.equal(serving.prompt_attention(q, k, v, bad), want)
+    falling = torch.tensor([64, 0], dtype=torch.int32, device=DEV)             # no rows at all
+    out = torch.full_like(q, 2.0)
+    assert torch.equal(serving.prompt_attention(q, k, v, falling, out=out), torch.full_like(q, 2.0))
+
+
+def test_same_bits_again_on_another_stream_and_in_a_replayed_graph():
+    lens = [300, 5, 190]
+    q, k, v = _case(lens, lens, 8, 2, 128, torch.bfloat16, seed=12)
+    cu = _cu(lens)
+    want = serving.prompt_attention(q, k, v, cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = serving.prompt_attention(q, k, v, cu)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = serving.prompt_attention(q, k, v, cu)
+    q2, _, _ = _case(lens, lens, 8, 2, 128, torch.bfloat16, seed=13)
+    want2 = serving.prompt_attention(q2, k, v, cu)
+    for src, w in ((q2.clone(), want2), (q.clone(), want)):
+        q.copy_(src)
+        graph.replay()
+        assert torch.equal(held, w)
