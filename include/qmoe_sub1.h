@@ -437,7 +437,8 @@ typedef struct qmoe_prompt_shape {
  *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j] + bias) v[j]
  * with bias = rel_bias_dev[h * n_dist + min(distance, n_dist - 1)] (fp32, may be NULL), the distance
  * being i + m - n - j: the one-directional relative bias of T5 / Switch (scale 1).  Statistics and
- * sums are fp32. */
+ * sums are fp32.  At most 262140 query rows and 32768 sequences a call.  A wait of the tensor-core kernel
+ * that runs out is counted by qmoe_moe_tile_timeouts. */
 int qmoe_prompt_attention(const void *q_dev, const void *k_dev, const void *v_dev, void *out_dev,
                           const int32_t *cu_q_dev, const int32_t *cu_k_dev, const float *rel_bias_dev,
                           const qmoe_prompt_shape *shape, int device, void *stream);

@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libqmoe_sub1.so")
 
 SOURCES = ["api.cu", "sub1_matmul.cu", "sub1_tile.cu", "sub1_pack.cu", "moe_route.cu", "moe_ep.cu", "decoder_glue.cu",
            "prompt_attention.cu", "quant_cache.cu", "sample.cu"]
-HEADERS = ["common.cuh", "sub1_walk.cuh", "serving.cuh"]
+HEADERS = ["common.cuh", "sub1_walk.cuh", "serving.cuh", "tcgen05.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

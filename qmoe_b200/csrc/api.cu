@@ -104,6 +104,7 @@ int set_tile_min_tokens(int tokens);
 void set_items_per_matrix(int wi, int wo);
 int set_fused_phases(int on);
 int set_tile_wait_limit(uint32_t spins);
+int prompt_timeouts(int reset, int *count);
 int work_summary(const void *work, int max_slots, int d_ff, int32_t *out, cudaStream_t stream);
 int launch_grouped_ffn(const SparseTable &tab, const int32_t *dec, const uint16_t *codes,
                        const int32_t *row_off, const void *minmax, const qmoe_matrix_desc *descs,
@@ -970,7 +971,10 @@ int qmoe_moe_tile_timeouts(int device, int reset, int *count_out) {
   QMOE_CUDA(cudaDeviceSynchronize());
   QMOE_CUDA(cudaMemcpy(count_out, word, sizeof(int), cudaMemcpyDeviceToHost));
   if (reset) QMOE_CUDA(cudaMemset(word, 0, sizeof(int)));
-  return QMOE_OK;
+  int prompt = 0;
+  const int rc = prompt_timeouts(reset, &prompt);
+  *count_out += prompt;
+  return rc;
 }
 
 }  // extern "C"

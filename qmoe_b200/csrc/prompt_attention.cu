@@ -2,6 +2,7 @@
 #include <math.h>
 
 #include "serving.cuh"
+#include "tcgen05.cuh"
 
 namespace qmoe {
 
@@ -13,16 +14,11 @@ struct PromptArgs {
   qmoe_prompt_shape s;
 };
 
-// One warp per query row and head, keys one after another with a running maximum: 32 lanes share the
-// head's values.
-template <typename T, int J>  // J = ceil(head_dim / 32)
-__global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
-  const int lane = threadIdx.x & 31, head = blockIdx.x;
-  const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (row >= a.s.total_q) return;
-  const int seq = packed_seq(a.cu_q, a.s.n_seqs, row);
-  if (seq < 0) return;
-  const int2 rq = packed_rows(a.cu_q, seq, a.s.total_q), rk = packed_rows(a.cu_k, seq, a.s.total_k);
+// One query row of one head by one warp, keys one after another with a running maximum; 32 lanes share
+// the head's values.  A key whose weight is 0 contributes nothing, whatever its value row holds.
+template <typename T, int J>  // J >= ceil(head_dim / 32)
+__device__ __forceinline__ void attend_row(const PromptArgs &a, int head, int row, int2 rq, int2 rk) {
+  const int lane = threadIdx.x & 31;
   const int last = row - rq.x + (rk.y - rk.x) - (rq.y - rq.x);  // last key that the query sees
   const int kv = head / (a.s.heads / a.s.kv_heads), d = a.s.head_dim;
   const T *q = reinterpret_cast<const T *>(a.q) + row * a.s.q_row + head * a.s.q_head;
@@ -51,7 +47,7 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
     sum = sum * keep + p;
 #pragma unroll
     for (int j = 0; j < J; j++)
-      if (lane + 32 * j < d) acc[j] = acc[j] * keep + (p != 0.f ? p * to_f32(v[lane + 32 * j]) : 0.f);  // weight 0: whatever is there
+      if (lane + 32 * j < d) acc[j] = acc[j] * keep + (p != 0.f ? p * to_f32(v[lane + 32 * j]) : 0.f);
   }
   T *out = reinterpret_cast<T *>(a.out) + row * a.s.out_row + head * a.s.out_head;
 #pragma unroll
@@ -60,14 +56,441 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 }
 
 template <typename T>
+__global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
+  if (row >= a.s.total_q) return;
+  const int seq = packed_seq(a.cu_q, a.s.n_seqs, row);
+  if (seq < 0) return;
+  attend_row<T, 8>(a, blockIdx.x, row, packed_rows(a.cu_q, seq, a.s.total_q), packed_rows(a.cu_k, seq, a.s.total_k));
+}
+
+// ---- tensor-core tiles ----------------------------------------------------------------------------
+// One CTA owns 256 queries of one head as two tiles of 128 and walks the keys 128 at a time:
+//   S[128 queries, 128 keys] = Q K^T        both from shared memory, fp32 in tensor memory
+//   P = exp2(S * scale * log2 e - m)        by a warpgroup per query tile, one thread per query; P
+//                                           replaces S in tensor memory as 16-bit values
+//   O[128 queries, head_dim] += P V         P from tensor memory, V from shared memory
+// Roles: warps 0-3 and 4-7 the two softmax warpgroups, warp 8 issues the matrix instructions, warps
+// 12-15 copy key and value tiles into a ring of four buffers.  While one query tile's softmax runs, the
+// tensor core works for the other.
+// Every tile lies in shared memory as [8-column chunk][row][16 bytes]: K-major without swizzle for Q and
+// K, and the same bytes read with the head axis contiguous for V.  Chunks are 16 bytes further apart than
+// their rows need so that a warp that copies along a row does not write one bank group again and again.
+// The running maximum is only moved when it grew by more than 2^8: O then stays as it is and P and the
+// sum are taken relative to the older maximum, which is exact up to rounding since both are scaled alike.
+// P is rounded to the type of the inputs for the second product (half a step of it relative to every
+// weight); the sum is taken from the unrounded fp32 weights.
+// A value row that is not finite would spoil queries that give it weight 0 (0 * inf): a query row whose
+// result is not finite is computed again key by key.
+// All waits are bounded; when one runs out the CTA counts itself in d_prompt_timeouts, frees its tensor
+// memory and returns.
+constexpr int kPromptThreads = 512;
+constexpr int kTileRows = 128;
+constexpr int kStages = 4;
+constexpr int kChunkStride = kTileRows * 16 + 16;
+constexpr uint32_t kPromptWait = 1u << 22;
+__device__ int d_prompt_timeouts;
+
+struct PromptBars {
+  uint64_t s_full[2], p_full[2], pv_done[2], kv_full[kStages], kv_empty[kStages], drain;
+};
+
+__device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, volatile int *fail) {
+  for (uint32_t i = 0; i < kPromptWait; i++) {
+    if (mbar_wait(bar, parity, 2)) return true;
+    if (*fail) return false;
+  }
+  *fail = 1;
+  return false;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A bias in units of log 2.  The lowest finite values stay finite: a row of them is a row of equal scores.
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float in_log2(float b) { return b == -INFINITY ? b : fmaxf(b * kLog2e, -FLT_MAX); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Rows [0, rows) of a tile from global memory (`pitch` elements apart), zeros behind them and behind the
+// head's values.  ALIGNED: every row begins on a 16-byte boundary (asynchronous copies).
+template <typename T>
+__device__ __forceinline__ void load_tile(uint8_t *tile, const T *src, long long pitch, int rows, int d, int chunks,
+                                          bool aligned, int tid, int threads) {
+  if (aligned) {
+    const uint32_t base = smem_u32(tile);
+    const int shift = chunks > 8 ? 4 : (chunks > 4 ? 3 : 2);
+    const int c = tid & ((1 << shift) - 1);
+    if (c >= chunks) return;
+    const int bytes = max(min(16, 2 * (d - 8 * c)), 0);
+    for (int r = tid >> shift; r < kTileRows; r += threads >> shift)
+      cp_async16(base + c * kChunkStride + r * 16, r < rows ? src + r * pitch + 8 * c : src, r < rows ? bytes : 0);
+    return;
+  }
+  const int lane = tid & 31, warps = threads >> 5;
+  for (int c0 = 0; c0 < 8 * chunks; c0 += 32) {
+    const int c = c0 + lane;
+    if (c >= 8 * chunks) continue;
+    T *dst = reinterpret_cast<T *>(tile + (c >> 3) * kChunkStride) + (c & 7);
+    for (int r0 = tid >> 5; r0 < kTileRows; r0 += 8 * warps) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int r = r0 + i * warps;
+        v[i] = c < d && r < rows ? src[r * pitch + c] : from_f32<T>(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (r0 + i * warps < kTileRows) dst[(r0 + i * warps) * 8] = v[i];
+    }
+  }
+}
+
+template <typename T, bool BIAS>
+__global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const bool aligned) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ PromptBars s_bar;
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_fail;
+  __shared__ int s_scan[kPromptThreads / 32];
+  __shared__ int s_seq, s_tile;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x;
+
+  // ---- which sequence and tile: blocks count the tiles of all sequences, the longest queries of each first
+  if (tid == 0) s_seq = -1;
+  int before = 0;
+  for (int s0 = 0; s0 < a.s.n_seqs; s0 += kPromptThreads) {
+    const int2 r = s0 + tid < a.s.n_seqs ? packed_rows(a.cu_q, s0 + tid, a.s.total_q) : make_int2(0, 0);
+    const int count = (r.y - r.x + 2 * kTileRows - 1) / (2 * kTileRows);
+    int upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = upto;
+    __syncthreads();
+    int all = 0, mine = before + upto;
+    for (int w = 0; w < kPromptThreads / 32; w++) {
+      if (w < warp) mine += s_scan[w];
+      all += s_scan[w];
+    }
+    const int block = blockIdx.y;
+    if (block < mine && block >= mine - count) {
+      s_seq = s0 + tid;
+      s_tile = mine - 1 - block;
+    }
+    before += all;
+    if (before > block) break;
+  }
+  __syncthreads();
+  const int seq = s_seq;
+  if (seq < 0) return;
+  const int2 rq = packed_rows(a.cu_q, seq, a.s.total_q), rk = packed_rows(a.cu_k, seq, a.s.total_k);
+  const int n = rq.y - rq.x, m = rk.y - rk.x, shift = m - n;
+  const int row0 = s_tile * 2 * kTileRows;
+  int steps[2];  // key tiles that each query tile walks
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int r = row0 + i * kTileRows, rows = min(kTileRows, n - r);
+    const int last = r + rows - 1 + shift;
+    steps[i] = rows <= 0 || last < 0 ? 0 : last / kTileRows + 1;
+  }
+  const int n_steps = max(steps[0], steps[1]);
+  const int d = a.s.head_dim, chunks = 2 * ((d + 15) / 16), tile_bytes = chunks * kChunkStride;
+  const int kv = head / (a.s.heads / a.s.kv_heads);
+  uint8_t *q_tile = smem, *ring = smem + 2 * tile_bytes;
+
+  auto bar = [&](uint64_t &b) { return smem_u32(&b); };
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(bar(s_bar.s_full[i]), 1);
+      mbar_init(bar(s_bar.p_full[i]), kTileRows);
+      mbar_init(bar(s_bar.pv_done[i]), 1);
+    }
+    for (int i = 0; i < kStages; i++) {
+      mbar_init(bar(s_bar.kv_full[i]), kTileRows);
+      mbar_init(bar(s_bar.kv_empty[i]), 1);
+    }
+    mbar_init(bar(s_bar.drain), 1);
+    s_fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc(smem_u32(&s_tmem), 512);
+  if (n_steps > 0) {
+    for (int i = 0; i < 2; i++) {
+      const int r = row0 + i * kTileRows;
+      load_tile(q_tile + i * tile_bytes,
+                reinterpret_cast<const T *>(a.q) + (rq.x + (r < n ? r : 0)) * a.s.q_row + head * a.s.q_head, a.s.q_row,
+                max(0, min(kTileRows, n - r)), d, chunks, aligned, tid, kPromptThreads);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    fence_async_proxy();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp >= 12) {
+      // ---- copies: K 0, V 0, K 1, V 1, ...
+      const int t = tid - 384;
+      for (int item = 0; item < 2 * n_steps; item++) {
+        const int stage = item % kStages;
+        if (item >= kStages && !wait_or_fail(bar(s_bar.kv_empty[stage]), (item / kStages - 1) & 1, &s_fail)) break;
+        const int key0 = (item >> 1) * kTileRows;
+        const bool is_v = item & 1;
+        const long long pitch = is_v ? a.s.v_row : a.s.k_row;
+        const T *src = reinterpret_cast<const T *>(is_v ? a.v : a.k) + (rk.x + (long long)key0) * pitch +
+                       kv * (is_v ? a.s.v_head : a.s.k_head);
+        load_tile(ring + stage * tile_bytes, src, pitch, min(kTileRows, m - key0), d, chunks, aligned, t, kTileRows);
+        cp_async_commit();
+        if (item > 0) {
+          cp_async_wait<1>();
+          fence_async_proxy();
+          mbar_arrive(bar(s_bar.kv_full[(item - 1) % kStages]));
+        }
+      }
+      cp_async_wait<0>();
+      fence_async_proxy();
+      if (n_steps > 0 && !s_fail) mbar_arrive(bar(s_bar.kv_full[(2 * n_steps - 1) % kStages]));
+    } else if (warp == 8 && lane == 0 && n_steps > 0) {
+      // ---- matrix instructions
+      const bool bf16 = sizeof(T) == 2 && a.s.dtype == QMOE_BF16;
+      const uint32_t idesc_s = make_instr_desc(kTileRows, kTileRows, bf16);
+      const uint32_t idesc_o = make_instr_desc(kTileRows, 8 * chunks, bf16, true);
+      auto tile_addr = [&](int item) { return smem_u32(ring + (item % kStages) * tile_bytes); };
+      auto wait_tile = [&](int item) { return wait_or_fail(bar(s_bar.kv_full[item % kStages]), (item / kStages) & 1, &s_fail); };
+      auto scores = [&](int i, int j) {
+        const uint32_t qa = smem_u32(q_tile + i * tile_bytes), ka = tile_addr(2 * j);
+        for (int c = 0; c < chunks; c += 2)
+          mma_bf16(tmem + i * kTileRows, make_smem_desc(qa + c * kChunkStride, kChunkStride, 128),
+                   make_smem_desc(ka + c * kChunkStride, kChunkStride, 128), idesc_s, c > 0);
+        mma_commit(bar(s_bar.s_full[i]));
+      };
+      bool ok = wait_tile(0);
+      if (ok) {
+        tc_fence_after();
+        for (int i = 0; i < 2; i++)
+          if (steps[i] > 0) scores(i, 0);
+        mma_commit(bar(s_bar.kv_empty[0]));
+      }
+      for (int j = 0; ok && j < n_steps; j++) {
+        const bool more = j + 1 < n_steps;
+        ok = wait_tile(2 * j + 1) && (!more || wait_tile(2 * j + 2));
+        for (int i = 0; ok && i < 2; i++) {
+          if (j >= steps[i]) continue;
+          ok = wait_or_fail(bar(s_bar.p_full[i]), j & 1, &s_fail);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = tile_addr(2 * j + 1);
+          for (int k = 0; k < kTileRows / 16; k++)
+            mma_f16_ta(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * k,
+                       make_smem_desc(va + k * 256, 128, kChunkStride), idesc_o, j > 0 || k > 0);
+          mma_commit(bar(s_bar.pv_done[i]));
+          if (j + 1 < steps[i]) scores(i, j + 1);
+        }
+        if (ok) {
+          mma_commit(bar(s_bar.kv_empty[(2 * j + 1) % kStages]));
+          if (more) mma_commit(bar(s_bar.kv_empty[(2 * j + 2) % kStages]));
+        }
+      }
+      if (!ok) {  // whatever is still in flight ends before tensor memory is freed
+        mma_commit(bar(s_bar.drain));
+        mbar_wait(bar(s_bar.drain), 0);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    // ---- softmax and output: thread t of the warpgroup owns query row t of its tile
+    const int i = warp >> 2, t = tid & (kTileRows - 1);
+    const int row = row0 + i * kTileRows + t;
+    const bool live = row < n;
+    const int last = live ? row + shift : -1;  // last key that the query sees
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_s = lane_base + i * kTileRows, t_o = lane_base + 256 + i * kTileRows;
+    const int o_cols = 8 * chunks;
+    const float sl2 = a.s.scale * kLog2e;
+    const float *bias = BIAS ? a.bias + (size_t)head * a.s.n_dist : nullptr;
+    float top = -INFINITY, sum = 0.f;  // maximum that O and the sum are relative to, in units of log 2
+    bool ok = true;
+    for (int j = 0; j < steps[i]; j++) {
+      ok = wait_or_fail(bar(s_bar.s_full[i]), j & 1, &s_fail);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+      float s[kTileRows];
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+      tmem_wait_ld();
+      const int key0 = j * kTileRows;
+      if (BIAS) {
+        // distances of the tile's keys from this query; all behind the last column: one value for all
+        const int first_row = row0 + i * kTileRows + shift;
+        if (first_row - (key0 + kTileRows - 1) >= a.s.n_dist - 1) {
+          const float b = in_log2(bias[a.s.n_dist - 1]);
+#pragma unroll
+          for (int c = 0; c < kTileRows; c++) s[c] = fmaf(s[c], sl2, b);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kTileRows; c++)
+            s[c] = fmaf(s[c], sl2, in_log2(__ldg(bias + max(0, min(last - key0 - c, a.s.n_dist - 1)))));
+        }
+      }
+      const int edge = last - key0;  // columns behind it are masked
+      if (__any_sync(0xffffffffu, edge < kTileRows - 1)) {
+#pragma unroll
+        for (int c = 0; c < kTileRows; c++) s[c] = c <= edge ? s[c] : -INFINITY;
+      }
+      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+      for (int c = 4; c < kTileRows; c += 4) {
+        m0 = fmaxf(m0, s[c]);
+        m1 = fmaxf(m1, s[c + 1]);
+        m2 = fmaxf(m2, s[c + 2]);
+        m3 = fmaxf(m3, s[c + 3]);
+      }
+      float tile_top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      if (!BIAS) tile_top *= sl2;
+      const bool grow = tile_top > top + 8.f || (top == -INFINITY && tile_top > top);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float next = grow ? tile_top : top;
+        const float keep = grow ? exp2_approx(top - next) : 1.f;
+        top = next;
+        sum *= keep;
+        if (j > 0) {
+          ok = wait_or_fail(bar(s_bar.pv_done[i]), (j - 1) & 1, &s_fail);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc_fence_after();
+          for (int c = 0; c < o_cols; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_o + c, o);
+#pragma unroll
+            for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+            tmem_st16(t_o + c, o);
+          }
+        }
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int c0 = 0; c0 < kTileRows; c0 += 32) {
+        uint32_t p[16];
+#pragma unroll
+        for (int c = 0; c < 16; c++) {
+          const float lo = exp2_approx(BIAS ? s[c0 + 2 * c] - base : fmaf(s[c0 + 2 * c], sl2, -base));
+          const float hi = exp2_approx(BIAS ? s[c0 + 2 * c + 1] - base : fmaf(s[c0 + 2 * c + 1], sl2, -base));
+          sum0 += lo;
+          sum1 += hi;
+          p[c] = pack2<T>(lo, hi);
+        }
+        tmem_st16(t_s + c0 / 2, p);
+      }
+      sum += sum0 + sum1;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(bar(s_bar.p_full[i]));
+    }
+    if (ok && steps[i] > 0) {
+      ok = wait_or_fail(bar(s_bar.pv_done[i]), (steps[i] - 1) & 1, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok) {
+      T *out = reinterpret_cast<T *>(a.out) + (rq.x + (long long)(live ? row : 0)) * a.s.out_row + head * a.s.out_head;
+      const bool vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.s.out_row * 2)) & 15u) == 0;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      bool finite = true;
+      for (int c = 0; c < o_cols; c += 16) {
+        uint32_t o[16];
+        if (steps[i] > 0) {
+          tmem_ld16(t_o + c, o);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 16; x++) o[x] = 0u;
+        }
+        float v[16];
+#pragma unroll
+        for (int x = 0; x < 16; x++) {
+          v[x] = __uint_as_float(o[x]) * inv;
+          finite = finite && fabsf(v[x]) <= FLT_MAX;
+        }
+        if (live && vec && c + 16 <= d) {
+          uint4 w[2];
+          uint32_t *p = reinterpret_cast<uint32_t *>(w);
+#pragma unroll
+          for (int x = 0; x < 8; x++) p[x] = pack2<T>(v[2 * x], v[2 * x + 1]);
+          *reinterpret_cast<uint4 *>(out + c) = w[0];
+          *reinterpret_cast<uint4 *>(out + c + 8) = w[1];
+        } else if (live) {
+#pragma unroll
+          for (int x = 0; x < 16; x++)
+            if (c + x < d) out[c + x] = from_f32<T>(v[x]);
+        }
+        __syncwarp();
+      }
+      unsigned again = __ballot_sync(0xffffffffu, live && !finite);
+      while (again != 0) {
+        const int l = __ffs(again) - 1;
+        again &= again - 1;
+        attend_row<T, 4>(a, head, rq.x + row0 + i * kTileRows + (t & ~31) + l, rq, rk);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && s_fail) atomicAdd(&d_prompt_timeouts, 1);
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+int prompt_timeouts(int reset, int *count) {
+  QMOE_CUDA(cudaMemcpyFromSymbol(count, d_prompt_timeouts, sizeof(int)));
+  const int zero = 0;
+  if (reset) QMOE_CUDA(cudaMemcpyToSymbol(d_prompt_timeouts, &zero, sizeof(int)));
+  return QMOE_OK;
+}
+
+template <typename T>
 static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
-  const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 3) / 4));
-  if (a.s.head_dim <= 64)
-    QMOE_LAUNCH((k_prompt_rows<T, 2>), grid, 128, 0, stream, a);
-  else if (a.s.head_dim <= 128)
-    QMOE_LAUNCH((k_prompt_rows<T, 4>), grid, 128, 0, stream, a);
-  else
-    QMOE_LAUNCH((k_prompt_rows<T, 8>), grid, 128, 0, stream, a);
+  if (a.s.head_dim > kTileRows) {
+    const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 3) / 4));
+    QMOE_LAUNCH((k_prompt_rows<T>), grid, 128, 0, stream, a);
+    QMOE_CUDA(cudaGetLastError());
+    return QMOE_OK;
+  }
+  // 16-byte copies where every row of q, k and v begins on a 16-byte boundary, else element by element
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                         (uintptr_t)(2 * (a.s.q_row | a.s.q_head | a.s.k_row | a.s.k_head | a.s.v_row | a.s.v_head));
+  const bool aligned = (bits & 15u) == 0;
+  const int smem = (2 + kStages) * 2 * ((a.s.head_dim + 15) / 16) * kChunkStride;
+  auto kernel = a.bias != nullptr ? k_prompt_tiles<T, true> : k_prompt_tiles<T, false>;
+  cudaFuncAttributes attr;
+  QMOE_CUDA(cudaFuncGetAttributes(&attr, kernel));
+  if (attr.numRegs * kPromptThreads < 65536) {  // the warpgroups' shares have to fit what the block is launched with
+    set_error("prompt attention: built with %d registers a thread, 128 are needed", attr.numRegs);
+    return QMOE_ERR_UNSUPPORTED;
+  }
+  QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 2 * kTileRows - 1) / (2 * kTileRows) + a.s.n_seqs));
+  QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, aligned);
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
 }
@@ -89,8 +512,8 @@ extern "C" int qmoe_prompt_attention(const void *q_dev, const void *k_dev, const
   QMOE_REQUIRE(isfinite(a.s.scale), "scale is not finite");
   if (a.s.n_seqs == 0 || a.s.total_q == 0) return QMOE_OK;
   QMOE_REQUIRE(q_dev && out_dev && (a.s.total_k == 0 || (k_dev && v_dev)), "null device pointer");
-  if (a.s.head_dim > 256 || a.s.total_q > (1 << 18) - 4 || a.s.total_k > 0x7fffffffLL) {
-    set_error("%s: head_dim <= 256, 262140 query rows and 2^31 - 1 key rows are supported", __func__);
+  if (a.s.head_dim > 256 || a.s.total_q > (1 << 18) - 4 || a.s.total_k > 0x7fffffffLL || a.s.n_seqs > 32768) {
+    set_error("%s: head_dim <= 256, 262140 query rows, 2^31 - 1 key rows and 32768 sequences are supported", __func__);
     return QMOE_ERR_UNSUPPORTED;
   }
   if (a.s.scale <= 0.f) a.s.scale = 1.f / sqrtf((float)a.s.head_dim);

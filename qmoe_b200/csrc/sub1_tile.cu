@@ -16,6 +16,7 @@
 // releases its tensor memory and returns.
 #include "common.cuh"
 #include "sub1_walk.cuh"
+#include "tcgen05.cuh"
 
 #include <atomic>
 
@@ -26,7 +27,6 @@ constexpr int kTileN = 64;         // token columns per item (zero padded)
 constexpr int kTileK = 128;        // matrix columns decoded per step
 constexpr int kTileChunks = kTileK / 8;
 constexpr uint32_t kTmemCols = 64; // fp32 accumulator columns (power of two >= 32)
-constexpr uint32_t kWaitLimit = 1u << 24;
 
 // Bound of the waits that DECIDE whether a CTA gives up (tests lower it to 1, "do not poll at all",
 // to make a wait run out without anything hanging; 0 = kWaitLimit).  The clean-up waits before tensor memory is
@@ -54,79 +54,6 @@ struct TileArgs {
   int flags;
   uint32_t wait_limit; // spins of the waits that decide to give up
 };
-
-// ---- PTX wrappers ---------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// Shared-memory matrix descriptor: K-major, no swizzle.  In 16-byte units: start address, leading
-// byte offset = distance between the two 8-column halves of one K=16 step, stride byte offset =
-// distance between groups of 8 rows; bits 46-47 = 1 (descriptor version of this architecture).
-__device__ __forceinline__ uint64_t make_smem_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3fffu);
-  d |= (uint64_t)((lbo_bytes >> 4) & 0x3fffu) << 16;
-  d |= (uint64_t)((sbo_bytes >> 4) & 0x3fffu) << 32;
-  d |= (uint64_t)1 << 46;
-  return d;
-}
-
-// Instruction descriptor of kind::f16: fp32 accumulate, bf16 x bf16, both K-major, M x N.
-__device__ __forceinline__ uint32_t make_instr_desc(int m, int n) {
-  uint32_t d = 0;
-  d |= 1u << 4;                    // accumulator format: F32
-  d |= 1u << 7;                    // A format: BF16
-  d |= 1u << 10;                   // B format: BF16
-  d |= (uint32_t)(n >> 3) << 17;   // N / 8
-  d |= (uint32_t)(m >> 4) << 24;   // M / 16
-  return d;
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t slot_addr, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_addr), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-__device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t mbar_addr) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar_addr) : "memory");
-}
-__device__ __forceinline__ void mbar_init(uint32_t mbar_addr, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(mbar_addr), "r"(count) : "memory");
-}
-// Bounded wait for the phase with the given parity: at most limit - 1 polls (each of which may itself
-// block for a short, hardware-defined time); false if they ran out.  A limit of 1 gives up at once.
-__device__ __forceinline__ bool mbar_wait(uint32_t mbar_addr, uint32_t parity, uint32_t limit = kWaitLimit) {
-  for (uint32_t i = 1; i < limit; i++) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done) : "r"(mbar_addr), "r"(parity) : "memory");
-    if (done) return true;
-  }
-  return false;
-}
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 16 consecutive fp32 accumulator columns of this thread's row (lane) of tensor memory.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 
 // ---- kernel ---------------------------------------------------------------------------------------
 constexpr int kTileThreads = 2 * kTileM;  // warps 0-3 decode rows, warps 4-7 stage the tiles
