@@ -1,4 +1,5 @@
 // Causal attention over a packed batch of prompts (qmoe_prompt_attention).
+#include <cuda.h>
 #include <math.h>
 
 #include "serving.cuh"
@@ -73,9 +74,10 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // Roles: warps 0-3 and 4-7 the two softmax warpgroups, warp 8 issues the matrix instructions, warps
 // 12-15 copy key and value tiles into a ring of four buffers.  While one query tile's softmax runs, the
 // tensor core works for the other.
-// Every tile lies in shared memory as [8-column chunk][row][16 bytes]: K-major without swizzle for Q and
-// K, and the same bytes read with the head axis contiguous for V.  Chunks are 16 bytes further apart than
-// their rows need so that a warp that copies along a row does not write one bank group again and again.
+// Every tile lies in shared memory as rows of 64 columns (128 bytes) under the 128-byte swizzle, one block
+// of 128 rows per 64 columns: K-major for Q and K, and the same bytes with the head axis contiguous for V.
+// Tiles come by bulk tensor copies where the tensors allow a tensor map (rows on 16-byte boundaries), else
+// and at a sequence's last, partial key tile by the copying warps, which write zeros behind the last row.
 // The running maximum is only moved when it grew by more than 2^8: O then stays as it is and P and the
 // sum are taken relative to the older maximum, which is exact up to rounding since both are scaled alike.
 // P is rounded to the type of the inputs for the second product (half a step of it relative to every
@@ -87,12 +89,16 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 constexpr int kPromptThreads = 512;
 constexpr int kTileRows = 128;
 constexpr int kStages = 4;
-constexpr int kChunkStride = kTileRows * 16 + 16;
+constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
 constexpr uint32_t kPromptWait = 1u << 22;
 __device__ int d_prompt_timeouts;
 
+struct PromptMaps {
+  CUtensorMap q, k, v;
+};
+
 struct PromptBars {
-  uint64_t s_full[2], p_full[2], pv_done[2], kv_full[kStages], kv_empty[kStages], drain;
+  uint64_t q_full, s_full[2], p_full[2], pv_done[2], kv_full[kStages], kv_empty[kStages], drain;
 };
 
 __device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, volatile int *fail) {
@@ -128,48 +134,57 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 }
 
 // Rows [0, rows) of a tile from global memory (`pitch` elements apart), zeros behind them and behind the
-// head's values.  ALIGNED: every row begins on a 16-byte boundary (asynchronous copies).
-template <typename T>
+// head's values up to 8 * chunks columns.  `aligned`: every row begins on a 16-byte boundary (asynchronous
+// 16-byte copies, to be waited for by the caller).
+__device__ __forceinline__ uint32_t tile_offset(int row, int unit) {
+  return (uint32_t)((unit >> 3) * kBlockBytes + row * 128 + (((unit & 7) ^ (row & 7)) << 4));
+}
+template <typename T, int THREADS>
 __device__ __forceinline__ void load_tile(uint8_t *tile, const T *src, long long pitch, int rows, int d, int chunks,
-                                          bool aligned, int tid, int threads) {
+                                          bool aligned, int tid) {
   if (aligned) {
     const uint32_t base = smem_u32(tile);
     const int shift = chunks > 8 ? 4 : (chunks > 4 ? 3 : 2);
     const int c = tid & ((1 << shift) - 1);
     if (c >= chunks) return;
     const int bytes = max(min(16, 2 * (d - 8 * c)), 0);
-    for (int r = tid >> shift; r < kTileRows; r += threads >> shift)
-      cp_async16(base + c * kChunkStride + r * 16, r < rows ? src + r * pitch + 8 * c : src, r < rows ? bytes : 0);
+#pragma unroll 8
+    for (int r = tid >> shift; r < kTileRows; r += THREADS >> shift)
+      cp_async16(base + tile_offset(r, c), r < rows ? src + r * pitch + 8 * c : src, r < rows ? bytes : 0);
     return;
   }
-  const int lane = tid & 31, warps = threads >> 5;
+  constexpr int kWarps = THREADS / 32, kBatch = kTileRows / kWarps < 16 ? kTileRows / kWarps : 16;
+  const int lane = tid & 31;
   for (int c0 = 0; c0 < 8 * chunks; c0 += 32) {
     const int c = c0 + lane;
     if (c >= 8 * chunks) continue;
-    T *dst = reinterpret_cast<T *>(tile + (c >> 3) * kChunkStride) + (c & 7);
-    for (int r0 = tid >> 5; r0 < kTileRows; r0 += 8 * warps) {
-      T v[8];
+    for (int r0 = tid >> 5; r0 < kTileRows; r0 += kBatch * kWarps) {
+      T v[kBatch];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int r = r0 + i * warps;
+      for (int i = 0; i < kBatch; i++) {
+        const int r = r0 + i * kWarps;
         v[i] = c < d && r < rows ? src[r * pitch + c] : from_f32<T>(0.f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (r0 + i * warps < kTileRows) dst[(r0 + i * warps) * 8] = v[i];
+      for (int i = 0; i < kBatch; i++)
+        *reinterpret_cast<T *>(tile + tile_offset(r0 + i * kWarps, c >> 3) + 2 * (c & 7)) = v[i];
     }
   }
 }
 
 template <typename T, bool BIAS>
-__global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const bool aligned) {
-  extern __shared__ __align__(128) uint8_t smem[];
+__global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const __grid_constant__ PromptMaps maps,
+                                                                    const bool aligned, const bool tma) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // the swizzle repeats every 1024 bytes
   __shared__ PromptBars s_bar;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
   __shared__ int s_scan[kPromptThreads / 32];
   __shared__ int s_seq, s_tile;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x;
+  __shared__ volatile int s_stop[2];
+  const int tid = threadIdx.x, lane = tid & 31, head = blockIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   // ---- which sequence and tile: blocks count the tiles of all sequences, the longest queries of each first
   if (tid == 0) s_seq = -1;
@@ -213,7 +228,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
     steps[i] = rows <= 0 || last < 0 ? 0 : last / kTileRows + 1;
   }
   const int n_steps = max(steps[0], steps[1]);
-  const int d = a.s.head_dim, chunks = 2 * ((d + 15) / 16), tile_bytes = chunks * kChunkStride;
+  const int d = a.s.head_dim, chunks = 2 * ((d + 15) / 16), blocks = (d + 63) / 64, tile_bytes = blocks * kBlockBytes;
   const int kv = head / (a.s.heads / a.s.kv_heads);
   uint8_t *q_tile = smem, *ring = smem + 2 * tile_bytes;
 
@@ -225,20 +240,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       mbar_init(bar(s_bar.pv_done[i]), 1);
     }
     for (int i = 0; i < kStages; i++) {
-      mbar_init(bar(s_bar.kv_full[i]), kTileRows);
+      mbar_init(bar(s_bar.kv_full[i]), 1);
       mbar_init(bar(s_bar.kv_empty[i]), 1);
     }
+    mbar_init(bar(s_bar.q_full), 1);
     mbar_init(bar(s_bar.drain), 1);
     s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(smem_u32(&s_tmem), 512);
-  if (n_steps > 0) {
+  if (n_steps > 0 && !tma) {
     for (int i = 0; i < 2; i++) {
       const int r = row0 + i * kTileRows;
-      load_tile(q_tile + i * tile_bytes,
-                reinterpret_cast<const T *>(a.q) + (rq.x + (r < n ? r : 0)) * a.s.q_row + head * a.s.q_head, a.s.q_row,
-                max(0, min(kTileRows, n - r)), d, chunks, aligned, tid, kPromptThreads);
+      load_tile<T, kPromptThreads>(q_tile + i * tile_bytes,
+                                   reinterpret_cast<const T *>(a.q) + (rq.x + (r < n ? r : 0)) * a.s.q_row + head * a.s.q_head,
+                                   a.s.q_row, max(0, min(kTileRows, n - r)), d, chunks, aligned, tid);
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -254,68 +270,100 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
     if (warp >= 12) {
       // ---- copies: K 0, V 0, K 1, V 1, ...
       const int t = tid - 384;
-      for (int item = 0; item < 2 * n_steps; item++) {
+      const int n_tma = tma ? 2 * min(n_steps, m / kTileRows) : 0;  // whole key tiles come by bulk copies
+      bool ok = true;
+      if (t == 0 && tma && n_steps > 0) {
+        const uint32_t q_full = bar(s_bar.q_full);
+        mbar_arrive_tx(q_full, (uint32_t)((steps[0] > 0) + (steps[1] > 0)) * tile_bytes);
+        for (int i = 0; i < 2; i++)
+          for (int b = 0; steps[i] > 0 && b < blocks; b++)
+            tma_load3(smem_u32(q_tile) + i * tile_bytes + b * kBlockBytes, &maps.q, 64 * b, head, rq.x + row0 + i * kTileRows, q_full);
+        int item = 0;
+        for (; item < n_tma; item++) {
+          const int stage = item % kStages;
+          ok = item < kStages || wait_or_fail(bar(s_bar.kv_empty[stage]), (item / kStages - 1) & 1, &s_fail);
+          if (!ok) break;
+          const uint32_t full = bar(s_bar.kv_full[stage]);
+          mbar_arrive_tx(full, tile_bytes);
+          for (int b = 0; b < blocks; b++)
+            tma_load3(smem_u32(ring) + stage * tile_bytes + b * kBlockBytes, (item & 1) ? &maps.v : &maps.k, 64 * b, kv,
+                      rk.x + (item >> 1) * kTileRows, full);
+        }
+        if (!ok || s_fail) {  // copies in flight land before the block ends
+          mbar_wait(q_full, 0);
+          for (int x = max(0, item - kStages); x < item; x++) mbar_wait(bar(s_bar.kv_full[x % kStages]), (x / kStages) & 1);
+        }
+      }
+      __syncwarp();
+      for (int item = n_tma; item < 2 * n_steps; item++) {
         const int stage = item % kStages;
-        if (item >= kStages && !wait_or_fail(bar(s_bar.kv_empty[stage]), (item / kStages - 1) & 1, &s_fail)) break;
+        if (t == 0) {
+          if (ok && item >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (item / kStages - 1) & 1, &s_fail);
+          s_stop[item & 1] = !ok;
+        }
+        named_sync(1, kTileRows);
+        if (s_stop[item & 1]) break;  // one decision for all: the other entry is written next
         const int key0 = (item >> 1) * kTileRows;
         const bool is_v = item & 1;
         const long long pitch = is_v ? a.s.v_row : a.s.k_row;
         const T *src = reinterpret_cast<const T *>(is_v ? a.v : a.k) + (rk.x + (long long)key0) * pitch +
                        kv * (is_v ? a.s.v_head : a.s.k_head);
-        load_tile(ring + stage * tile_bytes, src, pitch, min(kTileRows, m - key0), d, chunks, aligned, t, kTileRows);
+        load_tile<T, kTileRows>(ring + stage * tile_bytes, src, pitch, min(kTileRows, m - key0), d, chunks, aligned, t);
         cp_async_commit();
-        if (item > 0) {
-          cp_async_wait<1>();
-          fence_async_proxy();
-          mbar_arrive(bar(s_bar.kv_full[(item - 1) % kStages]));
-        }
+        cp_async_wait<0>();
+        fence_async_proxy();
+        named_sync(1, kTileRows);
+        if (t == 0) mbar_arrive(bar(s_bar.kv_full[stage]));
       }
-      cp_async_wait<0>();
-      fence_async_proxy();
-      if (n_steps > 0 && !s_fail) mbar_arrive(bar(s_bar.kv_full[(2 * n_steps - 1) % kStages]));
-    } else if (warp == 8 && lane == 0 && n_steps > 0) {
-      // ---- matrix instructions
-      const bool bf16 = sizeof(T) == 2 && a.s.dtype == QMOE_BF16;
+    } else if (warp == 8 && n_steps > 0) {
+      // ---- matrix instructions: the whole warp walks along, one elected lane issues
+      const bool bf16 = a.s.dtype == QMOE_BF16;
       const uint32_t idesc_s = make_instr_desc(kTileRows, kTileRows, bf16);
       const uint32_t idesc_o = make_instr_desc(kTileRows, 8 * chunks, bf16, true);
-      auto tile_addr = [&](int item) { return smem_u32(ring + (item % kStages) * tile_bytes); };
-      auto wait_tile = [&](int item) { return wait_or_fail(bar(s_bar.kv_full[item % kStages]), (item / kStages) & 1, &s_fail); };
-      auto scores = [&](int i, int j) {
-        const uint32_t qa = smem_u32(q_tile + i * tile_bytes), ka = tile_addr(2 * j);
-        for (int c = 0; c < chunks; c += 2)
-          mma_bf16(tmem + i * kTileRows, make_smem_desc(qa + c * kChunkStride, kChunkStride, 128),
-                   make_smem_desc(ka + c * kChunkStride, kChunkStride, 128), idesc_s, c > 0);
-        mma_commit(bar(s_bar.s_full[i]));
+      auto tile_addr = [&](int item) { return smem_u32(ring) + (item % kStages) * tile_bytes; };
+      auto wait_tile = [&](int item) {
+        return __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.kv_full[item % kStages]), (item / kStages) & 1, &s_fail));
       };
-      bool ok = wait_tile(0);
+      auto scores = [&](int i, int j) {
+        const uint64_t qa = make_swizzled_desc(smem_u32(q_tile) + i * tile_bytes, 16, 1024);
+        const uint64_t ka = make_swizzled_desc(tile_addr(2 * j), 16, 1024);
+        for (int c = 0; c < chunks / 2; c++) {  // 16 columns each
+          const uint32_t at = ((c >> 2) * kBlockBytes + (c & 3) * 32) >> 4;
+          mma_f16_warp(tmem + i * kTileRows, qa + at, ka + at, idesc_s, c > 0);
+        }
+        mma_commit_warp(bar(s_bar.s_full[i]));
+      };
+      bool ok = !tma || __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.q_full), 0, &s_fail));
+      ok = ok && wait_tile(0);
       if (ok) {
         tc_fence_after();
         for (int i = 0; i < 2; i++)
           if (steps[i] > 0) scores(i, 0);
-        mma_commit(bar(s_bar.kv_empty[0]));
+        mma_commit_warp(bar(s_bar.kv_empty[0]));
       }
       for (int j = 0; ok && j < n_steps; j++) {
         const bool more = j + 1 < n_steps;
         ok = wait_tile(2 * j + 1) && (!more || wait_tile(2 * j + 2));
-        for (int i = 0; ok && i < 2; i++) {
-          if (j >= steps[i]) continue;
-          ok = wait_or_fail(bar(s_bar.p_full[i]), j & 1, &s_fail);
-          if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          if (!ok || j >= steps[i]) continue;
+          ok = __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i]), j & 1, &s_fail));
+          if (!ok) continue;
           tc_fence_after();
-          const uint32_t va = tile_addr(2 * j + 1);
-          for (int k = 0; k < kTileRows / 16; k++)
-            mma_f16_ta(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * k,
-                       make_smem_desc(va + k * 256, 128, kChunkStride), idesc_o, j > 0 || k > 0);
-          mma_commit(bar(s_bar.pv_done[i]));
+          uint64_t va = make_swizzled_desc(tile_addr(2 * j + 1), kBlockBytes, 1024);
+#pragma unroll
+          for (int k = 0; k < kTileRows / 16; k++, va += 2048 >> 4)  // 16 keys each
+            mma_f16_ta_warp(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * k, va, idesc_o, j > 0 || k > 0);
+          mma_commit_warp(bar(s_bar.pv_done[i]));
           if (j + 1 < steps[i]) scores(i, j + 1);
         }
         if (ok) {
-          mma_commit(bar(s_bar.kv_empty[(2 * j + 1) % kStages]));
-          if (more) mma_commit(bar(s_bar.kv_empty[(2 * j + 2) % kStages]));
+          mma_commit_warp(bar(s_bar.kv_empty[(2 * j + 1) % kStages]));
+          if (more) mma_commit_warp(bar(s_bar.kv_empty[(2 * j + 2) % kStages]));
         }
       }
       if (!ok) {  // whatever is still in flight ends before tensor memory is freed
-        mma_commit(bar(s_bar.drain));
+        mma_commit_warp(bar(s_bar.drain));
         mbar_wait(bar(s_bar.drain), 0);
       }
     }
@@ -468,6 +516,36 @@ int prompt_timeouts(int reset, int *count) {
   return QMOE_OK;
 }
 
+// Tensor map of [rows][heads][head_dim] with boxes of 64 values, one head and 128 rows; false where the
+// driver has no such map (a stride of 0, for one): the tiles are then copied by threads.
+static bool make_map(CUtensorMap *map, const void *base, int dtype, int d, int heads, int64_t rows, int64_t head_stride,
+                     int64_t row_stride) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = [] {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return Encode(nullptr);
+    }
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (encode == nullptr || rows < 1) return false;
+  if (heads == 1) head_stride = 8;  // strides of axes of one entry are not used, but checked
+  if (rows == 1) row_stride = 8;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)kTileRows}, steps[3] = {1, 1, 1};
+  if (strides[0] == 0 || strides[1] == 0) return false;
+  return encode(map, dtype == QMOE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T>
 static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
   if (a.s.head_dim > kTileRows) {
@@ -480,7 +558,11 @@ static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                          (uintptr_t)(2 * (a.s.q_row | a.s.q_head | a.s.k_row | a.s.k_head | a.s.v_row | a.s.v_head));
   const bool aligned = (bits & 15u) == 0;
-  const int smem = (2 + kStages) * 2 * ((a.s.head_dim + 15) / 16) * kChunkStride;
+  PromptMaps maps{};
+  const bool tma = aligned && make_map(&maps.q, a.q, a.s.dtype, a.s.head_dim, a.s.heads, a.s.total_q, a.s.q_head, a.s.q_row) &&
+                   make_map(&maps.k, a.k, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.k_head, a.s.k_row) &&
+                   make_map(&maps.v, a.v, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.v_head, a.s.v_row);
+  const int smem = (2 + kStages) * ((a.s.head_dim + 63) / 64) * kBlockBytes + 1024;
   auto kernel = a.bias != nullptr ? k_prompt_tiles<T, true> : k_prompt_tiles<T, false>;
   cudaFuncAttributes attr;
   QMOE_CUDA(cudaFuncGetAttributes(&attr, kernel));
@@ -490,7 +572,7 @@ static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
   }
   QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 2 * kTileRows - 1) / (2 * kTileRows) + a.s.n_seqs));
-  QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, aligned);
+  QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, maps, aligned, tma);
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
 }

@@ -58,9 +58,6 @@ struct TileArgs {
 // ---- kernel ---------------------------------------------------------------------------------------
 constexpr int kTileThreads = 2 * kTileM;  // warps 0-3 decode rows, warps 4-7 stage the tiles
 
-__device__ __forceinline__ void named_sync(int id, int count) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
-}
 __device__ __forceinline__ void named_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
 }

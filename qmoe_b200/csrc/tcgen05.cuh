@@ -72,6 +72,10 @@ __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+__device__ __forceinline__ void named_sync(int id, int count) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
 // 16 consecutive fp32 accumulator columns of this thread's row (lane) of tensor memory.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
@@ -82,13 +86,28 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// D += A B with A (M rows in the lanes, two 16-bit values per column) in tensor memory.
-__device__ __forceinline__ void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
-                                           uint32_t accumulate) {
+// The same by a whole converged warp, one elected lane of which issues (the same one every time).  With the
+// control flow uniform the descriptors stay in uniform registers: 65 clocks a 128 x 128 x 16 product, the
+// tensor core's own time, against 115 when a branch on the lane number guards the instruction.
+__device__ __forceinline__ void mma_f16_warp(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                             uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// A (M rows in the lanes, two 16-bit values per column) from tensor memory.
+__device__ __forceinline__ void mma_f16_ta_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit_warp(uint32_t mbar_addr) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mbar_addr) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar_addr) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar_addr) : "memory");
@@ -113,6 +132,24 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Rows of 128 bytes under the 128-byte swizzle: 16-byte unit u of row r lies at unit u ^ (r & 7); eight rows
+// (1024 bytes, to which the tile is aligned) repeat.  K-major: `sbo` = 1024 between groups of 8 rows, the
+// next 16 columns 32 bytes on.  With the other axis contiguous: `lbo` between blocks of 64 of it, `sbo` =
+// 1024 between groups of 8 of the K axis.
+__device__ __forceinline__ uint64_t make_swizzled_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return make_smem_desc(addr, lbo_bytes, sbo_bytes) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t mbar_addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar_addr), "r"(bytes) : "memory");
+}
+// Box of a three-axis tensor map to shared memory.
+__device__ __forceinline__ void tma_load3(uint32_t smem_addr, const void *map, int x, int y, int z, uint32_t mbar_addr) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_addr), "l"(map), "r"(x), "r"(y), "r"(z), "r"(mbar_addr) : "memory");
+}
 
 // Copy of `bytes` <= 16 bytes to 16 bytes of shared memory, the rest zero; asynchronous.
 __device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void *src, int bytes) {
