@@ -2,6 +2,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "serving.cuh"
 #include "tcgen05.cuh"
 
@@ -90,6 +92,7 @@ constexpr int kPromptThreads = 512;
 constexpr int kTileRows = 128;
 constexpr int kStages = 4;
 constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
+constexpr int kPolyPairs = 2;
 constexpr uint32_t kPromptWait = 1u << 22;
 __device__ int d_prompt_timeouts;
 
@@ -98,7 +101,7 @@ struct PromptMaps {
 };
 
 struct PromptBars {
-  uint64_t q_full, s_full[2], p_full[2], pv_done[2], kv_full[kStages], kv_empty[kStages], drain;
+  uint64_t q_full, s_full[2], p_full[2][2], pv_done[2], kv_full[kStages], kv_empty[kStages], drain;
 };
 
 __device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, volatile int *fail) {
@@ -119,6 +122,56 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // A bias in units of log 2.  The lowest finite values stay finite: a row of them is a row of equal scores.
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float in_log2(float b) { return b == -INFINITY ? b : fmaxf(b * kLog2e, -FLT_MAX); }
+
+// Two fp32 values in one 64-bit register: one instruction works on both.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair_of(float lo, float hi) {
+  pair_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void pair_split(pair_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ pair_t pair_fma(pair_t a, pair_t b, pair_t c) {
+  pair_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ pair_t pair_add(pair_t a, pair_t b) {
+  pair_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of a pair without the special function unit, which is what bounds the softmax (16 results a clock and
+// SM).  x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by the
+// degree-4 polynomial of least relative error on [-1/2, 1/2] (2.6e-6, an order below the rounding of the
+// weights to 16 bits, 2^-9 or 2^-11), n added to the exponent.  x below -126 gives about 2^-126.
+__device__ __forceinline__ pair_t pair_exp2(pair_t x) {
+  float lo, hi;
+  pair_split(x, lo, hi);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.f));
+  x = pair_of(lo, hi);
+  const pair_t n = pair_add(x, pair_of(12582912.f, 12582912.f));
+  const pair_t whole = pair_add(n, pair_of(-12582912.f, -12582912.f));
+  const pair_t f = pair_fma(whole, pair_of(-1.f, -1.f), x);
+  pair_t p = pair_fma(pair_of(0.009570102207362652f, 0.009570102207362652f), f, pair_of(0.05591785907745361f, 0.05591785907745361f));
+  p = pair_fma(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
+  p = pair_fma(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+  p = pair_fma(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  float n_lo, n_hi;
+  pair_split(n, n_lo, n_hi);
+  pair_split(p, lo, hi);
+  return pair_of(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(n_lo) << 23)),
+                 __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n_hi) << 23)));
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -236,7 +289,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(bar(s_bar.s_full[i]), 1);
-      mbar_init(bar(s_bar.p_full[i]), kTileRows);
+      mbar_init(bar(s_bar.p_full[i][0]), kTileRows);
+      mbar_init(bar(s_bar.p_full[i][1]), kTileRows);
       mbar_init(bar(s_bar.pv_done[i]), 1);
     }
     for (int i = 0; i < kStages; i++) {
@@ -347,13 +401,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           if (!ok || j >= steps[i]) continue;
-          ok = __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i]), j & 1, &s_fail));
-          if (!ok) continue;
-          tc_fence_after();
           uint64_t va = make_swizzled_desc(tile_addr(2 * j + 1), kBlockBytes, 1024);
 #pragma unroll
-          for (int k = 0; k < kTileRows / 16; k++, va += 2048 >> 4)  // 16 keys each
-            mma_f16_ta_warp(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * k, va, idesc_o, j > 0 || k > 0);
+          for (int half = 0; half < 2; half++) {
+            ok = ok && __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i][half]), j & 1, &s_fail));
+            if (!ok) continue;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 4 * half; k < 4 * half + 4; k++, va += 2048 >> 4)  // 16 keys each
+              mma_f16_ta_warp(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * k, va, idesc_o, j > 0 || k > 0);
+          }
+          if (!ok) continue;
           mma_commit_warp(bar(s_bar.pv_done[i]));
           if (j + 1 < steps[i]) scores(i, j + 1);
         }
@@ -404,19 +462,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         }
       }
       const int edge = last - key0;  // columns behind it are masked
-      if (__any_sync(0xffffffffu, edge < kTileRows - 1)) {
+      const bool masked = __any_sync(0xffffffffu, edge < kTileRows - 1);
+      if (masked) {
 #pragma unroll
         for (int c = 0; c < kTileRows; c++) s[c] = c <= edge ? s[c] : -INFINITY;
       }
       float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-      for (int c = 4; c < kTileRows; c += 4) {
-        m0 = fmaxf(m0, s[c]);
-        m1 = fmaxf(m1, s[c + 1]);
-        m2 = fmaxf(m2, s[c + 2]);
-        m3 = fmaxf(m3, s[c + 3]);
+      for (int c = 4; c < kTileRows - 4; c += 8) {
+        m0 = max3(m0, s[c], s[c + 4]);
+        m1 = max3(m1, s[c + 1], s[c + 5]);
+        m2 = max3(m2, s[c + 2], s[c + 6]);
+        m3 = max3(m3, s[c + 3], s[c + 7]);
       }
-      float tile_top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      m0 = max3(m0, s[kTileRows - 4], s[kTileRows - 3]);
+      m1 = max3(m1, s[kTileRows - 2], s[kTileRows - 1]);
+      float tile_top = fmaxf(max3(m0, m1, m2), m3);
       if (!BIAS) tile_top *= sl2;
       const bool grow = tile_top > top + 8.f || (top == -INFINITY && tile_top > top);
       if (__any_sync(0xffffffffu, grow)) {
@@ -438,24 +499,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         }
       }
       const float base = top == -INFINITY ? 0.f : top;
-      float sum0 = 0.f, sum1 = 0.f;
+      const pair_t minus = pair_of(-base, -base), by = pair_of(sl2, sl2);
+      pair_t sums = pair_of(0.f, 0.f);
+      // `poly` of 8 pairs go through pair_exp2 (tiles without masked keys: it has no weight of exactly 0)
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int c0 = 0; c0 < kTileRows; c0 += 32) {
-        uint32_t p[16];
+        for (int half = 0; half < 2; half++) {
 #pragma unroll
-        for (int c = 0; c < 16; c++) {
-          const float lo = exp2_approx(BIAS ? s[c0 + 2 * c] - base : fmaf(s[c0 + 2 * c], sl2, -base));
-          const float hi = exp2_approx(BIAS ? s[c0 + 2 * c + 1] - base : fmaf(s[c0 + 2 * c + 1], sl2, -base));
-          sum0 += lo;
-          sum1 += hi;
-          p[c] = pack2<T>(lo, hi);
+          for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 32) {
+            uint32_t p[16];
+#pragma unroll
+            for (int c = 0; c < 16; c++) {
+              const pair_t v = pair_of(s[c0 + 2 * c], s[c0 + 2 * c + 1]);
+              const pair_t x = BIAS ? pair_add(v, minus) : pair_fma(v, by, minus);
+              float lo, hi;
+              pair_t e;
+              if ((c * decltype(poly)::value) % 8 + decltype(poly)::value > 7 && decltype(poly)::value > 0) {
+                e = pair_exp2(x);
+                pair_split(e, lo, hi);
+              } else {
+                pair_split(x, lo, hi);
+                lo = exp2_approx(lo);
+                hi = exp2_approx(hi);
+                e = pair_of(lo, hi);
+              }
+              sums = pair_add(sums, e);
+              p[c] = pack2<T>(lo, hi);
+            }
+            tmem_st16(t_s + c0 / 2, p);
+          }
+          // the product over these 64 keys starts while the next are worked on
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(s_bar.p_full[i][half]));
         }
-        tmem_st16(t_s + c0 / 2, p);
-      }
+      };
+      if (BIAS || masked) weights(std::integral_constant<int, 0>());
+      else weights(std::integral_constant<int, kPolyPairs>());
+      float sum0, sum1;
+      pair_split(sums, sum0, sum1);
       sum += sum0 + sum1;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(bar(s_bar.p_full[i]));
     }
     if (ok && steps[i] > 0) {
       ok = wait_or_fail(bar(s_bar.pv_done[i]), (steps[i] - 1) & 1, &s_fail);
