@@ -444,8 +444,8 @@ int qmoe_prompt_attention(const void *q_dev, const void *k_dev, const void *v_de
                           const qmoe_prompt_shape *shape, int device, void *stream);
 
 /* A paged cache whose keys and values are held in 8 bits.  codes: [n_pages][kv_heads][page_size]
- * [row_bytes], row_bytes = head_dim rounded up to 16, the padding zero, 16-byte aligned; scales: fp32
- * [n_pages][kv_heads][page_size].  Value = code * scale, with scale = max(amax / 448, 2^-126) (e4m3) or
+ * [row_bytes], row_bytes = head_dim rounded up to 16, the padding zero; scales: fp32
+ * [n_pages][kv_heads][page_size]; both 16-byte aligned.  Value = code * scale, with scale = max(amax / 448, 2^-126) (e4m3) or
  * max(amax / 127, 2^-126) (int8) over the head's row and the code nearest to value / scale, ties to
  * the even code.  A row with a value that is not finite is stored with scale NaN: it reads back as NaN.
  * A page table int32 [n_seqs][max_pages] gives the pages of every sequence in order; entries behind a
@@ -475,9 +475,8 @@ int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_
  * length - 1 - position.  Positions without a valid page are left out and counted in *status_dev: once
  * per 16 positions and key head on a bad page number, once per sequence and key head for all positions
  * behind max_pages * page_size.  work_dev: qmoe_decode_paged_work_bytes bytes, 16-byte
- * aligned, not shared by calls that may overlap. */
-int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int head_dim, int max_pages, int page_size,
-                                     int device);
+ * aligned, not shared by calls that may overlap.  At most 4096 sequences a call. */
+int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int head_dim, int device);
 int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev, int64_t q_row, int64_t q_head,
                                 void *out_dev, const int32_t *page_table_dev, const int32_t *lengths_dev,
                                 const float *rel_bias_dev, int n_dist, int32_t *status_dev, void *work_dev, int n_seqs,

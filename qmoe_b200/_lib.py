@@ -123,7 +123,7 @@ SIGNATURES = {
     "qmoe_prompt_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
     "qmoe_cache_append": (_I, [_P, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P]),
     "qmoe_cache_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P]),
-    "qmoe_decode_paged_work_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I]),
+    "qmoe_decode_paged_work_bytes": (_L, [_I, _I, _I, _I, _I]),
     "qmoe_decode_attention_paged": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, ctypes.c_float, _I, _I, _P]),
     "qmoe_sample": (_I, [_P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
     "qmoe_sub1_code_histogram": (_I, [_P, _L, _P, _I, _P]),

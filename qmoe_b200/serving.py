@@ -226,7 +226,7 @@ def decode_attention_paged(q: torch.Tensor, cache: QuantCache, page_table: torch
     bias, n_dist = _bias_args(rel_bias, heads, dev)
     out = torch.empty((n_seqs, heads, hd), dtype=q.dtype, device=dev)
     L = _lib.load()
-    nbytes = int(L.qmoe_decode_paged_work_bytes(n_seqs, heads, cache.kv_heads, hd, max_pages, cache.page_size, dev.index))
+    nbytes = int(L.qmoe_decode_paged_work_bytes(n_seqs, heads, cache.kv_heads, hd, dev.index))
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.check(L.qmoe_decode_attention_paged(
         ctypes.byref(cache.desc), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), page_table.data_ptr(),
