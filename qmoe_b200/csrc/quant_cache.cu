@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "serving.cuh"
+#include "tcgen05.cuh"
 
 namespace qmoe {
 
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(256) k_cache_read(const RowsArgs a) {
 //
 // Tile: S[heads, 16 positions] = Q K^T and O[heads, columns] += W V by mma.sync m16n8k16 in fp16 with fp32
 // sums; both code formats are exact in fp16.  The order of the K axis of a product is free, so every lane's
-// operand comes straight from global memory in pieces of 16 bytes: lane (g, c) of the warp (g = lane / 4,
+// operand comes from the tile's rows in pieces of 16 bytes: lane (g, c) of the warp (g = lane / 4,
 // c = lane % 4) holds bytes 16 c .. 16 c + 15 of every 64 of key g, and columns 16 g .. of values 2c, 2c + 1,
 // 2c + 8, 2c + 9.  Q is brought to fp16 by a power of two per head.
 // Weights: p = exp2(s - m), w = p * value scale / r with r the largest p * value scale so far, so that rows of
@@ -232,27 +233,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 ld_codes16(const uint8_t *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_codes8(const uint8_t *p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t ld_codes4(const uint8_t *p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t ld_codes2(const uint8_t *p) {
-  uint16_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
-  return v;
-}
-
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -262,75 +242,25 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// Registers of one tile: NB units of 16 columns.  Keys: blocks of 64 columns, then single units.  Values:
-// blocks of 128, 64, 32 and 16 columns (16, 8, 4 and 2 bytes a lane) for each of the lane's four rows.
+// A tile in shared memory: 16 rows of key codes, 16 of value codes, 16 + 16 scales.  Rows are `pitch` bytes
+// apart, pitch = 16 mod 64, so that the eight lanes that read together from four value rows meet different
+// banks (and those that read from two key rows at most twice the same).  Every warp has its own ring of
+// kPagedStages tiles, filled by asynchronous copies.
+//
+// A lane's columns of a value row: 16 bytes of every block of 128 columns, then 8, 4 and 2 bytes of blocks
+// of 64, 32 and 16.
+constexpr int kPagedStages = 3;
+__host__ __device__ constexpr int paged_pitch(int width) { return (width + 47) / 64 * 64 + 16; }
+__host__ __device__ constexpr int paged_stage(int width) { return 32 * paged_pitch(width) + 128; }
 template <int NB>
-struct CacheTile {
+struct CacheCols {
   static constexpr int KB = NB / 4, KR = NB % 4, V16 = NB / 8, V8 = NB % 8 / 4, V4 = NB % 4 / 2, V2 = NB % 2;
-  static constexpr int kWords = 4 * V16 + 2 * V8 + V4 + V2;  // value words per row and lane
-  uint32_t k[2][4 * KB + KR];
-  uint32_t v[4][kWords];
-  float2 ks[2], vs[2];
 };
-
-template <int NB>
-__device__ __forceinline__ void load_cache_tile(CacheTile<NB> &t, const CacheView &c, long long slot, int width, int left, int g,
-                                                int q) {
-  using C = CacheTile<NB>;
-  const int units = width >> 4;
-#pragma unroll
-  for (int n = 0; n < 2; n++) {
-    const uint8_t *row = c.k_codes + (slot + 8 * n + g) * width;
-#pragma unroll
-    for (int b = 0; b < C::KB; b++) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (4 * b + q < units) x = ld_codes16(row + 64 * b + 16 * q);
-      t.k[n][4 * b] = x.x;
-      t.k[n][4 * b + 1] = x.y;
-      t.k[n][4 * b + 2] = x.z;
-      t.k[n][4 * b + 3] = x.w;
-    }
-#pragma unroll
-    for (int r = 0; r < C::KR; r++) t.k[n][4 * C::KB + r] = 4 * C::KB + r < units ? ld_codes4(row + 64 * C::KB + 16 * r + 4 * q) : 0u;
-    t.ks[n] = *reinterpret_cast<const float2 *>(c.k_scale + slot + 8 * n + 2 * q);
-    t.vs[n] = *reinterpret_cast<const float2 *>(c.v_scale + slot + 8 * n + 2 * q);
-  }
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    const int at = 8 * (r >> 1) + 2 * q + (r & 1);
-    const uint8_t *row = c.v_codes + (slot + at) * width;
-    const bool in = at < left;  // places behind the last position may hold anything: zeros instead
-#pragma unroll
-    for (int b = 0; b < C::V16; b++) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (in && 128 * b + 16 * g < width) x = ld_codes16(row + 128 * b + 16 * g);
-      t.v[r][4 * b] = x.x;
-      t.v[r][4 * b + 1] = x.y;
-      t.v[r][4 * b + 2] = x.z;
-      t.v[r][4 * b + 3] = x.w;
-    }
-    if (C::V8) {
-      const int off = 128 * C::V16 + 8 * g;
-      uint2 x = make_uint2(0u, 0u);
-      if (in && off < width) x = ld_codes8(row + off);
-      t.v[r][4 * C::V16] = x.x;
-      t.v[r][4 * C::V16 + 1] = x.y;
-    }
-    if (C::V4) {
-      const int off = 128 * C::V16 + 64 * C::V8 + 4 * g;
-      t.v[r][4 * C::V16 + 2 * C::V8] = in && off < width ? ld_codes4(row + off) : 0u;
-    }
-    if (C::V2) {
-      const int off = 128 * C::V16 + 64 * C::V8 + 32 * C::V4 + 2 * g;
-      t.v[r][C::kWords - 1] = in && off < width ? ld_codes2(row + off) : 0u;
-    }
-  }
-}
 
 // Column of n-tile `n` (of 2 * NB) and its column index x (0 .. 7).
 template <int NB>
 __device__ __forceinline__ int value_column(int n, int x) {
-  using C = CacheTile<NB>;
+  using C = CacheCols<NB>;
   if (n < 16 * C::V16) return 128 * (n / 16) + 16 * x + n % 16;
   n -= 16 * C::V16;
   if (C::V8 && n < 8) return 128 * C::V16 + 8 * x + n;
@@ -342,13 +272,24 @@ __device__ __forceinline__ int value_column(int n, int x) {
 
 template <int NB, int FMT, bool WIDE>  // WIDE: more than 8 query heads per key head
 __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(const PagedArgs a) {
-  extern __shared__ long long s_prefix[];  // n_seqs + 1
+  extern __shared__ __align__(16) uint8_t paged_smem[];  // the warps' rings, then n_seqs + 1 prefixes
   __shared__ long long s_warp[kPagedThreads / 32];
-  using C = CacheTile<NB>;
+  using C = CacheCols<NB>;
   constexpr int R = WIDE ? 2 : 1;  // rows of a lane: g and g + 8
   const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const PagedShape shape = paged_shape(a.heads, a.c.kv_heads, a.c.head_dim);
   const int per_seq = a.c.kv_heads * shape.blocks, d = a.c.head_dim;
+  const int pitch = paged_pitch(shape.width), stage_bytes = paged_stage(shape.width), units = shape.width >> 4;
+  uint8_t *ring = paged_smem + (tid >> 5) * kPagedStages * stage_bytes;
+  long long *s_prefix = reinterpret_cast<long long *>(paged_smem + (kPagedThreads / 32) * kPagedStages * stage_bytes);
+  // copies of this lane: pieces lane, lane + 32, ... of 16 bytes of a tile's 16 rows
+  int piece_at[(NB + 1) / 2], piece_row[(NB + 1) / 2];
+#pragma unroll
+  for (int i = 0; i < (NB + 1) / 2; i++) {
+    const int piece = lane + 32 * i, row = piece / units;
+    piece_row[i] = piece < 16 * units ? row : 16;
+    piece_at[i] = row * pitch + (piece - row * units) * 16;
+  }
 
   // tiles before every sequence
   long long before = 0;
@@ -449,30 +390,45 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
       }
     };
 
-    auto process = [&](const CacheTile<NB> &t, int tile) {
+    auto process = [&](const uint8_t *keys, int tile) {
+      const uint8_t *values = keys + 16 * pitch;
+      const float *scales = reinterpret_cast<const float *>(keys + 32 * pitch);
       const int pos0 = tile * 16;
       float c[2][4];
 #pragma unroll
       for (int n = 0; n < 2; n++) {
 #pragma unroll
         for (int i = 0; i < 4; i++) c[n][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < NB; s++) {
+        const uint8_t *row = keys + (8 * n + g) * pitch;
+        auto product = [&](int s, uint32_t word) {
           uint32_t b0, b1;
-          codes_to_half<FMT>(t.k[n][s], b0, b1);
+          codes_to_half<FMT>(word, b0, b1);
           mma_16816(c[n], qa[s][0], WIDE ? qa[s][1] : 0u, qa[s][R], WIDE ? qa[s][2 * R - 1] : 0u, b0, b1);
+        };
+#pragma unroll
+        for (int b = 0; b < C::KB; b++) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (4 * b + q < units) x = *reinterpret_cast<const uint4 *>(row + 64 * b + 16 * q);
+          product(4 * b, x.x);
+          product(4 * b + 1, x.y);
+          product(4 * b + 2, x.z);
+          product(4 * b + 3, x.w);
         }
+#pragma unroll
+        for (int r = 0; r < C::KR; r++)
+          product(4 * C::KB + r, 4 * C::KB + r < units ? *reinterpret_cast<const uint32_t *>(row + 64 * C::KB + 16 * r + 4 * q) : 0u);
       }
+      const float2 ks0 = *reinterpret_cast<const float2 *>(scales + 2 * q), ks1 = *reinterpret_cast<const float2 *>(scales + 8 + 2 * q);
+      const float2 vs0 = *reinterpret_cast<const float2 *>(scales + 16 + 2 * q), vs1 = *reinterpret_cast<const float2 *>(scales + 24 + 2 * q);
+      const float ks[4] = {ks0.x, ks0.y, ks1.x, ks1.y}, vs[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
       uint32_t w16[R][2];
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        float s[4], vs[4];
+        float s[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int n = i >> 1, at = pos0 + 8 * n + 2 * q + (i & 1);
-          const float ks = (i & 1) ? t.ks[n].y : t.ks[n].x;
-          vs[i] = (i & 1) ? t.vs[n].y : t.vs[n].x;
-          s[i] = c[n][2 * r + (i & 1)] * ks * factor[r];
+          s[i] = c[n][2 * r + (i & 1)] * ks[i] * factor[r];
           if (a.bias != nullptr && g + 8 * r < n_heads && at < seen)
             s[i] += paged_log2(__ldg(a.bias + (size_t)(head0 + g + 8 * r) * a.n_dist + min(length - 1 - at, a.n_dist - 1)));
           if (at >= seen) s[i] = -INFINITY;
@@ -509,56 +465,103 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
       auto product = [&](int n, uint32_t b0, uint32_t b1) {
         mma_16816(o[n], w16[0][0], WIDE ? w16[R - 1][0] : 0u, w16[0][1], WIDE ? w16[R - 1][1] : 0u, b0, b1);
       };
-#pragma unroll
-      for (int w = 0; w < C::kWords; w++) {
-        // bytes of rows 2c and 2c + 1 side by side: two columns per word
+      // words of the lane's four rows (positions 2c, 2c + 1, 2c + 8, 2c + 9): bytes of two rows side by side
+      auto products = [&](int n, int count, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
         uint32_t p0, p1, r0, r1;
-        codes_to_half<FMT>(__byte_perm(t.v[0][w], t.v[1][w], 0x5140), p0, p1);
-        codes_to_half<FMT>(__byte_perm(t.v[2][w], t.v[3][w], 0x5140), r0, r1);
-        product(4 * w, p0, r0);
-        product(4 * w + 1, p1, r1);
-        if (!(C::V2 && w == C::kWords - 1)) {
-          codes_to_half<FMT>(__byte_perm(t.v[0][w], t.v[1][w], 0x7362), p0, p1);
-          codes_to_half<FMT>(__byte_perm(t.v[2][w], t.v[3][w], 0x7362), r0, r1);
-          product(4 * w + 2, p0, r0);
-          product(4 * w + 3, p1, r1);
+        codes_to_half<FMT>(__byte_perm(v0, v1, 0x5140), p0, p1);
+        codes_to_half<FMT>(__byte_perm(v2, v3, 0x5140), r0, r1);
+        product(n, p0, r0);
+        product(n + 1, p1, r1);
+        if (count > 2) {
+          codes_to_half<FMT>(__byte_perm(v0, v1, 0x7362), p0, p1);
+          codes_to_half<FMT>(__byte_perm(v2, v3, 0x7362), r0, r1);
+          product(n + 2, p0, r0);
+          product(n + 3, p1, r1);
         }
+      };
+      const uint8_t *row[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) row[r] = values + (8 * (r >> 1) + 2 * q + (r & 1)) * pitch;
+#pragma unroll
+      for (int b = 0; b < C::V16; b++) {
+        uint4 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          v[r] = 128 * b + 16 * g < shape.width ? *reinterpret_cast<const uint4 *>(row[r] + 128 * b + 16 * g) : make_uint4(0u, 0u, 0u, 0u);
+        products(16 * b, 4, v[0].x, v[1].x, v[2].x, v[3].x);
+        products(16 * b + 4, 4, v[0].y, v[1].y, v[2].y, v[3].y);
+        products(16 * b + 8, 4, v[0].z, v[1].z, v[2].z, v[3].z);
+        products(16 * b + 12, 4, v[0].w, v[1].w, v[2].w, v[3].w);
+      }
+      if (C::V8) {
+        const int off = 128 * C::V16 + 8 * g;
+        uint2 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = off < shape.width ? *reinterpret_cast<const uint2 *>(row[r] + off) : make_uint2(0u, 0u);
+        products(16 * C::V16, 4, v[0].x, v[1].x, v[2].x, v[3].x);
+        products(16 * C::V16 + 4, 4, v[0].y, v[1].y, v[2].y, v[3].y);
+      }
+      if (C::V4) {
+        const int off = 128 * C::V16 + 64 * C::V8 + 4 * g;
+        uint32_t v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = off < shape.width ? *reinterpret_cast<const uint32_t *>(row[r] + off) : 0u;
+        products(16 * C::V16 + 8 * C::V8, 4, v[0], v[1], v[2], v[3]);
+      }
+      if (C::V2) {
+        const int off = 128 * C::V16 + 64 * C::V8 + 32 * C::V4 + 2 * g;
+        uint32_t v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = off < shape.width ? *reinterpret_cast<const uint16_t *>(row[r] + off) : 0u;
+        products(16 * C::V16 + 8 * C::V8 + 4 * C::V4, 2, v[0], v[1], v[2], v[3]);
       }
     };
 
-    // ---- tiles; the next one's loads are on their way while one is worked on
-    int pages = 0;  // of lane l: page of tile (first of 32) + l
-    auto load = [&](CacheTile<NB> &t, int tile) {
-      const int in_window = (tile - tile0) & 31;
-      if (in_window == 0) {
-        const long long pos = (long long)(tile + lane) * 16;
-        pages = tile + lane < tile1 ? __ldg(a.c.table + (long long)seq * a.c.max_pages + (pos >> a.c.page_shift)) : -1;
+    // ---- tiles, kPagedStages - 1 of them ahead on their way
+    int pages = 0;        // of lane l: page of tile (first of 32) + l
+    unsigned good = 0;    // bit i: stage i holds a tile
+    auto load = [&](int tile) {
+      const int stage = (tile - tile0) % kPagedStages;
+      good &= ~(1u << stage);
+      if (tile < tile1) {
+        const int in_window = (tile - tile0) & 31;
+        if (in_window == 0) {
+          const long long pos = (long long)(tile + lane) * 16;
+          pages = tile + lane < tile1 ? __ldg(a.c.table + (long long)seq * a.c.max_pages + (pos >> a.c.page_shift)) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, in_window);
+        if (page >= 0 && page < a.c.n_pages) {
+          good |= 1u << stage;
+          const long long slot =
+              ((((long long)page * a.c.kv_heads + kv) << a.c.page_shift) + ((tile * 16) & ((1 << a.c.page_shift) - 1)));
+          const uint32_t to = smem_u32(ring + stage * stage_bytes);
+          const uint8_t *k = a.c.k_codes + slot * shape.width, *v = a.c.v_codes + slot * shape.width;
+          const int left = seen - tile * 16;  // places behind the last position may hold anything: zeros instead
+#pragma unroll
+          for (int i = 0; i < (NB + 1) / 2; i++) {
+            if (piece_row[i] >= 16) continue;
+            const int bytes = piece_row[i] < left ? 16 : 0, from = (lane + 32 * i) * 16;
+            cp_async16(to + piece_at[i], k + from, bytes);
+            cp_async16(to + 16 * pitch + piece_at[i], v + from, bytes);
+          }
+          if (lane < 8) cp_async16(to + 32 * pitch + lane * 16, (lane < 4 ? a.c.k_scale : a.c.v_scale) + slot + 4 * (lane & 3), 16);
+        } else if (lane == 0 && block == 0) {
+          atomicAdd(a.c.status, 1);
+        }
       }
-      const int page = __shfl_sync(0xffffffffu, pages, in_window);
-      const bool good = page >= 0 && page < a.c.n_pages;
-      if (!good) {
-        if (lane == 0 && block == 0) atomicAdd(a.c.status, 1);
-        return false;
-      }
-      const long long slot = ((((long long)page * a.c.kv_heads + kv) << a.c.page_shift) + ((tile * 16) & ((1 << a.c.page_shift) - 1)));
-      load_cache_tile<NB>(t, a.c, slot, shape.width, seen - tile * 16, g, q);
-      return true;
+      cp_async_commit();
     };
-    if (NB <= 8) {
-      CacheTile<NB> t0, t1;
-      bool good0 = load(t0, tile0), good1 = false;
-      for (int tile = tile0; tile < tile1; tile += 2) {
-        if (tile + 1 < tile1) good1 = load(t1, tile + 1);
-        if (good0) process(t0, tile);
-        if (tile + 1 >= tile1) break;
-        if (tile + 2 < tile1) good0 = load(t0, tile + 2);
-        if (good1) process(t1, tile + 1);
-      }
-    } else {
-      CacheTile<NB> t0;
-      for (int tile = tile0; tile < tile1; tile++)
-        if (load(t0, tile)) process(t0, tile);
+#pragma unroll
+    for (int i = 0; i < kPagedStages - 1; i++) load(tile0 + i);
+    for (int tile = tile0; tile < tile1; tile++) {
+      load(tile + kPagedStages - 1);
+      cp_async_wait<kPagedStages - 1>();
+      __syncwarp();
+      const int stage = (tile - tile0) % kPagedStages;
+      if (good >> stage & 1) process(ring + stage * stage_bytes, tile);
+      __syncwarp();  // the stage is filled again next
     }
+    cp_async_wait<0>();
 
     // ---- result of the segment, or the warp's part of it
     const bool whole = tile0 == 0 && tile1 == n_tiles;
@@ -804,26 +807,29 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = shape.group > 8, e4m3 = cache->format == QMOE_CACHE_E4M3;
-  const size_t smem = sizeof(long long) * (size_t)(n_seqs + 1);
+  const size_t smem = (size_t)(kPagedThreads / 32) * kPagedStages * paged_stage(shape.width) + sizeof(long long) * (size_t)(n_seqs + 1);
   const unsigned grid = (unsigned)(a.warps / (kPagedThreads / 32));
   auto run = [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
-    if (e4m3 && wide) QMOE_LAUNCH((k_decode_paged<NB, QMOE_CACHE_E4M3, true>), grid, kPagedThreads, smem, st, a);
-    else if (e4m3) QMOE_LAUNCH((k_decode_paged<NB, QMOE_CACHE_E4M3, false>), grid, kPagedThreads, smem, st, a);
-    else if (wide) QMOE_LAUNCH((k_decode_paged<NB, QMOE_CACHE_INT8, true>), grid, kPagedThreads, smem, st, a);
-    else QMOE_LAUNCH((k_decode_paged<NB, QMOE_CACHE_INT8, false>), grid, kPagedThreads, smem, st, a);
+    auto kernel = e4m3 ? (wide ? k_decode_paged<NB, QMOE_CACHE_E4M3, true> : k_decode_paged<NB, QMOE_CACHE_E4M3, false>)
+                       : (wide ? k_decode_paged<NB, QMOE_CACHE_INT8, true> : k_decode_paged<NB, QMOE_CACHE_INT8, false>);
+    QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    QMOE_LAUNCH(kernel, grid, kPagedThreads, smem, st, a);
+    QMOE_CUDA(cudaGetLastError());
+    return QMOE_OK;
   };
+  int done = QMOE_OK;
   switch (paged_units(shape.width)) {
-    case 1: run(std::integral_constant<int, 1>()); break;
-    case 2: run(std::integral_constant<int, 2>()); break;
-    case 4: run(std::integral_constant<int, 4>()); break;
-    case 5: run(std::integral_constant<int, 5>()); break;
-    case 6: run(std::integral_constant<int, 6>()); break;
-    case 8: run(std::integral_constant<int, 8>()); break;
-    case 12: run(std::integral_constant<int, 12>()); break;
-    default: run(std::integral_constant<int, 16>()); break;
+    case 1: done = run(std::integral_constant<int, 1>()); break;
+    case 2: done = run(std::integral_constant<int, 2>()); break;
+    case 4: done = run(std::integral_constant<int, 4>()); break;
+    case 5: done = run(std::integral_constant<int, 5>()); break;
+    case 6: done = run(std::integral_constant<int, 6>()); break;
+    case 8: done = run(std::integral_constant<int, 8>()); break;
+    case 12: done = run(std::integral_constant<int, 12>()); break;
+    default: done = run(std::integral_constant<int, 16>()); break;
   }
-  QMOE_CUDA(cudaGetLastError());
+  if (done != QMOE_OK) return done;
   QMOE_LAUNCH(k_decode_join, (unsigned)(n_seqs * cache->kv_heads * shape.blocks), kPagedThreads, 0, st, a);
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
