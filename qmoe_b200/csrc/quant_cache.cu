@@ -250,8 +250,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 // A lane's columns of a value row: 16 bytes of every block of 128 columns, then 8, 4 and 2 bytes of blocks
 // of 64, 32 and 16.
 constexpr int kPagedStages = 3;
-__host__ __device__ constexpr int paged_pitch(int width) { return (width + 47) / 64 * 64 + 16; }
-__host__ __device__ constexpr int paged_stage(int width) { return 32 * paged_pitch(width) + 128; }
+__host__ __device__ constexpr int paged_pitch(int nb) { return (16 * nb + 47) / 64 * 64 + 16; }
+__host__ __device__ constexpr int paged_stage(int nb) { return 32 * paged_pitch(nb) + 128; }
 template <int NB>
 struct CacheCols {
   static constexpr int KB = NB / 4, KR = NB % 4, V16 = NB / 8, V8 = NB % 8 / 4, V4 = NB % 4 / 2, V2 = NB % 2;
@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
   const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const PagedShape shape = paged_shape(a.heads, a.c.kv_heads, a.c.head_dim);
   const int per_seq = a.c.kv_heads * shape.blocks, d = a.c.head_dim;
-  const int pitch = paged_pitch(shape.width), stage_bytes = paged_stage(shape.width), units = shape.width >> 4;
+  constexpr int pitch = paged_pitch(NB), stage_bytes = paged_stage(NB);
+  const int units = shape.width >> 4;
   uint8_t *ring = paged_smem + (tid >> 5) * kPagedStages * stage_bytes;
   long long *s_prefix = reinterpret_cast<long long *>(paged_smem + (kPagedThreads / 32) * kPagedStages * stage_bytes);
   // copies of this lane: pieces lane, lane + 32, ... of 16 bytes of a tile's 16 rows
@@ -290,6 +291,12 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
     piece_row[i] = piece < 16 * units ? row : 16;
     piece_at[i] = row * pitch + (piece - row * units) * 16;
   }
+
+  // a kernel may be built for more columns than the rows have: zeros there
+  if (units < NB)
+    for (int i = lane; i < kPagedStages * 32; i += 32)
+      for (int u = units; u < NB; u++)
+        *reinterpret_cast<uint4 *>(ring + (i >> 5) * stage_bytes + (i & 31) * pitch + 16 * u) = make_uint4(0u, 0u, 0u, 0u);
 
   // tiles before every sequence
   long long before = 0;
@@ -345,27 +352,30 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
     for (int r = 0; r < R; r++) {
       const bool live = g + 8 * r < n_heads;
       const long long at = seq * a.q_row + (long long)(head0 + (live ? g + 8 * r : 0)) * a.q_head;
-      auto element = [&](int col) {
-        if (!live || col >= d) return 0.f;
-        return a.dtype == QMOE_BF16 ? to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.q)[at + col])
-                                    : to_f32(reinterpret_cast<const __half *>(a.q)[at + col]);
-      };
       float v[NB][4], amax = 0.f;
 #pragma unroll
-      for (int n = 0; n < NB; n++)
+      for (int n = 0; n < NB; n++) {
+        const int col = n < 4 * C::KB ? 64 * (n >> 2) + 16 * q + 4 * (n & 3) : 16 * n + 4 * q;
+        if (a.dtype == QMOE_BF16) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          v[n][i] = element(n < 4 * C::KB ? 64 * (n >> 2) + 16 * q + 4 * (n & 3) + i : 16 * n + 4 * q + i);
-          amax = fmaxf(amax, fabsf(v[n][i]));
+          for (int i = 0; i < 4; i++) v[n][i] = live && col + i < d ? to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.q)[at + col + i]) : 0.f;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[n][i] = live && col + i < d ? to_f32(reinterpret_cast<const __half *>(a.q)[at + col + i]) : 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(v[n][i]));
+      }
       amax = quad_max(amax);
+      // 2^-e in two factors, either of which is a normal number
       const int e = amax > 0.f && amax <= FLT_MAX ? ilogbf(amax) : 0;
+      const float down0 = scalbnf(1.f, -(e / 2)), down1 = scalbnf(1.f, -(e - e / 2));
       factor[r] = scalbnf(a.scale * 1.4426950408889634f, e);
 #pragma unroll
       for (int n = 0; n < NB; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const __half2 h = __floats2half2_rn(scalbnf(v[n][2 * i], -e), scalbnf(v[n][2 * i + 1], -e));
+          const __half2 h = __floats2half2_rn(v[n][2 * i] * down0 * down1, v[n][2 * i + 1] * down0 * down1);
           qa[n][i * R + r] = *reinterpret_cast<const uint32_t *>(&h);
         }
     }
@@ -375,12 +385,13 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
     for (int n = 0; n < 2 * NB; n++)
 #pragma unroll
       for (int i = 0; i < 4; i++) o[n][i] = 0.f;
-    float m[R], sum[R], unit[R];  // maximum in units of log 2, sum of p, r
+    float m[R], sum[R], unit[R], inv[R];  // maximum in units of log 2, sum of p, r, 1 / r
 #pragma unroll
     for (int r = 0; r < R; r++) {
       m[r] = -INFINITY;
       sum[r] = 0.f;
       unit[r] = 0.f;
+      inv[r] = 0.f;
     }
     auto rescale = [&](int r, float by) {
 #pragma unroll
@@ -407,8 +418,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         };
 #pragma unroll
         for (int b = 0; b < C::KB; b++) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (4 * b + q < units) x = *reinterpret_cast<const uint4 *>(row + 64 * b + 16 * q);
+          const uint4 x = *reinterpret_cast<const uint4 *>(row + 64 * b + 16 * q);
           product(4 * b, x.x);
           product(4 * b + 1, x.y);
           product(4 * b + 2, x.z);
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         }
 #pragma unroll
         for (int r = 0; r < C::KR; r++)
-          product(4 * C::KB + r, 4 * C::KB + r < units ? *reinterpret_cast<const uint32_t *>(row + 64 * C::KB + 16 * r + 4 * q) : 0u);
+          product(4 * C::KB + r, *reinterpret_cast<const uint32_t *>(row + 64 * C::KB + 16 * r + 4 * q));
       }
       const float2 ks0 = *reinterpret_cast<const float2 *>(scales + 2 * q), ks1 = *reinterpret_cast<const float2 *>(scales + 8 + 2 * q);
       const float2 vs0 = *reinterpret_cast<const float2 *>(scales + 16 + 2 * q), vs1 = *reinterpret_cast<const float2 *>(scales + 24 + 2 * q);
@@ -426,12 +436,17 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
       for (int r = 0; r < R; r++) {
         float s[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int n = i >> 1, at = pos0 + 8 * n + 2 * q + (i & 1);
-          s[i] = c[n][2 * r + (i & 1)] * ks[i] * factor[r];
-          if (a.bias != nullptr && g + 8 * r < n_heads && at < seen)
-            s[i] += paged_log2(__ldg(a.bias + (size_t)(head0 + g + 8 * r) * a.n_dist + min(length - 1 - at, a.n_dist - 1)));
-          if (at >= seen) s[i] = -INFINITY;
+        for (int i = 0; i < 4; i++) s[i] = c[i >> 1][2 * r + (i & 1)] * (ks[i] * factor[r]);
+        if (a.bias != nullptr && g + 8 * r < n_heads) {
+          const float *bias = a.bias + (size_t)(head0 + g + 8 * r) * a.n_dist;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            s[i] += paged_log2(__ldg(bias + max(0, min(length - 1 - (pos0 + 8 * (i >> 1) + 2 * q + (i & 1)), a.n_dist - 1))));
+        }
+        if (pos0 + 16 > seen) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (pos0 + 8 * (i >> 1) + 2 * q + (i & 1) >= seen) s[i] = -INFINITY;
         }
         const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
         if (__any_sync(0xffffffffu, top > m[r] + 8.f)) {
@@ -454,11 +469,11 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
           const float next = fmaxf(fmaxf(quad_max(largest), unit[r]), 0x1p-100f);
           rescale(r, unit[r] / next);
           unit[r] = next;
+          inv[r] = 1.f / next;
         }
-        const float inv = unit[r] > 0.f ? 1.f / unit[r] : 0.f;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-          const __half2 h = __floats2half2_rn(u[2 * n] * inv, u[2 * n + 1] * inv);
+          const __half2 h = __floats2half2_rn(u[2 * n] * inv[r], u[2 * n + 1] * inv[r]);
           w16[r][n] = *reinterpret_cast<const uint32_t *>(&h);
         }
       }
@@ -487,7 +502,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         uint4 v[4];
 #pragma unroll
         for (int r = 0; r < 4; r++)
-          v[r] = 128 * b + 16 * g < shape.width ? *reinterpret_cast<const uint4 *>(row[r] + 128 * b + 16 * g) : make_uint4(0u, 0u, 0u, 0u);
+          v[r] = *reinterpret_cast<const uint4 *>(row[r] + 128 * b + 16 * g);
         products(16 * b, 4, v[0].x, v[1].x, v[2].x, v[3].x);
         products(16 * b + 4, 4, v[0].y, v[1].y, v[2].y, v[3].y);
         products(16 * b + 8, 4, v[0].z, v[1].z, v[2].z, v[3].z);
@@ -497,7 +512,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         const int off = 128 * C::V16 + 8 * g;
         uint2 v[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = off < shape.width ? *reinterpret_cast<const uint2 *>(row[r] + off) : make_uint2(0u, 0u);
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint2 *>(row[r] + off);
         products(16 * C::V16, 4, v[0].x, v[1].x, v[2].x, v[3].x);
         products(16 * C::V16 + 4, 4, v[0].y, v[1].y, v[2].y, v[3].y);
       }
@@ -505,61 +520,73 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         const int off = 128 * C::V16 + 64 * C::V8 + 4 * g;
         uint32_t v[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = off < shape.width ? *reinterpret_cast<const uint32_t *>(row[r] + off) : 0u;
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint32_t *>(row[r] + off);
         products(16 * C::V16 + 8 * C::V8, 4, v[0], v[1], v[2], v[3]);
       }
       if (C::V2) {
         const int off = 128 * C::V16 + 64 * C::V8 + 32 * C::V4 + 2 * g;
         uint32_t v[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = off < shape.width ? *reinterpret_cast<const uint16_t *>(row[r] + off) : 0u;
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint16_t *>(row[r] + off);
         products(16 * C::V16 + 8 * C::V8 + 4 * C::V4, 2, v[0], v[1], v[2], v[3]);
       }
     };
 
     // ---- tiles, kPagedStages - 1 of them ahead on their way
-    int pages = 0;        // of lane l: page of tile (first of 32) + l
-    unsigned good = 0;    // bit i: stage i holds a tile
-    auto load = [&](int tile) {
-      const int stage = (tile - tile0) % kPagedStages;
-      good &= ~(1u << stage);
-      if (tile < tile1) {
-        const int in_window = (tile - tile0) & 31;
+    const int tiles_per_page = 1 << (a.c.page_shift - 4);
+    const long long row_bytes = shape.width;
+    int pages = 0, ahead = tile0, fill = 0;  // of lane l: page of tile l of a window of 32; next tile to load and its stage
+    unsigned good = 0;                       // bit i: stage i holds a tile
+    auto load = [&]() {
+      good &= ~(1u << fill);
+      if (ahead < tile1) {
+        const int in_window = (ahead - tile0) & 31;
         if (in_window == 0) {
-          const long long pos = (long long)(tile + lane) * 16;
-          pages = tile + lane < tile1 ? __ldg(a.c.table + (long long)seq * a.c.max_pages + (pos >> a.c.page_shift)) : -1;
+          const int at = ahead + lane;
+          pages = at < tile1 ? __ldg(a.c.table + (long long)seq * a.c.max_pages + (at >> (a.c.page_shift - 4))) : -1;
         }
         const int page = __shfl_sync(0xffffffffu, pages, in_window);
         if (page >= 0 && page < a.c.n_pages) {
-          good |= 1u << stage;
-          const long long slot =
-              ((((long long)page * a.c.kv_heads + kv) << a.c.page_shift) + ((tile * 16) & ((1 << a.c.page_shift) - 1)));
-          const uint32_t to = smem_u32(ring + stage * stage_bytes);
-          const uint8_t *k = a.c.k_codes + slot * shape.width, *v = a.c.v_codes + slot * shape.width;
-          const int left = seen - tile * 16;  // places behind the last position may hold anything: zeros instead
+          good |= 1u << fill;
+          const long long slot = (((long long)page * a.c.kv_heads + kv) << a.c.page_shift) + 16 * (ahead & (tiles_per_page - 1));
+          const uint32_t to = smem_u32(ring) + fill * stage_bytes;
+          const uint8_t *k = a.c.k_codes + slot * row_bytes + lane * 16, *v = a.c.v_codes + slot * row_bytes + lane * 16;
+          const int left = seen - ahead * 16;
+          if (left >= 16) {
 #pragma unroll
-          for (int i = 0; i < (NB + 1) / 2; i++) {
-            if (piece_row[i] >= 16) continue;
-            const int bytes = piece_row[i] < left ? 16 : 0, from = (lane + 32 * i) * 16;
-            cp_async16(to + piece_at[i], k + from, bytes);
-            cp_async16(to + 16 * pitch + piece_at[i], v + from, bytes);
+            for (int i = 0; i < (NB + 1) / 2; i++) {
+              if (piece_row[i] >= 16) continue;
+              cp_async16(to + piece_at[i], k + 512 * i);
+              cp_async16(to + 16 * pitch + piece_at[i], v + 512 * i);
+            }
+          } else {  // places behind the last position may hold anything: zeros instead
+#pragma unroll
+            for (int i = 0; i < (NB + 1) / 2; i++) {
+              if (piece_row[i] >= 16) continue;
+              const int bytes = piece_row[i] < left ? 16 : 0;
+              cp_async16(to + piece_at[i], k + 512 * i, bytes);
+              cp_async16(to + 16 * pitch + piece_at[i], v + 512 * i, bytes);
+            }
           }
-          if (lane < 8) cp_async16(to + 32 * pitch + lane * 16, (lane < 4 ? a.c.k_scale : a.c.v_scale) + slot + 4 * (lane & 3), 16);
+          if (lane < 8) cp_async16(to + 32 * pitch + lane * 16, (lane < 4 ? a.c.k_scale : a.c.v_scale) + slot + 4 * (lane & 3));
         } else if (lane == 0 && block == 0) {
           atomicAdd(a.c.status, 1);
         }
       }
       cp_async_commit();
+      ahead++;
+      fill = fill == kPagedStages - 1 ? 0 : fill + 1;
     };
 #pragma unroll
-    for (int i = 0; i < kPagedStages - 1; i++) load(tile0 + i);
+    for (int i = 0; i < kPagedStages - 1; i++) load();
+    int stage = 0;
     for (int tile = tile0; tile < tile1; tile++) {
-      load(tile + kPagedStages - 1);
+      load();
       cp_async_wait<kPagedStages - 1>();
       __syncwarp();
-      const int stage = (tile - tile0) % kPagedStages;
       if (good >> stage & 1) process(ring + stage * stage_bytes, tile);
       __syncwarp();  // the stage is filled again next
+      stage = stage == kPagedStages - 1 ? 0 : stage + 1;
     }
     cp_async_wait<0>();
 
@@ -603,40 +630,85 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
   }
 }
 
-// One CTA per sequence and block of query heads: joins the parts of the warps that share it, writes zeros
-// for a sequence without positions, counts a length that its page table cannot hold.
-__global__ void __launch_bounds__(kPagedThreads) k_decode_join(const PagedArgs a) {
+// One CTA per sequence and query head: joins the parts of the warps that share it, writes zeros for a
+// sequence without positions, counts a length that its page table cannot hold.  The parts' weights are found
+// by all threads at once; then every warp sums its share of the parts, four at a time.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) k_decode_join(const PagedArgs a) {
+  extern __shared__ float s_weight[];  // one per warp of the first kernel, then [warps of this CTA][columns]
+  __shared__ float s_red[kJoinThreads / 32];
   const PagedShape shape = paged_shape(a.heads, a.c.kv_heads, a.c.head_dim);
-  const int per_seq = a.c.kv_heads * shape.blocks, seq = blockIdx.x / per_seq, which = blockIdx.x % per_seq;
-  const int kv = which / shape.blocks, block = which % shape.blocks, d = a.c.head_dim, row_floats = shape.width + 2;
-  const int head0 = kv * shape.group + block * 16, n_heads = min(16, shape.group - block * 16);
+  const int seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads, d = a.c.head_dim, row_floats = shape.width + 2;
+  const int kv = head / shape.group, block = head % shape.group / 16, row = head % shape.group % 16;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seen = paged_seen(a, seq), n_tiles = (seen + 15) / 16;
-  if (threadIdx.x == 0 && block == 0 && a.lengths[seq] > seen) atomicAdd(a.c.status, 1);
-  const long long quota = paged_quota(a.prefix[a.n_seqs], a.warps);
-  const long long begin = a.prefix[seq] + (long long)which * n_tiles, end = begin + n_tiles;
-  const int w0 = (int)(begin / quota), w1 = n_tiles > 0 ? (int)((end - 1) / quota) : w0;
-  if (n_tiles > 0 && w0 == w1) return;
-  auto part = [&](int w, int row) {
-    return a.parts + ((size_t)(2 * w + (w == w0 ? 1 : 0)) * shape.rows + row) * row_floats;
-  };
-  for (int at = threadIdx.x; at < n_heads * d; at += kPagedThreads) {
-    const int row = at / d, col = at % d;
-    float top = -INFINITY, sum = 0.f, o = 0.f;
-    if (n_tiles > 0) {
-      for (int w = w0; w <= w1; w++) top = fmaxf(top, part(w, row)[0]);
-      const float base = top == -INFINITY ? 0.f : top;
-      for (int w = w0; w <= w1; w++) {
-        const float *p = part(w, row);
-        const float l = p[1];
-        const float weight = l == 0.f ? 0.f : l * paged_exp2(p[0] - base);
-        sum += weight;
-        if (weight != 0.f) o += weight * p[2 + col];
-      }
-    }
-    const float v = sum == 0.f ? 0.f : o / sum;
-    const long long to = ((long long)seq * a.heads + head0 + row) * d + col;
+  if (tid == 0 && head % shape.group == 0 && a.lengths[seq] > seen) atomicAdd(a.c.status, 1);
+  auto store = [&](int col, float v) {
+    const long long to = ((long long)seq * a.heads + head) * d + col;
     if (a.dtype == QMOE_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[to] = from_f32<__nv_bfloat16>(v);
     else reinterpret_cast<__half *>(a.out)[to] = from_f32<__half>(v);
+  };
+  if (n_tiles == 0) {
+    for (int col = tid; col < d; col += kJoinThreads) store(col, 0.f);
+    return;
+  }
+  const long long quota = paged_quota(a.prefix[a.n_seqs], a.warps);
+  const long long begin = a.prefix[seq] + (long long)(kv * shape.blocks + block) * n_tiles, end = begin + n_tiles;
+  const int w0 = (int)(begin / quota), n_parts = (int)((end - 1) / quota) - w0 + 1;
+  if (n_parts == 1) return;
+  auto part = [&](int p) { return a.parts + ((size_t)(2 * (w0 + p) + (p == 0 ? 1 : 0)) * shape.rows + row) * row_floats; };
+  float top = -INFINITY;
+  for (int p = tid; p < n_parts; p += kJoinThreads) top = fmaxf(top, part(p)[0]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_red[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < kJoinThreads / 32; w++) top = fmaxf(top, s_red[w]);
+  const float base = top == -INFINITY ? 0.f : top;
+  __syncthreads();
+  float sum = 0.f;
+  for (int p = tid; p < n_parts; p += kJoinThreads) {
+    const float2 ml = make_float2(part(p)[0], part(p)[1]);
+    const float weight = ml.y == 0.f ? 0.f : ml.y * paged_exp2(ml.x - base);
+    s_weight[p] = weight;
+    sum += weight;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_red[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+  for (int w = 0; w < kJoinThreads / 32; w++) sum += s_red[w];
+  float *s_acc = s_weight + a.warps + warp * 256;
+  for (int c0 = 0; c0 < d; c0 += 128) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = warp; p0 < n_parts; p0 += 4 * (kJoinThreads / 32)) {
+      float v[4][4], weight[4];
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const int p = p0 + x * (kJoinThreads / 32);
+        weight[x] = p < n_parts ? s_weight[p] : 0.f;
+        const float *from = part(p < n_parts ? p : p0) + 2;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int col = c0 + lane + 32 * i;
+          v[x][i] = col < d && weight[x] != 0.f ? from[col] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] += weight[x] * v[x][i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (c0 + lane + 32 * i < d) s_acc[c0 + lane + 32 * i] = acc[i];
+  }
+  __syncthreads();
+  for (int col = tid; col < d; col += kJoinThreads) {
+    float o = 0.f;
+    for (int w = 0; w < kJoinThreads / 32; w++) o += s_weight[a.warps + w * 256 + col];
+    store(col, sum == 0.f ? 0.f : o / sum);
   }
 }
 
@@ -784,7 +856,7 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
   if (n_seqs == 0) return QMOE_OK;
   QMOE_REQUIRE(q_dev && out_dev && lengths_dev && work_dev, "null device pointer");
   QMOE_REQUIRE((reinterpret_cast<uintptr_t>(work_dev) & 15u) == 0, "workspace must be 16-byte aligned");
-  if (n_seqs > kPagedMaxSeqs) {
+  if (n_seqs > kPagedMaxSeqs || (int64_t)n_seqs * heads > 0x7fffffffLL) {
     set_error("%s: at most %d sequences", __func__, kPagedMaxSeqs);
     return QMOE_ERR_UNSUPPORTED;
   }
@@ -807,7 +879,7 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = shape.group > 8, e4m3 = cache->format == QMOE_CACHE_E4M3;
-  const size_t smem = (size_t)(kPagedThreads / 32) * kPagedStages * paged_stage(shape.width) + sizeof(long long) * (size_t)(n_seqs + 1);
+  const size_t smem = (size_t)(kPagedThreads / 32) * kPagedStages * paged_stage(paged_units(shape.width)) + sizeof(long long) * (size_t)(n_seqs + 1);
   const unsigned grid = (unsigned)(a.warps / (kPagedThreads / 32));
   auto run = [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
@@ -830,7 +902,7 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
     default: done = run(std::integral_constant<int, 16>()); break;
   }
   if (done != QMOE_OK) return done;
-  QMOE_LAUNCH(k_decode_join, (unsigned)(n_seqs * cache->kv_heads * shape.blocks), kPagedThreads, 0, st, a);
+  QMOE_LAUNCH(k_decode_join, (unsigned)(n_seqs * heads), kJoinThreads, (a.warps + 256 * (kJoinThreads / 32)) * sizeof(float), st, a);
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
 }

@@ -172,6 +172,9 @@ __device__ __forceinline__ void tma_load3(uint32_t smem_addr, const void *map, i
 __device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
