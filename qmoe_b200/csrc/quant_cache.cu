@@ -156,12 +156,15 @@ __global__ void __launch_bounds__(256) k_cache_read(const RowsArgs a) {
 // contiguous run of tiles; what belongs to one (sequence, head block) is a segment.  A segment that lies
 // wholly in one warp's run is written to the output at once, of the others each warp leaves its part
 // (maximum, sum, quotient) in the workspace, and a second kernel joins the parts.  No warp waits for another.
+// (Two to four times as many, shorter runs, started as earlier ones end, even out the warps' speeds but cost
+// more in starts and parts: 131 us became 135 to 148 on a batch of 64 sequences and 616 MB.)
 //
-// Tile: S[heads, 16 positions] = Q K^T and O[heads, columns] += W V by mma.sync m16n8k16 in fp16 with fp32
-// sums; both code formats are exact in fp16.  The order of the K axis of a product is free, so every lane's
-// operand comes from the tile's rows in pieces of 16 bytes: lane (g, c) of the warp (g = lane / 4,
-// c = lane % 4) holds bytes 16 c .. 16 c + 15 of every 64 of key g, and columns 16 g .. of values 2c, 2c + 1,
-// 2c + 8, 2c + 9.  Q is brought to fp16 by a power of two per head.
+// Tile: S[16 positions, 8 heads] = K Q^T and O[columns, 8 heads] += V^T W by mma.sync m16n8k16 in fp16 with
+// fp32 sums; both code formats are exact in fp16.  The order of the K axis of a product and of the columns is
+// free, so every lane's operand comes from the tile's rows in pieces of 16 bytes: lane (g, c) of the warp
+// (g = lane / 4, c = lane % 4) holds bytes 16 c .. 16 c + 15 of every 64 of keys g and g + 8, and columns 16 g ..
+// of values 2c, 2c + 1, 2c + 8, 2c + 9.  Q is brought to fp16 by a power of two per head.  W comes out of S with
+// positions along g and heads along c and is turned by movmatrix.
 // Weights: p = exp2(s - m), w = p * value scale / r with r the largest p * value scale so far, so that rows of
 // small and large scale keep their accuracy in fp16.  m and r only move when p or w grew by more than 2^8 or
 // 2^12.
@@ -233,13 +236,25 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Over the lanes of a quad (one g), and over those of one c.
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float column_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float column_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {  // of 16-bit values, two of a row per lane
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
 }
 
 // A tile in shared memory: 16 rows of key codes, 16 of value codes, 16 + 16 scales.  Rows are `pitch` bytes
@@ -257,7 +272,7 @@ struct CacheCols {
   static constexpr int KB = NB / 4, KR = NB % 4, V16 = NB / 8, V8 = NB % 8 / 4, V4 = NB % 4 / 2, V2 = NB % 2;
 };
 
-// Column of n-tile `n` (of 2 * NB) and its column index x (0 .. 7).
+// Column `n` (of 2 * NB) of lane g = x.
 template <int NB>
 __device__ __forceinline__ int value_column(int n, int x) {
   using C = CacheCols<NB>;
@@ -272,10 +287,10 @@ __device__ __forceinline__ int value_column(int n, int x) {
 
 template <int NB, int FMT, bool WIDE>  // WIDE: more than 8 query heads per key head
 __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(const PagedArgs a) {
-  extern __shared__ __align__(16) uint8_t paged_smem[];  // the warps' rings, then n_seqs + 1 prefixes
+  extern __shared__ __align__(16) uint8_t paged_smem[];  // the warps' rings, n_seqs + 1 prefixes, n_seqs lengths
   __shared__ long long s_warp[kPagedThreads / 32];
   using C = CacheCols<NB>;
-  constexpr int R = WIDE ? 2 : 1;  // rows of a lane: g and g + 8
+  constexpr int R = WIDE ? 2 : 1;  // blocks of 8 heads
   const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const PagedShape shape = paged_shape(a.heads, a.c.kv_heads, a.c.head_dim);
   const int per_seq = a.c.kv_heads * shape.blocks, d = a.c.head_dim;
@@ -283,6 +298,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
   const int units = shape.width >> 4;
   uint8_t *ring = paged_smem + (tid >> 5) * kPagedStages * stage_bytes;
   long long *s_prefix = reinterpret_cast<long long *>(paged_smem + (kPagedThreads / 32) * kPagedStages * stage_bytes);
+  int *s_seen = reinterpret_cast<int *>(s_prefix + a.n_seqs + 1);
   // copies of this lane: pieces lane, lane + 32, ... of 16 bytes of a tile's 16 rows
   int piece_at[(NB + 1) / 2], piece_row[(NB + 1) / 2];
 #pragma unroll
@@ -302,7 +318,9 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
   long long before = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += kPagedThreads) {
     const int s = s0 + tid;
-    long long upto = s < a.n_seqs ? (long long)((paged_seen(a, s) + 15) / 16) * per_seq : 0;
+    const int seen = s < a.n_seqs ? paged_seen(a, s) : 0;
+    if (s < a.n_seqs) s_seen[s] = seen;
+    long long upto = (long long)((seen + 15) / 16) * per_seq;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -337,200 +355,14 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
       if (s_prefix[mid] <= x) lo = mid;
       else hi = mid - 1;
     }
-    const int seq = lo, seen = paged_seen(a, seq), length = a.lengths[seq], n_tiles = (seen + 15) / 16;
+    const int seq = lo, seen = s_seen[seq], n_tiles = (seen + 15) / 16;
     const long long in_seq = x - s_prefix[seq];
-    const int which = (int)(in_seq / n_tiles), tile0 = (int)(in_seq % n_tiles);
+    const int which = in_seq <= 0x7fffffff ? (int)((uint32_t)in_seq / (uint32_t)n_tiles) : (int)(in_seq / n_tiles);
+    const int tile0 = (int)(in_seq - (long long)which * n_tiles);
     const long long seg_begin = x - tile0;
     const int tile1 = (int)min((long long)n_tiles, run_end - seg_begin);
     const int kv = which / shape.blocks, block = which % shape.blocks;
     const int head0 = kv * shape.group + block * 16, n_heads = min(16, shape.group - block * 16);
-
-    // ---- queries of the lane's rows in the order of the key bytes, brought to fp16
-    uint32_t qa[NB][2 * R];
-    float factor[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-      const bool live = g + 8 * r < n_heads;
-      const long long at = seq * a.q_row + (long long)(head0 + (live ? g + 8 * r : 0)) * a.q_head;
-      float v[NB][4], amax = 0.f;
-#pragma unroll
-      for (int n = 0; n < NB; n++) {
-        const int col = n < 4 * C::KB ? 64 * (n >> 2) + 16 * q + 4 * (n & 3) : 16 * n + 4 * q;
-        if (a.dtype == QMOE_BF16) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) v[n][i] = live && col + i < d ? to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.q)[at + col + i]) : 0.f;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; i++) v[n][i] = live && col + i < d ? to_f32(reinterpret_cast<const __half *>(a.q)[at + col + i]) : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(v[n][i]));
-      }
-      amax = quad_max(amax);
-      // 2^-e in two factors, either of which is a normal number
-      const int e = amax > 0.f && amax <= FLT_MAX ? ilogbf(amax) : 0;
-      const float down0 = scalbnf(1.f, -(e / 2)), down1 = scalbnf(1.f, -(e - e / 2));
-      factor[r] = scalbnf(a.scale * 1.4426950408889634f, e);
-#pragma unroll
-      for (int n = 0; n < NB; n++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const __half2 h = __floats2half2_rn(v[n][2 * i] * down0 * down1, v[n][2 * i + 1] * down0 * down1);
-          qa[n][i * R + r] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-    }
-
-    float o[2 * NB][4];
-#pragma unroll
-    for (int n = 0; n < 2 * NB; n++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[n][i] = 0.f;
-    float m[R], sum[R], unit[R], inv[R];  // maximum in units of log 2, sum of p, r, 1 / r
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-      m[r] = -INFINITY;
-      sum[r] = 0.f;
-      unit[r] = 0.f;
-      inv[r] = 0.f;
-    }
-    auto rescale = [&](int r, float by) {
-#pragma unroll
-      for (int n = 0; n < 2 * NB; n++) {
-        o[n][2 * r] *= by;
-        o[n][2 * r + 1] *= by;
-      }
-    };
-
-    auto process = [&](const uint8_t *keys, int tile) {
-      const uint8_t *values = keys + 16 * pitch;
-      const float *scales = reinterpret_cast<const float *>(keys + 32 * pitch);
-      const int pos0 = tile * 16;
-      float c[2][4];
-#pragma unroll
-      for (int n = 0; n < 2; n++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) c[n][i] = 0.f;
-        const uint8_t *row = keys + (8 * n + g) * pitch;
-        auto product = [&](int s, uint32_t word) {
-          uint32_t b0, b1;
-          codes_to_half<FMT>(word, b0, b1);
-          mma_16816(c[n], qa[s][0], WIDE ? qa[s][1] : 0u, qa[s][R], WIDE ? qa[s][2 * R - 1] : 0u, b0, b1);
-        };
-#pragma unroll
-        for (int b = 0; b < C::KB; b++) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(row + 64 * b + 16 * q);
-          product(4 * b, x.x);
-          product(4 * b + 1, x.y);
-          product(4 * b + 2, x.z);
-          product(4 * b + 3, x.w);
-        }
-#pragma unroll
-        for (int r = 0; r < C::KR; r++)
-          product(4 * C::KB + r, *reinterpret_cast<const uint32_t *>(row + 64 * C::KB + 16 * r + 4 * q));
-      }
-      const float2 ks0 = *reinterpret_cast<const float2 *>(scales + 2 * q), ks1 = *reinterpret_cast<const float2 *>(scales + 8 + 2 * q);
-      const float2 vs0 = *reinterpret_cast<const float2 *>(scales + 16 + 2 * q), vs1 = *reinterpret_cast<const float2 *>(scales + 24 + 2 * q);
-      const float ks[4] = {ks0.x, ks0.y, ks1.x, ks1.y}, vs[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
-      uint32_t w16[R][2];
-#pragma unroll
-      for (int r = 0; r < R; r++) {
-        float s[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = c[i >> 1][2 * r + (i & 1)] * (ks[i] * factor[r]);
-        if (a.bias != nullptr && g + 8 * r < n_heads) {
-          const float *bias = a.bias + (size_t)(head0 + g + 8 * r) * a.n_dist;
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            s[i] += paged_log2(__ldg(bias + max(0, min(length - 1 - (pos0 + 8 * (i >> 1) + 2 * q + (i & 1)), a.n_dist - 1))));
-        }
-        if (pos0 + 16 > seen) {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (pos0 + 8 * (i >> 1) + 2 * q + (i & 1) >= seen) s[i] = -INFINITY;
-        }
-        const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        if (__any_sync(0xffffffffu, top > m[r] + 8.f)) {
-          const float next = fmaxf(m[r], quad_max(top));
-          const float keep = next == -INFINITY ? 1.f : paged_exp2(m[r] - next);
-          m[r] = next;
-          sum[r] *= keep;
-          rescale(r, keep);
-        }
-        const float base = m[r] == -INFINITY ? 0.f : m[r];
-        float u[4], largest = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float p = paged_exp2(s[i] - base);
-          sum[r] += p;
-          u[i] = p != 0.f ? p * vs[i] : 0.f;  // weight 0: whatever the scale is
-          largest = fmaxf(largest, u[i]);
-        }
-        if (__any_sync(0xffffffffu, largest > unit[r] * 4096.f)) {
-          const float next = fmaxf(fmaxf(quad_max(largest), unit[r]), 0x1p-100f);
-          rescale(r, unit[r] / next);
-          unit[r] = next;
-          inv[r] = 1.f / next;
-        }
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const __half2 h = __floats2half2_rn(u[2 * n] * inv[r], u[2 * n + 1] * inv[r]);
-          w16[r][n] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-      }
-      auto product = [&](int n, uint32_t b0, uint32_t b1) {
-        mma_16816(o[n], w16[0][0], WIDE ? w16[R - 1][0] : 0u, w16[0][1], WIDE ? w16[R - 1][1] : 0u, b0, b1);
-      };
-      // words of the lane's four rows (positions 2c, 2c + 1, 2c + 8, 2c + 9): bytes of two rows side by side
-      auto products = [&](int n, int count, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
-        uint32_t p0, p1, r0, r1;
-        codes_to_half<FMT>(__byte_perm(v0, v1, 0x5140), p0, p1);
-        codes_to_half<FMT>(__byte_perm(v2, v3, 0x5140), r0, r1);
-        product(n, p0, r0);
-        product(n + 1, p1, r1);
-        if (count > 2) {
-          codes_to_half<FMT>(__byte_perm(v0, v1, 0x7362), p0, p1);
-          codes_to_half<FMT>(__byte_perm(v2, v3, 0x7362), r0, r1);
-          product(n + 2, p0, r0);
-          product(n + 3, p1, r1);
-        }
-      };
-      const uint8_t *row[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) row[r] = values + (8 * (r >> 1) + 2 * q + (r & 1)) * pitch;
-#pragma unroll
-      for (int b = 0; b < C::V16; b++) {
-        uint4 v[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          v[r] = *reinterpret_cast<const uint4 *>(row[r] + 128 * b + 16 * g);
-        products(16 * b, 4, v[0].x, v[1].x, v[2].x, v[3].x);
-        products(16 * b + 4, 4, v[0].y, v[1].y, v[2].y, v[3].y);
-        products(16 * b + 8, 4, v[0].z, v[1].z, v[2].z, v[3].z);
-        products(16 * b + 12, 4, v[0].w, v[1].w, v[2].w, v[3].w);
-      }
-      if (C::V8) {
-        const int off = 128 * C::V16 + 8 * g;
-        uint2 v[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint2 *>(row[r] + off);
-        products(16 * C::V16, 4, v[0].x, v[1].x, v[2].x, v[3].x);
-        products(16 * C::V16 + 4, 4, v[0].y, v[1].y, v[2].y, v[3].y);
-      }
-      if (C::V4) {
-        const int off = 128 * C::V16 + 64 * C::V8 + 4 * g;
-        uint32_t v[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint32_t *>(row[r] + off);
-        products(16 * C::V16 + 8 * C::V8, 4, v[0], v[1], v[2], v[3]);
-      }
-      if (C::V2) {
-        const int off = 128 * C::V16 + 64 * C::V8 + 32 * C::V4 + 2 * g;
-        uint32_t v[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint16_t *>(row[r] + off);
-        products(16 * C::V16 + 8 * C::V8 + 4 * C::V4, 2, v[0], v[1], v[2], v[3]);
-      }
-    };
 
     // ---- tiles, kPagedStages - 1 of them ahead on their way
     const int tiles_per_page = 1 << (a.c.page_shift - 4);
@@ -579,6 +411,207 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
     };
 #pragma unroll
     for (int i = 0; i < kPagedStages - 1; i++) load();
+
+    // ---- queries of the lane's rows in the order of the key bytes, brought to fp16
+    uint32_t qa[NB][2 * R];
+    float factor[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const bool live = g + 8 * r < n_heads;
+      const long long at = seq * a.q_row + (long long)(head0 + (live ? g + 8 * r : 0)) * a.q_head;
+      float v[NB][4], amax = 0.f;
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        const int col = n < 4 * C::KB ? 64 * (n >> 2) + 16 * q + 4 * (n & 3) : 16 * n + 4 * q;
+        if (a.dtype == QMOE_BF16) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[n][i] = live && col + i < d ? to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.q)[at + col + i]) : 0.f;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[n][i] = live && col + i < d ? to_f32(reinterpret_cast<const __half *>(a.q)[at + col + i]) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(v[n][i]));
+      }
+      amax = quad_max(amax);
+      // 2^-e in two factors, either of which is a normal number
+      const int e = amax > 0.f && amax <= FLT_MAX ? ilogbf(amax) : 0;
+      const float down0 = scalbnf(1.f, -(e / 2)), down1 = scalbnf(1.f, -(e - e / 2));
+      factor[r] = scalbnf(a.scale * 1.4426950408889634f, e);
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const __half2 h = __floats2half2_rn(v[n][2 * i] * down0 * down1, v[n][2 * i + 1] * down0 * down1);
+          qa[n][i * R + r] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+
+    // The lane's heads from here on: 2c and 2c + 1 of every block of 8.
+    float o[NB][R][4];  // two columns by two heads
+    float m[R][2], sum[R][2], unit[R][2], inv[R][2], by_head[R][2];  // maximum in units of log 2, sum of p, r, 1 / r
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[n][r][i] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        m[r][h] = -INFINITY;
+        sum[r][h] = unit[r][h] = inv[r][h] = 0.f;
+        by_head[r][h] = __shfl_sync(0xffffffffu, factor[r], 4 * (2 * q + h));
+      }
+    }
+    auto rescale = [&](int r, float by0, float by1) {
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        o[n][r][0] *= by0;
+        o[n][r][1] *= by1;
+        o[n][r][2] *= by0;
+        o[n][r][3] *= by1;
+      }
+    };
+
+    auto process = [&](const uint8_t *keys, int tile) {
+      const uint8_t *values = keys + 16 * pitch;
+      const float *scales = reinterpret_cast<const float *>(keys + 32 * pitch);
+      const int pos0 = tile * 16;
+      float c[R][4];
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[r][i] = 0.f;
+      auto scores = [&](int s, uint32_t key0, uint32_t key8) {
+        uint32_t a0, a1, a2, a3;
+        codes_to_half<FMT>(key0, a0, a2);
+        codes_to_half<FMT>(key8, a1, a3);
+#pragma unroll
+        for (int r = 0; r < R; r++) mma_16816(c[r], a0, a1, a2, a3, qa[s][r], qa[s][R + r]);
+      };
+#pragma unroll
+      for (int b = 0; b < C::KB; b++) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(keys + g * pitch + 64 * b + 16 * q);
+        const uint4 y = *reinterpret_cast<const uint4 *>(keys + (g + 8) * pitch + 64 * b + 16 * q);
+        scores(4 * b, x.x, y.x);
+        scores(4 * b + 1, x.y, y.y);
+        scores(4 * b + 2, x.z, y.z);
+        scores(4 * b + 3, x.w, y.w);
+      }
+#pragma unroll
+      for (int i = 0; i < C::KR; i++) {
+        const int off = 64 * C::KB + 16 * i + 4 * q;
+        scores(4 * C::KB + i, *reinterpret_cast<const uint32_t *>(keys + g * pitch + off),
+               *reinterpret_cast<const uint32_t *>(keys + (g + 8) * pitch + off));
+      }
+      const float ks0 = scales[g], ks8 = scales[g + 8], vs0 = scales[16 + g], vs8 = scales[24 + g];
+      uint32_t w16[R][2];
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        // [0] position g, head 2c  [1] position g, head 2c + 1  [2], [3] position g + 8
+        float s[4];
+        s[0] = c[r][0] * (ks0 * by_head[r][0]);
+        s[1] = c[r][1] * (ks0 * by_head[r][1]);
+        s[2] = c[r][2] * (ks8 * by_head[r][0]);
+        s[3] = c[r][3] * (ks8 * by_head[r][1]);
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int row = min(8 * r + 2 * q + (i & 1), n_heads - 1);
+            const int far = a.lengths[seq] - 1 - (pos0 + 8 * (i >> 1) + g);
+            s[i] += paged_log2(__ldg(a.bias + (size_t)(head0 + row) * a.n_dist + max(0, min(far, a.n_dist - 1))));
+          }
+        }
+        if (pos0 + 16 > seen) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (pos0 + 8 * (i >> 1) + g >= seen) s[i] = -INFINITY;
+        }
+        const float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
+        if (__any_sync(0xffffffffu, top0 > m[r][0] + 8.f || top1 > m[r][1] + 8.f)) {
+          const float next0 = fmaxf(m[r][0], column_max(top0)), next1 = fmaxf(m[r][1], column_max(top1));
+          const float keep0 = next0 == -INFINITY ? 1.f : paged_exp2(m[r][0] - next0);
+          const float keep1 = next1 == -INFINITY ? 1.f : paged_exp2(m[r][1] - next1);
+          m[r][0] = next0;
+          m[r][1] = next1;
+          sum[r][0] *= keep0;
+          sum[r][1] *= keep1;
+          rescale(r, keep0, keep1);
+        }
+        const float base0 = m[r][0] == -INFINITY ? 0.f : m[r][0], base1 = m[r][1] == -INFINITY ? 0.f : m[r][1];
+        const float p0 = paged_exp2(s[0] - base0), p1 = paged_exp2(s[1] - base1);
+        const float p2 = paged_exp2(s[2] - base0), p3 = paged_exp2(s[3] - base1);
+        sum[r][0] += p0 + p2;
+        sum[r][1] += p1 + p3;
+        // weight 0: whatever the scale is
+        const float u0 = p0 != 0.f ? p0 * vs0 : 0.f, u1 = p1 != 0.f ? p1 * vs0 : 0.f;
+        const float u2 = p2 != 0.f ? p2 * vs8 : 0.f, u3 = p3 != 0.f ? p3 * vs8 : 0.f;
+        const float large0 = fmaxf(u0, u2), large1 = fmaxf(u1, u3);
+        if (__any_sync(0xffffffffu, large0 > unit[r][0] * 4096.f || large1 > unit[r][1] * 4096.f)) {
+          const float next0 = fmaxf(fmaxf(column_max(large0), unit[r][0]), 0x1p-100f);
+          const float next1 = fmaxf(fmaxf(column_max(large1), unit[r][1]), 0x1p-100f);
+          rescale(r, unit[r][0] / next0, unit[r][1] / next1);
+          unit[r][0] = next0;
+          unit[r][1] = next1;
+          inv[r][0] = 1.f / next0;
+          inv[r][1] = 1.f / next1;
+        }
+        const __half2 h0 = __floats2half2_rn(u0 * inv[r][0], u1 * inv[r][1]);
+        const __half2 h8 = __floats2half2_rn(u2 * inv[r][0], u3 * inv[r][1]);
+        w16[r][0] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&h0));
+        w16[r][1] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&h8));
+      }
+      // words of the lane's four rows (positions 2c, 2c + 1, 2c + 8, 2c + 9): bytes of two rows side by side;
+      // two columns a product
+      auto products = [&](int n, int count, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+        uint32_t a0, a1, a2, a3;
+        codes_to_half<FMT>(__byte_perm(v0, v1, 0x5140), a0, a1);
+        codes_to_half<FMT>(__byte_perm(v2, v3, 0x5140), a2, a3);
+#pragma unroll
+        for (int r = 0; r < R; r++) mma_16816(o[n][r], a0, a1, a2, a3, w16[r][0], w16[r][1]);
+        if (count > 2) {
+          codes_to_half<FMT>(__byte_perm(v0, v1, 0x7362), a0, a1);
+          codes_to_half<FMT>(__byte_perm(v2, v3, 0x7362), a2, a3);
+#pragma unroll
+          for (int r = 0; r < R; r++) mma_16816(o[n + 1][r], a0, a1, a2, a3, w16[r][0], w16[r][1]);
+        }
+      };
+      const uint8_t *row[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) row[r] = values + (8 * (r >> 1) + 2 * q + (r & 1)) * pitch;
+#pragma unroll
+      for (int b = 0; b < C::V16; b++) {
+        uint4 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint4 *>(row[r] + 128 * b + 16 * g);
+        products(8 * b, 4, v[0].x, v[1].x, v[2].x, v[3].x);
+        products(8 * b + 2, 4, v[0].y, v[1].y, v[2].y, v[3].y);
+        products(8 * b + 4, 4, v[0].z, v[1].z, v[2].z, v[3].z);
+        products(8 * b + 6, 4, v[0].w, v[1].w, v[2].w, v[3].w);
+      }
+      if constexpr (C::V8 != 0) {
+        uint2 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint2 *>(row[r] + 128 * C::V16 + 8 * g);
+        products(8 * C::V16, 4, v[0].x, v[1].x, v[2].x, v[3].x);
+        products(8 * C::V16 + 2, 4, v[0].y, v[1].y, v[2].y, v[3].y);
+      }
+      if constexpr (C::V4 != 0) {
+        const int off = 128 * C::V16 + 64 * C::V8 + 4 * g;
+        uint32_t v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint32_t *>(row[r] + off);
+        products(8 * C::V16 + 4 * C::V8, 4, v[0], v[1], v[2], v[3]);
+      }
+      if constexpr (C::V2 != 0) {
+        const int off = 128 * C::V16 + 64 * C::V8 + 32 * C::V4 + 2 * g;
+        uint32_t v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint16_t *>(row[r] + off);
+        products(NB - 1, 2, v[0], v[1], v[2], v[3]);
+      }
+    };
+
     int stage = 0;
     for (int tile = tile0; tile < tile1; tile++) {
       load();
@@ -594,40 +627,32 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
     const bool whole = tile0 == 0 && tile1 == n_tiles;
     float *part = a.parts + (size_t)(2 * worker + (tile0 == 0 ? 1 : 0)) * shape.rows * row_floats;
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-      const int row = g + 8 * r;
-      const float l = quad_sum(sum[r]);
-      const float by = l == 0.f ? 0.f : unit[r] / l;
-      if (row >= n_heads) continue;
-      if (whole) {
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int row = 8 * r + 2 * q + h;
+        const float l = column_sum(sum[r][h]);
+        const float by = l == 0.f ? 0.f : unit[r][h] / l;
+        if (row >= n_heads) continue;
         const long long at = ((long long)seq * a.heads + head0 + row) * d;
-#pragma unroll
-        for (int n = 0; n < 2 * NB; n++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const int col = value_column<NB>(n, 2 * q + i);
-            if (col >= d) continue;
-            const float v = o[n][2 * r + i] * by;
-            if (a.dtype == QMOE_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[at + col] = from_f32<__nv_bfloat16>(v);
-            else reinterpret_cast<__half *>(a.out)[at + col] = from_f32<__half>(v);
-          }
-      } else {
         float *p = part + (size_t)row * row_floats;
-        if (q == 0) {
-          p[0] = m[r];
+        if (!whole && g == 0) {
+          p[0] = m[r][h];
           p[1] = l;
         }
 #pragma unroll
-        for (int n = 0; n < 2 * NB; n++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const int col = value_column<NB>(n, 2 * q + i);
-            if (col < d) p[2 + col] = o[n][2 * r + i] * by;
-          }
+        for (int n = 0; n < 2 * NB; n++) {
+          const int col = value_column<NB>(n, g);
+          if (col >= d) continue;
+          const float v = o[n >> 1][r][2 * (n & 1) + h] * by;
+          if (!whole) p[2 + col] = v;
+          else if (a.dtype == QMOE_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[at + col] = from_f32<__nv_bfloat16>(v);
+          else reinterpret_cast<__half *>(a.out)[at + col] = from_f32<__half>(v);
+        }
       }
-    }
     x = seg_begin + tile1;
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // One CTA per sequence and query head: joins the parts of the warps that share it, writes zeros for a
@@ -642,6 +667,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_decode_join(const PagedArgs a)
   const int kv = head / shape.group, block = head % shape.group / 16, row = head % shape.group % 16;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seen = paged_seen(a, seq), n_tiles = (seen + 15) / 16;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first kernel ends
   if (tid == 0 && head % shape.group == 0 && a.lengths[seq] > seen) atomicAdd(a.c.status, 1);
   auto store = [&](int col, float v) {
     const long long to = ((long long)seq * a.heads + head) * d + col;
@@ -879,7 +905,7 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = shape.group > 8, e4m3 = cache->format == QMOE_CACHE_E4M3;
-  const size_t smem = (size_t)(kPagedThreads / 32) * kPagedStages * paged_stage(paged_units(shape.width)) + sizeof(long long) * (size_t)(n_seqs + 1);
+  const size_t smem = (size_t)(kPagedThreads / 32) * kPagedStages * paged_stage(paged_units(shape.width)) + 12 * (size_t)(n_seqs + 1);
   const unsigned grid = (unsigned)(a.warps / (kPagedThreads / 32));
   auto run = [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
@@ -902,7 +928,18 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
     default: done = run(std::integral_constant<int, 16>()); break;
   }
   if (done != QMOE_OK) return done;
-  QMOE_LAUNCH(k_decode_join, (unsigned)(n_seqs * heads), kJoinThreads, (a.warps + 256 * (kJoinThreads / 32)) * sizeof(float), st, a);
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)(n_seqs * heads));
+  config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = (a.warps + 256 * (kJoinThreads / 32)) * sizeof(float);
+  config.stream = st;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  QMOE_CUDA(cudaLaunchKernelEx(&config, k_decode_join, a));
+  count_launch();
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
 }
