@@ -123,26 +123,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float in_log2(float b) { return b == -INFINITY ? b : fmaxf(b * kLog2e, -FLT_MAX); }
 
-// Two fp32 values in one 64-bit register: one instruction works on both.
-using pair_t = unsigned long long;
-__device__ __forceinline__ pair_t pair_of(float lo, float hi) {
-  pair_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ void pair_split(pair_t v, float &lo, float &hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ pair_t pair_fma(pair_t a, pair_t b, pair_t c) {
-  pair_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ pair_t pair_add(pair_t a, pair_t b) {
-  pair_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

@@ -27,41 +27,83 @@ __device__ __forceinline__ long long cache_slot(const CacheView &c, int seq, lon
   return (((long long)page * c.kv_heads) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
 }
 
-__device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ float from_e4m3(uint8_t c) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
 }
 
-// Code nearest to x / s, ties to the even code.  x * (1 / s) is within 2^-23 of the quotient, so it
-// decides unless a rounding border lies that near; then the sign of x - border * s, which one fused
-// multiply-add gives exactly, does.  (The border has 5 bits, s 24: both operands are scaled up where
-// their difference could leave the normal range.)
-__device__ __forceinline__ float beyond_border(float x, float s, float border) {
-  const float up = s < 1e-25f ? 1.8446744e19f : 1.f;  // 2^64
-  return fmaf(-border, s * up, x * up);
+// Four codes to two pairs of fp16: (bytes 0, 1) and (bytes 2, 3).  int8: 0x6400 + (code + 128) is 1024 +
+// code + 128 in fp16.
+template <int FMT>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  if (FMT == QMOE_CACHE_E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
+    lo = *reinterpret_cast<const uint32_t *>(&hx);
+    hi = *reinterpret_cast<const uint32_t *>(&hy);
+  }
+}
+
+// Codes nearest to x / s, ties to the even code, of four values of a row at once; `inv` is 1 / s to 2^-23.
+// Rounding the fp32 quotient would round twice, so the quotient is rounded to odd instead: q, one
+// Newton step from x * inv, is within one unit of its last place of the quotient, x - q * s is exact in one
+// fused multiply-add, and where it is not zero q is replaced by the neighbour with the last bit set on the
+// quotient's side.  That is never a rounding border, and lies on the quotient's side of every border. 
+// (A branch for quotients that look like borders is taken by most warps: s is a rounded amax / 448, so that many
+// quotients of 16-bit values lie within its rounding of a border.)
+struct RowScale {
+  float s, inv;
+};
+__device__ __forceinline__ uint32_t to_odd(float q, float rest, float x) {
+  const uint32_t bits = __float_as_uint(q);
+  const uint32_t moved = (bits + (uint32_t)((int)(__float_as_uint(rest) ^ __float_as_uint(x)) >> 31)) | 1u;  // 1 less: towards 0
+  return rest != 0.f ? moved : bits;
 }
 template <int FMT>
-__device__ __forceinline__ uint8_t quantise(float x, float s, float inv) {
-  const float q = x * inv;
-  if (FMT == QMOE_CACHE_E4M3) {
-    const uint8_t lo = to_e4m3(q * (1.f - 0x1p-21f)), hi = to_e4m3(q * (1.f + 0x1p-21f));
-    if (lo == hi) return lo;
-    const float r = beyond_border(x, s, 0.5f * (from_e4m3(lo) + from_e4m3(hi))) * copysignf(1.f, q);
-    return r > 0.f ? hi : (r < 0.f ? lo : ((lo & 1) ? hi : lo));
-  } else {
-    const float n = rintf(q);
-    int code = (int)n;
-    if (fabsf(fabsf(q - n) - 0.5f) < 0x1p-14f) {
-      const float f = floorf(q), r = beyond_border(x, s, f + 0.5f);
-      code = (int)f;
-      if (r > 0.f || (r == 0.f && (code & 1))) code++;
-    }
-    return (uint8_t)(int8_t)code;
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[4], const RowScale &r) {
+  const pair_t s_minus = pair_of(-r.s, -r.s), inv = pair_of(r.inv, r.inv);
+  float q[4], rest[4];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const pair_t x2 = pair_of(x[2 * i], x[2 * i + 1]), q0 = pair_mul(x2, inv);
+    const pair_t q2 = pair_fma(pair_fma(q0, s_minus, x2), inv, q0);
+    pair_split(q2, q[2 * i], q[2 * i + 1]);
+    pair_split(pair_fma(q2, s_minus, x2), rest[2 * i], rest[2 * i + 1]);
   }
+#pragma unroll
+  for (int i = 0; i < 4; i++) q[i] = __uint_as_float(to_odd(q[i], rest[i], x[i]));
+  if (FMT == QMOE_CACHE_E4M3) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(q[1]), "f"(q[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(q[3]), "f"(q[2]));
+    return __byte_perm(lo, hi, 0x5410);
+  }
+  // q + 1.5 * 2^23 holds the nearest integer in its low bits
+  uint32_t n[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) n[i] = __float_as_uint(q[i] + 12582912.f);
+  return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
 }
 template <int FMT>
 __device__ __forceinline__ float code_value(uint8_t c) {
   return FMT == QMOE_CACHE_E4M3 ? from_e4m3(c) : (float)(int8_t)c;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_values(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_values<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_values<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
 }
 
 struct RowsArgs {
@@ -70,80 +112,219 @@ struct RowsArgs {
   void *k_out, *v_out;   // read: destinations
   long long k_row, k_head, v_row, v_head;
   const int32_t *cu, *start;
-  int n_seqs;
+  int n_seqs, tokens;  // tokens of a CTA
+  uint32_t per_token_inverse;  // 2^32 / (2 * kv_heads), rounded up
   long long n_rows;
 };
 
-// One warp per row, head and tensor: four values per lane and step.
-template <typename T, int FMT>
-__global__ void __launch_bounds__(256) k_cache_append(const RowsArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int which = (int)(item & 1);
-  const int head = (int)((item >> 1) % a.c.kv_heads);
-  const long long row = (item >> 1) / a.c.kv_heads;
-  if (row >= a.n_rows) return;
-  const int seq = packed_seq(a.cu, a.n_seqs, (int)row);
-  if (seq < 0) return;
-  const long long slot0 = cache_slot(a.c, seq, (long long)a.start[seq] + (row - a.cu[seq]));
-  if (slot0 < 0) {
-    if (head == 0 && which == 0 && lane == 0) atomicAdd(a.c.status, 1);
-    return;
-  }
-  const long long slot = slot0 + ((long long)head << a.c.page_shift);
-  const T *src = which ? reinterpret_cast<const T *>(a.v) + row * a.v_row + head * a.v_head
-                       : reinterpret_cast<const T *>(a.k) + row * a.k_row + head * a.k_head;
-  const int d = a.c.head_dim, width = cache_row_bytes(d);
-  float x[2][4], amax = 0.f;
-  bool finite = true;
-#pragma unroll
-  for (int j = 0; j < 2; j++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int at = 128 * j + 4 * lane + i;
-      x[j][i] = at < d ? to_f32(src[at]) : 0.f;
-      finite = finite && fabsf(x[j][i]) <= FLT_MAX;
-      amax = fmaxf(amax, fabsf(x[j][i]));
+// Both directions are bounded by memory: 2 bytes read or written per value of the 16-bit side, 1 of the codes,
+// 4 per row for the scale; what is left to do is to spend few instructions on a value.  A CTA takes `tokens`
+// tokens with all their heads, keys and values: their places in the cache are looked up once, one thread a
+// token, then every thread moves pieces of 16 values.  A row of one head is shared by LANES neighbouring lanes
+// (a power of two), heads run fastest, so that 16-bit rows are read or written in order.
+// Where the 16-bit tensors' rows do not begin on 16-byte boundaries (VEC false) a warp moves them value by
+// value, neighbouring lanes neighbouring values, through shared memory: [row of the warp][16 * LANES values].
+constexpr int kRowsThreads = 256;
+constexpr int kRowsPieces = 8;  // of a thread, at most
+constexpr int kRowsTokens = 64;
+
+__host__ __device__ constexpr int row_lanes(int width) { return width <= 16 ? 1 : (width <= 32 ? 2 : (width <= 64 ? 4 : (width <= 128 ? 8 : 16))); }
+
+// Places of the CTA's tokens: index of (page, head 0, place); -1 without a valid page, -2 when nobody owns the
+// row.
+__device__ __forceinline__ void find_slots(const RowsArgs &a, long long *s_slot) {
+  if (threadIdx.x < a.tokens) {
+    const long long row = (long long)blockIdx.x * a.tokens + threadIdx.x;
+    long long slot = -2;
+    const int seq = row < a.n_rows ? packed_seq(a.cu, a.n_seqs, (int)row) : -1;
+    if (seq >= 0) {
+      slot = cache_slot(a.c, seq, (long long)a.start[seq] + (row - a.cu[seq]));
+      if (slot < 0) atomicAdd(a.c.status, 1);
     }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  finite = __all_sync(0xffffffffu, finite);
-  const float s = fmaxf(__fdiv_rn(amax, FMT == QMOE_CACHE_E4M3 ? 448.f : 127.f), kScaleFloor);
-  const float inv = __fdiv_rn(1.f, s);
-  uint8_t *dst = (which ? a.c.v_codes : a.c.k_codes) + slot * width;
-#pragma unroll
-  for (int j = 0; j < 2; j++) {
-    if (128 * j + 4 * lane >= width) break;
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) word |= (uint32_t)(finite ? quantise<FMT>(x[j][i], s, inv) : 0) << (8 * i);
-    *reinterpret_cast<uint32_t *>(dst + 128 * j + 4 * lane) = word;
+    s_slot[threadIdx.x] = slot;
   }
-  if (lane == 0) (which ? a.c.v_scale : a.c.k_scale)[slot] = finite ? s : __int_as_float(0x7fffffff);
+  __syncthreads();
 }
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(256) k_cache_read(const RowsArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int which = (int)(item & 1);
-  const int head = (int)((item >> 1) % a.c.kv_heads);
-  const long long row = (item >> 1) / a.c.kv_heads;
-  if (row >= a.n_rows) return;
-  const int seq = packed_seq(a.cu, a.n_seqs, (int)row);
-  if (seq < 0) return;
-  const long long slot0 = cache_slot(a.c, seq, (long long)a.start[seq] + (row - a.cu[seq]));
-  if (slot0 < 0 && head == 0 && which == 0 && lane == 0) atomicAdd(a.c.status, 1);
-  const long long slot = slot0 + ((long long)head << a.c.page_shift);
-  const int d = a.c.head_dim, width = cache_row_bytes(d);
-  const uint8_t *src = (which ? a.c.v_codes : a.c.k_codes) + slot * width;
-  const float s = slot0 < 0 ? 0.f : (which ? a.c.v_scale : a.c.k_scale)[slot];
-  T *dst = reinterpret_cast<T *>(which ? a.v_out : a.k_out) + (row * a.c.kv_heads + head) * d;
-  for (int at = 4 * lane; at < d; at += 128) {
-    const uint32_t word = slot0 < 0 ? 0u : *reinterpret_cast<const uint32_t *>(src + at);
+// Row `r` of the CTA's (token, key or value, head) rows.
+struct CacheRow {
+  long long row, slot;
+  int head;
+  bool is_v;
+};
+__device__ __forceinline__ CacheRow cache_row(const RowsArgs &a, const long long *s_slot, int r) {
+  CacheRow c;
+  const int token = (int)__umulhi((uint32_t)r, a.per_token_inverse), in_token = r - token * 2 * a.c.kv_heads;
+  c.is_v = in_token >= a.c.kv_heads;
+  c.head = in_token - (c.is_v ? a.c.kv_heads : 0);
+  c.row = (long long)blockIdx.x * a.tokens + token;
+  c.slot = token < a.tokens ? s_slot[token] : -2;
+  if (c.slot >= 0) c.slot += (long long)c.head << a.c.page_shift;
+  return c;
+}
+
+__device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t v, __nv_bfloat16) {
+  const uint32_t u = v & 0x7fff7fffu;
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&m), *reinterpret_cast<const __nv_bfloat162 *>(&u));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t v, __half) {
+  const uint32_t u = v & 0x7fff7fffu;
+  const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2 *>(&m), *reinterpret_cast<const __half2 *>(&u));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <typename T>
+__device__ __forceinline__ float2 pair_values(uint32_t v);
+template <>
+__device__ __forceinline__ float2 pair_values<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 pair_values<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+
+template <typename T, int FMT, int LANES, bool VEC>
+__global__ void __launch_bounds__(kRowsThreads) k_cache_append(const RowsArgs a) {
+  constexpr int kPerWarp = 32 / LANES;
+  __shared__ long long s_slot[kRowsTokens];
+  __shared__ __align__(16) T s_rows[VEC ? 1 : kRowsThreads / 32][VEC ? 1 : 512];
+  const int lane = threadIdx.x & 31, at = 16 * (lane % LANES);
+  const int d = a.c.head_dim, width = cache_row_bytes(d), rows = a.tokens * 2 * a.c.kv_heads;
+  find_slots(a, s_slot);
+  auto source = [&](const CacheRow &c) {
+    return c.is_v ? reinterpret_cast<const T *>(a.v) + c.row * a.v_row + c.head * a.v_head
+                  : reinterpret_cast<const T *>(a.k) + c.row * a.k_row + c.head * a.k_head;
+  };
+  auto finish = [&](const CacheRow &c, const uint4 (&v)[2]) {
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (at + i < d) dst[at + i] = from_f32<T>(code_value<FMT>((uint8_t)(word >> (8 * i))) * s);
+    for (int i = 0; i < 8; i++) m = abs_max2(m, w[i], T());
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) m = abs_max2(m, __shfl_xor_sync(0xffffffffu, m, o), T());
+    const float2 m2 = pair_values<T>(m);
+    const bool finite = m2.x <= FLT_MAX && m2.y <= FLT_MAX;  // NaN and infinity stay in the maximum
+    if (c.slot < 0 || at >= width) return;
+    RowScale r;
+    r.s = fmaxf(__fdiv_rn(fmaxf(m2.x, m2.y), FMT == QMOE_CACHE_E4M3 ? 448.f : 127.f), kScaleFloor);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));  // s is a normal number, and so is 1 / s
+    const float stored = r.s;
+    const bool tiny = r.s < 1e-25f;  // remainders would leave the normal range: all of it 2^64 times as large
+    if (tiny) {
+      r.inv *= 0x1p-64f;
+      r.s *= 0x1p64f;
+    }
+    uint32_t codes[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 p = pair_values<T>(w[2 * i]), q = pair_values<T>(w[2 * i + 1]);
+      float x[4] = {p.x, p.y, q.x, q.y};
+      if (tiny) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] *= 0x1p64f;
+      }
+      codes[i] = finite ? quantise4<FMT>(x, r) : 0u;
+    }
+    *reinterpret_cast<uint4 *>((c.is_v ? a.c.v_codes : a.c.k_codes) + c.slot * width + at) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    if (at == 0) (c.is_v ? a.c.v_scale : a.c.k_scale)[c.slot] = finite ? stored : __int_as_float(0x7fffffff);
+  };
+  if (VEC) {
+    // two pieces at a time: both loads are under way before the first is used
+    for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += 2 * kRowsThreads / LANES) {
+      const int r0 = base + lane / LANES;
+      CacheRow c[2];
+      uint4 v[2][2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        c[b] = cache_row(a, s_slot, r0 + b * (kRowsThreads / LANES));
+        v[b][0] = v[b][1] = make_uint4(0u, 0u, 0u, 0u);
+        const T *src = source(c[b]) + at;
+        if (c[b].slot >= 0 && at + 16 <= d) {
+          v[b][0] = __ldg(reinterpret_cast<const uint4 *>(src));
+          v[b][1] = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
+        } else if (c[b].slot >= 0) {
+          T *to = reinterpret_cast<T *>(v[b]);
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (at + i < d) to[i] = src[i];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; b++) finish(c[b], v[b]);
+    }
+  } else {
+    T *stage = s_rows[threadIdx.x >> 5];
+    for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += kRowsThreads / LANES) {
+      const CacheRow c = cache_row(a, s_slot, base + lane / LANES);
+      const T *src = source(c);
+#pragma unroll
+      for (int i = 0; i < kPerWarp; i++) {
+        const T *from = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, (unsigned long long)src, i * LANES));
+        const bool in = __shfl_sync(0xffffffffu, (int)(c.slot >= 0), i * LANES);
+        for (int col = lane; col < 16 * LANES; col += 32) stage[i * 16 * LANES + col] = in && col < d ? from[col] : from_f32<T>(0.f);
+      }
+      __syncwarp();
+      const uint4 *from = reinterpret_cast<const uint4 *>(stage + (lane / LANES) * 16 * LANES + at);
+      const uint4 v[2] = {from[0], from[1]};
+      finish(c, v);
+      __syncwarp();
+    }
+  }
+}
+
+template <typename T, int FMT, int LANES, bool VEC>
+__global__ void __launch_bounds__(kRowsThreads) k_cache_read(const RowsArgs a) {
+  constexpr int kPerWarp = 32 / LANES;
+  __shared__ long long s_slot[kRowsTokens];
+  __shared__ __align__(16) T s_rows[VEC ? 1 : kRowsThreads / 32][VEC ? 1 : 512];
+  const int lane = threadIdx.x & 31, at = 16 * (lane % LANES);
+  const int d = a.c.head_dim, width = cache_row_bytes(d), rows = a.tokens * 2 * a.c.kv_heads;
+  find_slots(a, s_slot);
+  for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += 2 * kRowsThreads / LANES) {  // uniform in a warp
+    const int r0 = base + lane / LANES;
+    CacheRow c[2];
+    uint4 codes[2];
+    float scale[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      c[b] = cache_row(a, s_slot, r0 + b * (kRowsThreads / LANES));
+      codes[b] = make_uint4(0u, 0u, 0u, 0u);
+      scale[b] = 0.f;
+      if (c[b].slot >= 0 && at < width) {
+        codes[b] = __ldg(reinterpret_cast<const uint4 *>((c[b].is_v ? a.c.v_codes : a.c.k_codes) + c[b].slot * width + at));
+        scale[b] = __ldg((c[b].is_v ? a.c.v_scale : a.c.k_scale) + c[b].slot);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const uint32_t w[4] = {codes[b].x, codes[b].y, codes[b].z, codes[b].w};
+      T *dst = reinterpret_cast<T *>(c[b].is_v ? a.v_out : a.k_out) + (c[b].row * a.c.kv_heads + c[b].head) * d;
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t lo, hi;
+        codes_to_half<FMT>(w[i], lo, hi);
+        const float2 x = pair_values<__half>(lo), y = pair_values<__half>(hi);
+        v[2 * i] = pack_values<T>(x.x * scale[b], x.y * scale[b]);
+        v[2 * i + 1] = pack_values<T>(y.x * scale[b], y.y * scale[b]);
+      }
+      if (!VEC) {
+        T *stage = s_rows[threadIdx.x >> 5];
+        uint4 *to = reinterpret_cast<uint4 *>(stage + (lane / LANES) * 16 * LANES + at);
+        to[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        to[1] = make_uint4(v[4], v[5], v[6], v[7]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPerWarp; i++) {
+          T *out = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, (unsigned long long)dst, i * LANES));
+          const bool owned = __shfl_sync(0xffffffffu, (int)(c[b].slot != -2), i * LANES);
+          for (int col = lane; owned && col < d; col += 32) out[col] = stage[i * 16 * LANES + col];
+        }
+        __syncwarp();
+      } else if (c[b].slot != -2) {  // d is a multiple of 8
+        if (at + 8 <= d) *reinterpret_cast<uint4 *>(dst + at) = make_uint4(v[0], v[1], v[2], v[3]);
+        if (at + 16 <= d) *reinterpret_cast<uint4 *>(dst + at + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+      }
+    }
   }
 }
 
@@ -210,23 +391,6 @@ __device__ __forceinline__ float paged_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Four codes to two pairs of fp16: (bytes 0, 1) and (bytes 2, 3).  int8: 0x6400 + (code + 128) is 1024 +
-// code + 128 in fp16.
-template <int FMT>
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  if (FMT == QMOE_CACHE_E4M3) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-        : "=r"(lo), "=r"(hi) : "r"(w));
-  } else {
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
-    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
-    lo = *reinterpret_cast<const uint32_t *>(&hx);
-    hi = *reinterpret_cast<const uint32_t *>(&hy);
-  }
 }
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -794,18 +958,44 @@ static int cache_view(const char *fn, const qmoe_quant_cache *cache, const int32
 
 using namespace qmoe;
 
-#define QMOE_CACHE_DISPATCH(kernel, dtype, format, grid, block, stream, args)                                  \
-  do {                                                                                                         \
-    if ((dtype) == QMOE_BF16 && (format) == QMOE_CACHE_E4M3)                                                   \
-      QMOE_LAUNCH((kernel<__nv_bfloat16, QMOE_CACHE_E4M3>), grid, block, 0, stream, args);                     \
-    else if ((dtype) == QMOE_BF16)                                                                             \
-      QMOE_LAUNCH((kernel<__nv_bfloat16, QMOE_CACHE_INT8>), grid, block, 0, stream, args);                     \
-    else if ((format) == QMOE_CACHE_E4M3)                                                                      \
-      QMOE_LAUNCH((kernel<__half, QMOE_CACHE_E4M3>), grid, block, 0, stream, args);                            \
-    else                                                                                                       \
-      QMOE_LAUNCH((kernel<__half, QMOE_CACHE_INT8>), grid, block, 0, stream, args);                            \
-    QMOE_CUDA(cudaGetLastError());                                                                             \
-  } while (0)
+// Launches a row kernel for the activations' type, the code format, the lanes that share a row and the
+// alignment of the 16-bit tensors.
+#define QMOE_ROWS_KERNELS(kernel, T, FMT, vec)                                                                  \
+  (lanes == 1   ? (vec ? kernel<T, FMT, 1, true> : kernel<T, FMT, 1, false>)                                    \
+   : lanes == 2 ? (vec ? kernel<T, FMT, 2, true> : kernel<T, FMT, 2, false>)                                    \
+   : lanes == 4 ? (vec ? kernel<T, FMT, 4, true> : kernel<T, FMT, 4, false>)                                    \
+   : lanes == 8 ? (vec ? kernel<T, FMT, 8, true> : kernel<T, FMT, 8, false>)                                    \
+                : (vec ? kernel<T, FMT, 16, true> : kernel<T, FMT, 16, false>))
+template <bool READ>
+static int run_rows(RowsArgs a, int dtype, int format, bool vec, int device, cudaStream_t stream) {
+  const int lanes = row_lanes(cache_row_bytes(a.c.head_dim));
+  // tokens of a CTA: what gives its threads kRowsPieces pieces each, fewer where the GPU would not be filled
+  const long long pieces = 2LL * a.c.kv_heads * lanes, fill = (a.n_rows + 8 * sm_count(device) - 1) / (8 * sm_count(device));
+  long long tokens = kRowsPieces * kRowsThreads / pieces;
+  tokens = tokens < fill ? tokens : fill;
+  a.tokens = (int)(tokens < 1 ? 1 : (tokens > kRowsTokens ? kRowsTokens : tokens));
+  a.per_token_inverse = (uint32_t)(((1ull << 32) + 2 * a.c.kv_heads - 1) / (2 * a.c.kv_heads));
+  const dim3 grid((unsigned)((a.n_rows + a.tokens - 1) / a.tokens));
+  void (*kernel)(RowsArgs);
+  if (READ) {
+    if (dtype == QMOE_BF16)
+      kernel = format == QMOE_CACHE_E4M3 ? QMOE_ROWS_KERNELS(k_cache_read, __nv_bfloat16, QMOE_CACHE_E4M3, vec)
+                                         : QMOE_ROWS_KERNELS(k_cache_read, __nv_bfloat16, QMOE_CACHE_INT8, vec);
+    else
+      kernel = format == QMOE_CACHE_E4M3 ? QMOE_ROWS_KERNELS(k_cache_read, __half, QMOE_CACHE_E4M3, vec)
+                                         : QMOE_ROWS_KERNELS(k_cache_read, __half, QMOE_CACHE_INT8, vec);
+  } else {
+    if (dtype == QMOE_BF16)
+      kernel = format == QMOE_CACHE_E4M3 ? QMOE_ROWS_KERNELS(k_cache_append, __nv_bfloat16, QMOE_CACHE_E4M3, vec)
+                                         : QMOE_ROWS_KERNELS(k_cache_append, __nv_bfloat16, QMOE_CACHE_INT8, vec);
+    else
+      kernel = format == QMOE_CACHE_E4M3 ? QMOE_ROWS_KERNELS(k_cache_append, __half, QMOE_CACHE_E4M3, vec)
+                                         : QMOE_ROWS_KERNELS(k_cache_append, __half, QMOE_CACHE_INT8, vec);
+  }
+  QMOE_LAUNCH(kernel, grid, kRowsThreads, 0, stream, a);
+  QMOE_CUDA(cudaGetLastError());
+  return QMOE_OK;
+}
 
 extern "C" {
 
@@ -829,13 +1019,15 @@ int qmoe_cache_append(const qmoe_quant_cache *cache, const void *k_dev, const vo
   a.start = start_dev;
   a.n_seqs = n_seqs;
   a.n_rows = n_rows;
-  const int64_t items = 2 * n_rows * cache->kv_heads;
-  QMOE_REQUIRE(items <= 8LL * 0x7fffffffLL, "too many rows");
+  if (cache->kv_heads > 1024) {
+    set_error("%s: at most 1024 key heads", __func__);
+    return QMOE_ERR_UNSUPPORTED;
+  }
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
-  QMOE_CACHE_DISPATCH(k_cache_append, dtype, cache->format, (unsigned)((items + 7) / 8), 256,
-                      reinterpret_cast<cudaStream_t>(stream), a);
-  return QMOE_OK;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_dev) | reinterpret_cast<uintptr_t>(v_dev) |
+                         (uintptr_t)(2 * (k_row | k_head | v_row | v_head));
+  return run_rows<false>(a, dtype, cache->format, (bits & 15u) == 0, device, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_dev, const int32_t *cu_dev,
@@ -853,13 +1045,14 @@ int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_
   a.start = start_dev;
   a.n_seqs = n_seqs;
   a.n_rows = n_rows;
-  const int64_t items = 2 * n_rows * cache->kv_heads;
-  QMOE_REQUIRE(items <= 8LL * 0x7fffffffLL, "too many rows");
+  if (cache->kv_heads > 1024) {
+    set_error("%s: at most 1024 key heads", __func__);
+    return QMOE_ERR_UNSUPPORTED;
+  }
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
-  QMOE_CACHE_DISPATCH(k_cache_read, dtype, cache->format, (unsigned)((items + 7) / 8), 256,
-                      reinterpret_cast<cudaStream_t>(stream), a);
-  return QMOE_OK;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_out_dev) | reinterpret_cast<uintptr_t>(v_out_dev);
+  return run_rows<true>(a, dtype, cache->format, (bits & 15u) == 0 && cache->head_dim % 8 == 0, device, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int head_dim, int device) {

@@ -45,6 +45,32 @@ __device__ __forceinline__ int packed_seq(const int32_t *__restrict__ cu, int n_
   return lo;
 }
 
+// Two fp32 values in one 64-bit register: one instruction works on both.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair_of(float lo, float hi) {
+  pair_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void pair_split(pair_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ pair_t pair_fma(pair_t a, pair_t b, pair_t c) {
+  pair_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ pair_t pair_add(pair_t a, pair_t b) {
+  pair_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ pair_t pair_mul(pair_t a, pair_t b) {
+  pair_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 __host__ __device__ constexpr int cache_row_bytes(int head_dim) { return (head_dim + 15) & ~15; }
 
 }  // namespace qmoe
