@@ -21,7 +21,7 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
-from . import sub1, synth
+from . import serving, sub1, synth
 
 
 class ReplicatedTokenMoE:
@@ -276,8 +276,117 @@ class SwitchDecoderLM:
                             "decode_s": t_end - t_capture, "decode_steps": n_new - 1}
         return torch.cat(out)
 
+    # ---- several sequences at once -------------------------------------------------------------------
+    def start_batch(self, prompts: List[torch.Tensor], n_new: int, cache_format: str = "e4m3",
+                    page_size: int = 64) -> "BatchState":
+        """Prefill ``prompts`` (int64 id vectors of any lengths) as one packed batch: causal attention within
+        every prompt, keys and values into paged 8-bit caches (one per block, one page table for all) with
+        room for ``n_new`` more tokens per sequence.  ``state.logits`` fp32 ``[n, vocab]`` are those behind
+        the prompts.  All tokens of a step count as one sequence for the router's capacity rule."""
+        lens = [int(p.numel()) for p in prompts]
+        if not lens or min(lens) < 1:
+            raise ValueError("start_batch needs at least one prompt, and no empty one")
+        if n_new < 0 or max(lens) + n_new > self.max_len:
+            raise ValueError(f"prompt and new tokens must fit max_len = {self.max_len}")
+        state = BatchState(self, lens, n_new, cache_format, page_size)
+        x = self.embed[torch.cat([p.reshape(-1) for p in prompts]).to(self.dev)]
+        n = x.shape[0]
+        for b, cache in zip(self.blocks, state.caches):
+            qkv = (_rms_norm(x, b["ln1"]) @ b["wqkv"].t()).view(n, 3, self.h, self.hd)
+            q, k, v = qkv.unbind(1)
+            att = serving.prompt_attention(q, k, v, state.cu)
+            serving.cache_append(cache, k, v, state.cu, state.start, state.table)
+            x = x + att.view(n, -1) @ b["wo"].t()
+            x = x + b["moe"](_rms_norm(x, b["ln2"]).contiguous())
+        last = x[state.cu[1:].long() - 1]
+        state.logits = (_rms_norm(last, self.final_norm) @ self.lm_head.t()).float()
+        return state
+
+    def step_batch(self, state: "BatchState", tokens: torch.Tensor) -> torch.Tensor:
+        """One more token (int64[n]) for every sequence of ``state``; returns the logits fp32 ``[n, vocab]``
+        behind them.  The position is ``state.lengths``, which the caller moves on (``+= 1``), so that the call
+        can be captured and replayed."""
+        x = self.embed[tokens]
+        n = x.shape[0]
+        seen = state.lengths + 1
+        for b, cache in zip(self.blocks, state.caches):
+            q, k, v = (sub1.rms_norm(x, b["ln1"]) @ b["wqkv"].t()).view(n, 3, self.h, self.hd).unbind(1)
+            serving.cache_append(cache, k, v, state.one_each, state.lengths, state.table)
+            att = serving.decode_attention_paged(q, cache, state.table, seen)
+            x = x + att.view(n, -1) @ b["wo"].t()
+            x = x + b["moe"](sub1.rms_norm(x, b["ln2"]))
+        return (sub1.rms_norm(x, self.final_norm) @ self.lm_head.t()).float()
+
+    def generate_batch(self, prompts: List[torch.Tensor], n_new: int, temperature: float = 0.0, top_k: int = 0,
+                       top_p: float = 1.0, min_p: float = 0.0, uniform: Optional[torch.Tensor] = None,
+                       cache_format: str = "e4m3", page_size: int = 64, use_graph: bool = True) -> torch.Tensor:
+        """``n_new`` tokens for every prompt, int64 ``[n, n_new]``.  Tokens are sampled as
+        :func:`qmoe_b200.serving.sample_tokens` does (``temperature`` 0: the largest logit) from ``uniform``
+        fp32 ``[n_new, n]``, by default torch's generator of the device.  The decoding step is captured into
+        a CUDA graph for this call when there are enough steps."""
+        if n_new < 1:
+            raise ValueError("n_new must be at least 1")
+        n = len(prompts)
+        if uniform is None:
+            uniform = torch.rand((n_new, n), device=self.dev)
+        if uniform.shape != (n_new, n) or uniform.dtype != torch.float32:
+            raise ValueError(f"uniform must be fp32 [{n_new}, {n}], got {uniform.dtype} {tuple(uniform.shape)}")
+        uniform = uniform.to(self.dev).contiguous()
+        fixed = {"temperature": torch.full((n,), temperature, dtype=torch.float32, device=self.dev),
+                 "top_k": torch.full((n,), top_k, dtype=torch.int32, device=self.dev),
+                 "top_p": torch.full((n,), top_p, dtype=torch.float32, device=self.dev),
+                 "min_p": torch.full((n,), min_p, dtype=torch.float32, device=self.dev)}
+        state = self.start_batch(prompts, n_new, cache_format, page_size)
+        tokens = serving.sample_tokens(state.logits, uniform[0], **fixed)
+        out = [tokens.clone()]
+        u = torch.empty(n, dtype=torch.float32, device=self.dev)
+
+        def step(ids: torch.Tensor) -> torch.Tensor:
+            return serving.sample_tokens(self.step_batch(state, ids), u, **fixed)
+
+        graph = None
+        if use_graph and n_new > 4:
+            from .graph import GraphedStep
+            u.copy_(uniform[1])
+            graph = GraphedStep(step, tokens)        # its warm-up runs write what the first step writes again
+        try:
+            for i in range(1, n_new):
+                u.copy_(uniform[i])
+                tokens = step(tokens) if graph is None else graph(tokens)
+                out.append(tokens.clone())
+                state.lengths += 1
+            torch.cuda.synchronize(self.dev)
+        finally:
+            if graph is not None:
+                graph.close()
+        refused = sum(c.refused() for c in state.caches)
+        if refused:
+            raise RuntimeError(f"{refused} cache positions had no page")
+        return torch.stack(out, 1)
+
     def close(self) -> None:
         """Destroy the captured decode graph (before tearing down a process group it captured)."""
         if self._graph is not None:
             self._graph.close()
             self._graph = None
+
+
+class BatchState:
+    """Caches and positions of the sequences of one :meth:`SwitchDecoderLM.start_batch`: a
+    :class:`qmoe_b200.serving.QuantCache` per block, ``table`` int32 ``[n, pages]``, ``lengths`` int32[n] =
+    positions filled (the caller adds 1 after every :meth:`SwitchDecoderLM.step_batch`)."""
+
+    def __init__(self, model: SwitchDecoderLM, lens: List[int], n_new: int, cache_format: str, page_size: int):
+        dev = model.dev
+        pages = [-(-(n + n_new) // page_size) for n in lens]
+        rows, first = [], 0
+        for count in pages:
+            rows.append(list(range(first, first + count)) + [-1] * (max(pages) - count))
+            first += count
+        self.table = torch.tensor(rows, dtype=torch.int32, device=dev)
+        self.caches = [serving.QuantCache(first, page_size, model.h, model.hd, dev, fmt=cache_format) for _ in model.blocks]
+        self.cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+        self.start = torch.zeros(len(lens), dtype=torch.int32, device=dev)
+        self.one_each = torch.arange(len(lens) + 1, dtype=torch.int32, device=dev)
+        self.lengths = torch.tensor(lens, dtype=torch.int32, device=dev)
+        self.logits: Optional[torch.Tensor] = None
