@@ -420,7 +420,12 @@ int qmoe_decode_attention_ex(const void *qkv_dev, void *k_cache_dev, void *v_cac
 #define QMOE_CACHE_E4M3 0
 #define QMOE_CACHE_INT8 1
 
-typedef struct qmoe_prompt_shape {
+typedef struct qmoe_prompt_args {
+  const void *q_dev, *k_dev, *v_dev;
+  void *out_dev;
+  const int32_t *cu_q_dev, *cu_k_dev;
+  const float *rel_bias_dev;
+  void *work_dev;
   int64_t total_q, total_k;                     /* rows of q / out and of k / v */
   int64_t q_row, q_head, k_row, k_head;         /* strides */
   int64_t v_row, v_head, out_row, out_head;
@@ -428,7 +433,7 @@ typedef struct qmoe_prompt_shape {
   int32_t dtype;
   int32_t n_dist;                               /* columns of the relative bias (0: none) */
   float scale;                                  /* <= 0: 1 / sqrt(head_dim) */
-} qmoe_prompt_shape;
+} qmoe_prompt_args;
 
 /* Causal attention over a packed batch of prompts.  Sequence s has n = cu_q[s + 1] - cu_q[s] queries
  * and m = cu_k[s + 1] - cu_k[s] keys; query i sees keys 0 .. i + m - n (its own position when n = m;
@@ -438,10 +443,11 @@ typedef struct qmoe_prompt_shape {
  * with bias = rel_bias_dev[h * n_dist + min(distance, n_dist - 1)] (fp32, may be NULL), the distance
  * being i + m - n - j: the one-directional relative bias of T5 / Switch (scale 1).  Statistics and
  * sums are fp32.  At most 262140 query rows and 32768 sequences a call.  A wait of the tensor-core kernel
- * that runs out is counted by qmoe_moe_tile_timeouts. */
-int qmoe_prompt_attention(const void *q_dev, const void *k_dev, const void *v_dev, void *out_dev,
-                          const int32_t *cu_q_dev, const int32_t *cu_k_dev, const float *rel_bias_dev,
-                          const qmoe_prompt_shape *shape, int device, void *stream);
+ * that runs out is counted by qmoe_moe_tile_timeouts.  work_dev: qmoe_prompt_work_bytes bytes for the same
+ * arguments (0 where every row of q, k and v begins on a 16-byte boundary), 256-byte aligned, not shared by
+ * calls that may overlap. */
+int64_t qmoe_prompt_work_bytes(const qmoe_prompt_args *args);
+int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, void *stream);
 
 /* A paged cache whose keys and values are held in 8 bits.  codes: [n_pages][kv_heads][page_size]
  * [row_bytes], row_bytes = head_dim rounded up to 16, the padding zero; scales: fp32
@@ -461,13 +467,16 @@ typedef struct qmoe_quant_cache {
  * >= max_pages * page_size) or on a page number outside [0, n_pages) is refused: *status_dev is
  * incremented once per row, nothing is written to the cache, and a row read from there is zero.  Pages
  * that are written must belong to one sequence; pages that are only read may be shared. */
-int qmoe_cache_append(const qmoe_quant_cache *cache, const void *k_dev, const void *v_dev, int64_t k_row,
-                      int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *cu_dev,
-                      const int32_t *start_dev, const int32_t *page_table_dev, int32_t *status_dev, int n_seqs,
-                      int max_pages, int64_t n_rows, int dtype, int device, void *stream);
-int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_dev, const int32_t *cu_dev,
-                    const int32_t *start_dev, const int32_t *page_table_dev, int32_t *status_dev, int n_seqs,
-                    int max_pages, int64_t n_rows, int dtype, int device, void *stream);
+typedef struct qmoe_cache_rows {
+  void *k_dev, *v_dev;                          /* read from by append, written by read */
+  int64_t k_row, k_head, v_row, v_head;         /* strides (append) */
+  const int32_t *cu_dev, *start_dev, *page_table_dev;
+  int32_t *status_dev;
+  int64_t n_rows;
+  int32_t n_seqs, max_pages, dtype;
+} qmoe_cache_rows;
+int qmoe_cache_append(const qmoe_quant_cache *cache, const qmoe_cache_rows *rows, int device, void *stream);
+int qmoe_cache_read(const qmoe_quant_cache *cache, const qmoe_cache_rows *rows, int device, void *stream);
 
 /* Attention of one new token per sequence over such a cache: q_dev [n_seqs][heads][head_dim], out_dev
  * contiguous of the same shape, lengths_dev int32 [n_seqs] = positions to attend to (the new token's
@@ -475,12 +484,21 @@ int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_
  * length - 1 - position.  Positions without a valid page are left out and counted in *status_dev: once
  * per 16 positions and key head on a bad page number, once per sequence and key head for all positions
  * behind max_pages * page_size.  work_dev: qmoe_decode_paged_work_bytes bytes, 16-byte
- * aligned, not shared by calls that may overlap.  At most 4096 sequences a call. */
+ * aligned, not shared by calls that may overlap.  At most 4096 sequences a call.
+ * heads is a multiple of the cache's kv_heads. */
 int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int head_dim, int device);
-int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev, int64_t q_row, int64_t q_head,
-                                void *out_dev, const int32_t *page_table_dev, const int32_t *lengths_dev,
-                                const float *rel_bias_dev, int n_dist, int32_t *status_dev, void *work_dev, int n_seqs,
-                                int heads, int max_pages, float scale, int dtype, int device, void *stream);
+typedef struct qmoe_paged_args {
+  const void *q_dev;
+  void *out_dev;
+  const int32_t *page_table_dev, *lengths_dev;
+  const float *rel_bias_dev;
+  int32_t *status_dev;
+  void *work_dev;
+  int64_t q_row, q_head;
+  int32_t n_dist, n_seqs, heads, max_pages, dtype;
+  float scale;
+} qmoe_paged_args;
+int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const qmoe_paged_args *args, int device, void *stream);
 
 /* One token per row of logits [rows][vocab] (fp32, bf16 or fp16, rows row_stride apart), vocab <=
  * 262144.  Per row, all device arrays of `rows` entries, each may be NULL but uniform:
@@ -495,9 +513,17 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev
  * are exp((l - max) / temperature) held as 64-bit multiples of 2^-45, so that sums do not depend on
  * their order.  A row without a distribution (a NaN or +inf among the logits, all of them -inf, a
  * temperature that is negative or not finite) gives token -1 and logprob NaN. */
-int qmoe_sample(const void *logits_dev, int64_t row_stride, int rows, int vocab, int dtype, const float *temperature_dev,
-                const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev, const float *uniform_dev,
-                int64_t *tokens_dev, float *logprob_dev, int device, void *stream);
+typedef struct qmoe_sample_args {
+  const void *logits_dev;
+  const float *temperature_dev;
+  const int32_t *top_k_dev;
+  const float *top_p_dev, *min_p_dev, *uniform_dev;
+  int64_t *tokens_dev;
+  float *logprob_dev;
+  int64_t row_stride;
+  int32_t rows, vocab, dtype;
+} qmoe_sample_args;
+int qmoe_sample(const qmoe_sample_args *args, int device, void *stream);
 
 /* Number of kernels this library has launched in the calling process (all devices, all entry points). */
 int64_t qmoe_launch_count(void);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional
 
 from . import build as _build
@@ -55,21 +56,18 @@ class InterleavedStore(ctypes.Structure):
                 ("dec", ctypes.c_void_p), ("rows", ctypes.c_void_p)]
 
 
-class PromptShape(ctypes.Structure):
-    """Mirror of ``qmoe_prompt_shape``."""
-
-    _fields_ = [(name, ctypes.c_int64) for name in
-                ("total_q", "total_k", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")] \
-        + [(name, ctypes.c_int32) for name in ("n_seqs", "heads", "kv_heads", "head_dim", "dtype", "n_dist")] \
-        + [("scale", ctypes.c_float)]
-
-
 class QuantCacheDesc(ctypes.Structure):
     """Mirror of ``qmoe_quant_cache``."""
 
     _fields_ = [(name, ctypes.c_void_p) for name in ("k_codes", "v_codes", "k_scale", "v_scale")] \
         + [(name, ctypes.c_int32) for name in ("n_pages", "page_size", "kv_heads", "head_dim", "format")]
 
+
+# Packed layouts of the argument structures, pointers as unsigned integers.
+PROMPT_ARGS = struct.Struct("8Q10q6if4x")     # qmoe_prompt_args
+CACHE_ROWS = struct.Struct("2Q4q4Qq3i4x")     # qmoe_cache_rows
+PAGED_ARGS = struct.Struct("7Q2q5if")         # qmoe_paged_args
+SAMPLE_ARGS = struct.Struct("8Qq3i4x")        # qmoe_sample_args
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -120,12 +118,14 @@ SIGNATURES = {
     "qmoe_gemv": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_float, _I, _I, _P]),
     "qmoe_decode_attention": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "qmoe_decode_attention_ex": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, ctypes.c_float, _P, _P, _I, _P]),
-    "qmoe_prompt_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
-    "qmoe_cache_append": (_I, [_P, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P]),
-    "qmoe_cache_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P]),
+    # the argument structures are passed as packed bytes: one argument is converted instead of twenty
+    "qmoe_prompt_work_bytes": (_L, [ctypes.c_char_p]),
+    "qmoe_prompt_attention": (_I, [ctypes.c_char_p, _I, _P]),
+    "qmoe_cache_append": (_I, [_P, ctypes.c_char_p, _I, _P]),
+    "qmoe_cache_read": (_I, [_P, ctypes.c_char_p, _I, _P]),
     "qmoe_decode_paged_work_bytes": (_L, [_I, _I, _I, _I, _I]),
-    "qmoe_decode_attention_paged": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, ctypes.c_float, _I, _I, _P]),
-    "qmoe_sample": (_I, [_P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
+    "qmoe_decode_attention_paged": (_I, [_P, ctypes.c_char_p, _I, _P]),
+    "qmoe_sample": (_I, [ctypes.c_char_p, _I, _P]),
     "qmoe_sub1_code_histogram": (_I, [_P, _L, _P, _I, _P]),
     "qmoe_sub1_remap_tables": (_I, [_P, _P, _P, _P, _I, _P]),
     "qmoe_moe_combine": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),

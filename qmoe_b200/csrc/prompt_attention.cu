@@ -14,7 +14,7 @@ struct PromptArgs {
   void *out;
   const int32_t *cu_q, *cu_k;
   const float *bias;
-  qmoe_prompt_shape s;
+  qmoe_prompt_args s;
 };
 
 // One query row of one head by one warp, keys one after another with a running maximum; 32 lanes share
@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // tensor core works for the other.
 // Every tile lies in shared memory as rows of 64 columns (128 bytes) under the 128-byte swizzle, one block
 // of 128 rows per 64 columns: K-major for Q and K, and the same bytes with the head axis contiguous for V.
-// Tiles come by bulk tensor copies where the tensors allow a tensor map (rows on 16-byte boundaries), else
-// and at a sequence's last, partial key tile by the copying warps, which write zeros behind the last row.
+// Tiles come by bulk tensor copies, a sequence's last, partial key tile by the copying warps, which write zeros
+// behind the last row.  Tensors that no tensor map describes are packed first.
 // The running maximum is only moved when it grew by more than 2^8: O then stays as it is and P and the
 // sum are taken relative to the older maximum, which is exact up to rounding since both are scaled alike.
 // P is rounded to the type of the inputs for the second product (half a step of it relative to every
@@ -166,48 +166,52 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Rows [0, rows) of a tile from global memory (`pitch` elements apart), zeros behind them and behind the
-// head's values up to 8 * chunks columns.  `aligned`: every row begins on a 16-byte boundary (asynchronous
-// 16-byte copies, to be waited for by the caller).
+// Rows [0, rows) of a tile from global memory (`pitch` elements apart, on 16-byte boundaries), zeros behind them
+// and behind the head's values up to 8 * chunks columns: asynchronous copies, to be waited for by the caller.
 __device__ __forceinline__ uint32_t tile_offset(int row, int unit) {
   return (uint32_t)((unit >> 3) * kBlockBytes + row * 128 + (((unit & 7) ^ (row & 7)) << 4));
 }
 template <typename T, int THREADS>
-__device__ __forceinline__ void load_tile(uint8_t *tile, const T *src, long long pitch, int rows, int d, int chunks,
-                                          bool aligned, int tid) {
-  if (aligned) {
-    const uint32_t base = smem_u32(tile);
-    const int shift = chunks > 8 ? 4 : (chunks > 4 ? 3 : 2);
-    const int c = tid & ((1 << shift) - 1);
-    if (c >= chunks) return;
-    const int bytes = max(min(16, 2 * (d - 8 * c)), 0);
+__device__ __forceinline__ void load_tile(uint8_t *tile, const T *src, long long pitch, int rows, int d, int chunks, int tid) {
+  const uint32_t base = smem_u32(tile);
+  const int shift = chunks > 8 ? 4 : (chunks > 4 ? 3 : 2);
+  const int c = tid & ((1 << shift) - 1);
+  if (c >= chunks) return;
+  const int bytes = max(min(16, 2 * (d - 8 * c)), 0);
 #pragma unroll 8
-    for (int r = tid >> shift; r < kTileRows; r += THREADS >> shift)
-      cp_async16(base + tile_offset(r, c), r < rows ? src + r * pitch + 8 * c : src, r < rows ? bytes : 0);
-    return;
-  }
-  constexpr int kWarps = THREADS / 32, kBatch = kTileRows / kWarps < 16 ? kTileRows / kWarps : 16;
-  const int lane = tid & 31;
-  for (int c0 = 0; c0 < 8 * chunks; c0 += 32) {
-    const int c = c0 + lane;
-    if (c >= 8 * chunks) continue;
-    for (int r0 = tid >> 5; r0 < kTileRows; r0 += kBatch * kWarps) {
-      T v[kBatch];
+  for (int r = tid >> shift; r < kTileRows; r += THREADS >> shift)
+    cp_async16(base + tile_offset(r, c), r < rows ? src + r * pitch + 8 * c : src, r < rows ? bytes : 0);
+}
+
+// Copies of tensors whose rows do not begin on 16-byte boundaries, as [rows][heads][pitch] with pitch = head_dim
+// rounded up to 8 (what stands behind the head's values is not read).  A pass over the inputs is little next to
+// the attention itself; copying such rows value by value inside it was slower even for one tile of 128 queries
+// (25 us against PACKED us for 32 heads of 65).
+struct PackArgs {
+  const void *src[3];
+  void *dst[3];
+  long long row[3], head[3], rows[3];
+  int heads[3], d, pitch;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) k_prompt_pack(const PackArgs a) {
+  const int which = blockIdx.y, units = a.pitch / 8;
+  if (a.dst[which] == nullptr) return;
+  const long long n = a.rows[which] * a.heads[which] * units;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long item = i / units, row = item / a.heads[which];
+    const int unit = (int)(i - item * units), head = (int)(item - row * a.heads[which]);
+    const T *src = reinterpret_cast<const T *>(a.src[which]) + row * a.row[which] + head * a.head[which] + 8 * unit;
+    __align__(16) T v[8];
 #pragma unroll
-      for (int i = 0; i < kBatch; i++) {
-        const int r = r0 + i * kWarps;
-        v[i] = c < d && r < rows ? src[r * pitch + c] : from_f32<T>(0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; i++)
-        *reinterpret_cast<T *>(tile + tile_offset(r0 + i * kWarps, c >> 3) + 2 * (c & 7)) = v[i];
-    }
+    for (int x = 0; x < 8; x++) v[x] = 8 * unit + x < a.d ? src[x] : from_f32<T>(0.f);
+    reinterpret_cast<uint4 *>(a.dst[which])[i] = *reinterpret_cast<const uint4 *>(v);
   }
 }
 
 template <typename T, bool BIAS>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    const bool aligned, const bool tma) {
+                                                                    const bool tma) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // the swizzle repeats every 1024 bytes
   __shared__ PromptBars s_bar;
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       const int r = row0 + i * kTileRows;
       load_tile<T, kPromptThreads>(q_tile + i * tile_bytes,
                                    reinterpret_cast<const T *>(a.q) + (rq.x + (r < n ? r : 0)) * a.s.q_row + head * a.s.q_head,
-                                   a.s.q_row, max(0, min(kTileRows, n - r)), d, chunks, aligned, tid);
+                                   a.s.q_row, max(0, min(kTileRows, n - r)), d, chunks, tid);
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         const long long pitch = is_v ? a.s.v_row : a.s.k_row;
         const T *src = reinterpret_cast<const T *>(is_v ? a.v : a.k) + (rk.x + (long long)key0) * pitch +
                        kv * (is_v ? a.s.v_head : a.s.k_head);
-        load_tile<T, kTileRows>(ring + stage * tile_bytes, src, pitch, min(kTileRows, m - key0), d, chunks, aligned, t);
+        load_tile<T, kTileRows>(ring + stage * tile_bytes, src, pitch, min(kTileRows, m - key0), d, chunks, t);
         cp_async_commit();
         cp_async_wait<0>();
         fence_async_proxy();
@@ -526,38 +530,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       tc_fence_after();
     }
     if (ok) {
-      T *out = reinterpret_cast<T *>(a.out) + (rq.x + (long long)(live ? row : 0)) * a.s.out_row + head * a.s.out_head;
-      const bool vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.s.out_row * 2)) & 15u) == 0;
+      // Rows go through shared memory (the query tile's, which nothing reads any more) so that a warp writes
+      // them one after another instead of one piece of 32 rows at a time.
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      uint8_t *stage = q_tile + i * tile_bytes;
       bool finite = true;
       for (int c = 0; c < o_cols; c += 16) {
-        uint32_t o[16];
+        uint32_t o[16], w[8];
         if (steps[i] > 0) {
           tmem_ld16(t_o + c, o);
         } else {
 #pragma unroll
           for (int x = 0; x < 16; x++) o[x] = 0u;
         }
-        float v[16];
 #pragma unroll
-        for (int x = 0; x < 16; x++) {
-          v[x] = __uint_as_float(o[x]) * inv;
-          finite = finite && fabsf(v[x]) <= FLT_MAX;
+        for (int x = 0; x < 8; x++) {
+          const float lo = __uint_as_float(o[2 * x]) * inv, hi = __uint_as_float(o[2 * x + 1]) * inv;
+          finite = finite && fabsf(lo) <= FLT_MAX && fabsf(hi) <= FLT_MAX;
+          w[x] = pack2<T>(lo, hi);
         }
-        if (live && vec && c + 16 <= d) {
-          uint4 w[2];
-          uint32_t *p = reinterpret_cast<uint32_t *>(w);
-#pragma unroll
-          for (int x = 0; x < 8; x++) p[x] = pack2<T>(v[2 * x], v[2 * x + 1]);
-          *reinterpret_cast<uint4 *>(out + c) = w[0];
-          *reinterpret_cast<uint4 *>(out + c + 8) = w[1];
-        } else if (live) {
-#pragma unroll
-          for (int x = 0; x < 16; x++)
-            if (c + x < d) out[c + x] = from_f32<T>(v[x]);
-        }
-        __syncwarp();
+        *reinterpret_cast<uint4 *>(stage + tile_offset(t, c >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(stage + tile_offset(t, (c >> 3) + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
       }
+      __syncwarp();
+      const int t0 = t & ~31, rows = min(32, n - (row0 + i * kTileRows + t0));  // of this warp
+      T *out = reinterpret_cast<T *>(a.out) + (rq.x + (long long)(row0 + i * kTileRows + t0)) * a.s.out_row + head * a.s.out_head;
+      if (((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.s.out_row * 2) | (uintptr_t)(d * 2)) & 15u) == 0) {
+        const int units = d / 8, shift = units > 8 ? 4 : (units > 4 ? 3 : 2), u = lane & ((1 << shift) - 1);
+        for (int r = lane >> shift; r < rows && u < units; r += 32 >> shift)
+          *reinterpret_cast<uint4 *>(out + r * a.s.out_row + 8 * u) = *reinterpret_cast<const uint4 *>(stage + tile_offset(t0 + r, u));
+      } else {
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          for (int c = lane; c < d; c += 32) {
+            T v[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) v[r] = *reinterpret_cast<const T *>(stage + tile_offset(t0 + r0 + r, c >> 3) + 2 * (c & 7));
+#pragma unroll
+            for (int r = 0; r < 8; r++)
+              if (r0 + r < rows) out[(r0 + r) * a.s.out_row + c] = v[r];
+          }
+        }
+      }
+      __syncwarp();
       unsigned again = __ballot_sync(0xffffffffu, live && !finite);
       while (again != 0) {
         const int l = __ffs(again) - 1;
@@ -609,20 +623,53 @@ static bool make_map(CUtensorMap *map, const void *base, int dtype, int d, int h
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Whether a tensor has to be packed before the tiles can be copied: rows off 16-byte boundaries, or a stride that
+// a tensor map does not take (0: one head broadcast to all).
+static bool needs_packing(const void *base, int64_t rows, int heads, int64_t row, int64_t head) {
+  if (rows <= 0) return false;
+  const bool row_ok = rows == 1 || (row > 0 && row % 8 == 0 && row < (1LL << 38)), head_ok = heads == 1 || (head > 0 && head % 8 == 0 && head < (1LL << 38));
+  return (reinterpret_cast<uintptr_t>(base) & 15u) != 0 || !row_ok || !head_ok;
+}
+static int64_t packed_bytes(int64_t rows, int heads, int d) { return (rows * heads * ((d + 7) / 8 * 16) + 255) / 256 * 256; }
+
 template <typename T>
-static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
+static int run_prompt(PromptArgs a, void *work, cudaStream_t stream) {
   if (a.s.head_dim > kTileRows) {
     const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 3) / 4));
     QMOE_LAUNCH((k_prompt_rows<T>), grid, 128, 0, stream, a);
     QMOE_CUDA(cudaGetLastError());
     return QMOE_OK;
   }
-  // 16-byte copies where every row of q, k and v begins on a 16-byte boundary, else element by element
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
-                         (uintptr_t)(2 * (a.s.q_row | a.s.q_head | a.s.k_row | a.s.k_head | a.s.v_row | a.s.v_head));
-  const bool aligned = (bits & 15u) == 0;
+  // tensors that need it are packed first
+  PackArgs pack{};
+  pack.d = a.s.head_dim;
+  pack.pitch = (a.s.head_dim + 7) / 8 * 8;
+  uint8_t *at = reinterpret_cast<uint8_t *>(work);
+  long long largest = 0;
+  auto prepare = [&](int i, const void *&base, int64_t rows, int heads, int64_t &row, int64_t &head) {
+    if (!needs_packing(base, rows, heads, row, head)) return;
+    pack.src[i] = base;
+    pack.dst[i] = at;
+    pack.row[i] = row;
+    pack.head[i] = head;
+    pack.rows[i] = rows;
+    pack.heads[i] = heads;
+    base = at;
+    head = pack.pitch;
+    row = (int64_t)heads * pack.pitch;
+    at += packed_bytes(rows, heads, a.s.head_dim);
+    largest = largest > rows * heads * (pack.pitch / 8) ? largest : rows * heads * (pack.pitch / 8);
+  };
+  prepare(0, a.q, a.s.total_q, a.s.heads, a.s.q_row, a.s.q_head);
+  prepare(1, a.k, a.s.total_k, a.s.kv_heads, a.s.k_row, a.s.k_head);
+  prepare(2, a.v, a.s.total_k, a.s.kv_heads, a.s.v_row, a.s.v_head);
+  if (largest > 0) {
+    const long long blocks = (largest + 255) / 256;
+    QMOE_LAUNCH((k_prompt_pack<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384), 3), 256, 0, stream, pack);
+    QMOE_CUDA(cudaGetLastError());
+  }
   PromptMaps maps{};
-  const bool tma = aligned && make_map(&maps.q, a.q, a.s.dtype, a.s.head_dim, a.s.heads, a.s.total_q, a.s.q_head, a.s.q_row) &&
+  const bool tma = make_map(&maps.q, a.q, a.s.dtype, a.s.head_dim, a.s.heads, a.s.total_q, a.s.q_head, a.s.q_row) &&
                    make_map(&maps.k, a.k, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.k_head, a.s.k_row) &&
                    make_map(&maps.v, a.v, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.v_head, a.s.v_row);
   const int smem = (2 + kStages) * ((a.s.head_dim + 63) / 64) * kBlockBytes + 1024;
@@ -635,7 +682,7 @@ static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
   }
   QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 2 * kTileRows - 1) / (2 * kTileRows) + a.s.n_seqs));
-  QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, maps, aligned, tma);
+  QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, maps, tma);
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
 }
@@ -644,26 +691,36 @@ static int run_prompt(const PromptArgs &a, cudaStream_t stream) {
 
 using namespace qmoe;
 
-extern "C" int qmoe_prompt_attention(const void *q_dev, const void *k_dev, const void *v_dev, void *out_dev,
-                                     const int32_t *cu_q_dev, const int32_t *cu_k_dev, const float *rel_bias_dev,
-                                     const qmoe_prompt_shape *shape, int device, void *stream) {
-  QMOE_REQUIRE(shape != nullptr && cu_q_dev && cu_k_dev, "null pointer");
-  PromptArgs a{q_dev, k_dev, v_dev, out_dev, cu_q_dev, cu_k_dev, rel_bias_dev, *shape};
+extern "C" int64_t qmoe_prompt_work_bytes(const qmoe_prompt_args *args) {
+  if (args == nullptr || args->head_dim > kTileRows || args->head_dim < 1) return 0;
+  const qmoe_prompt_args &s = *args;
+  int64_t bytes = 0;
+  if (needs_packing(s.q_dev, s.total_q, s.heads, s.q_row, s.q_head)) bytes += packed_bytes(s.total_q, s.heads, s.head_dim);
+  if (needs_packing(s.k_dev, s.total_k, s.kv_heads, s.k_row, s.k_head)) bytes += packed_bytes(s.total_k, s.kv_heads, s.head_dim);
+  if (needs_packing(s.v_dev, s.total_k, s.kv_heads, s.v_row, s.v_head)) bytes += packed_bytes(s.total_k, s.kv_heads, s.head_dim);
+  return bytes;
+}
+
+extern "C" int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, void *stream) {
+  QMOE_REQUIRE(args != nullptr && args->cu_q_dev && args->cu_k_dev, "null pointer");
+  PromptArgs a{args->q_dev, args->k_dev, args->v_dev, args->out_dev, args->cu_q_dev, args->cu_k_dev, args->rel_bias_dev, *args};
   QMOE_REQUIRE(a.s.n_seqs >= 0 && a.s.total_q >= 0 && a.s.total_k >= 0, "negative size");
   QMOE_REQUIRE(a.s.heads >= 1 && a.s.kv_heads >= 1 && a.s.heads % a.s.kv_heads == 0 && a.s.head_dim >= 1,
                "heads must be a positive multiple of kv_heads");
   QMOE_REQUIRE(a.s.dtype == QMOE_BF16 || a.s.dtype == QMOE_FP16, "q, k and v are bf16 or fp16");
-  QMOE_REQUIRE((rel_bias_dev == nullptr) == (a.s.n_dist == 0) && a.s.n_dist >= 0, "bias and n_dist do not agree");
+  QMOE_REQUIRE((a.bias == nullptr) == (a.s.n_dist == 0) && a.s.n_dist >= 0, "bias and n_dist do not agree");
   QMOE_REQUIRE(isfinite(a.s.scale), "scale is not finite");
   if (a.s.n_seqs == 0 || a.s.total_q == 0) return QMOE_OK;
-  QMOE_REQUIRE(q_dev && out_dev && (a.s.total_k == 0 || (k_dev && v_dev)), "null device pointer");
+  QMOE_REQUIRE(a.q && a.out && (a.s.total_k == 0 || (a.k && a.v)), "null device pointer");
   if (a.s.head_dim > 256 || a.s.total_q > (1 << 18) - 4 || a.s.total_k > 0x7fffffffLL || a.s.n_seqs > 32768) {
     set_error("%s: head_dim <= 256, 262140 query rows, 2^31 - 1 key rows and 32768 sequences are supported", __func__);
     return QMOE_ERR_UNSUPPORTED;
   }
+  QMOE_REQUIRE(qmoe_prompt_work_bytes(args) == 0 || (args->work_dev != nullptr && (reinterpret_cast<uintptr_t>(args->work_dev) & 255u) == 0),
+               "workspace is missing or not 256-byte aligned");
   if (a.s.scale <= 0.f) a.s.scale = 1.f / sqrtf((float)a.s.head_dim);
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return a.s.dtype == QMOE_BF16 ? run_prompt<__nv_bfloat16>(a, st) : run_prompt<__half>(a, st);
+  return a.s.dtype == QMOE_BF16 ? run_prompt<__nv_bfloat16>(a, args->work_dev, st) : run_prompt<__half>(a, args->work_dev, st);
 }

@@ -997,62 +997,54 @@ static int run_rows(RowsArgs a, int dtype, int format, bool vec, int device, cud
   return QMOE_OK;
 }
 
-extern "C" {
-
-int qmoe_cache_append(const qmoe_quant_cache *cache, const void *k_dev, const void *v_dev, int64_t k_row,
-                      int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *cu_dev,
-                      const int32_t *start_dev, const int32_t *page_table_dev, int32_t *status_dev, int n_seqs,
-                      int max_pages, int64_t n_rows, int dtype, int device, void *stream) {
+template <bool READ>
+static int rows_entry(const char *fn, const qmoe_quant_cache *cache, const qmoe_cache_rows *rows, int device, void *stream) {
+  if (rows == nullptr) {
+    set_error("%s: null pointer", fn);
+    return QMOE_ERR_INVALID_ARG;
+  }
   RowsArgs a{};
-  const int rc = cache_view(__func__, cache, page_table_dev, status_dev, n_seqs, max_pages, dtype, &a.c);
+  const int rc = cache_view(fn, cache, rows->page_table_dev, rows->status_dev, rows->n_seqs, rows->max_pages, rows->dtype, &a.c);
   if (rc != QMOE_OK) return rc;
-  QMOE_REQUIRE(n_rows >= 0 && n_rows <= 0x7fffffffLL, "bad number of rows");
-  if (n_rows == 0 || n_seqs == 0) return QMOE_OK;
-  QMOE_REQUIRE(k_dev && v_dev && cu_dev && start_dev, "null device pointer");
-  a.k = k_dev;
-  a.v = v_dev;
-  a.k_row = k_row;
-  a.k_head = k_head;
-  a.v_row = v_row;
-  a.v_head = v_head;
-  a.cu = cu_dev;
-  a.start = start_dev;
-  a.n_seqs = n_seqs;
-  a.n_rows = n_rows;
+  if (rows->n_rows < 0 || rows->n_rows > 0x7fffffffLL) {
+    set_error("%s: bad number of rows", fn);
+    return QMOE_ERR_INVALID_ARG;
+  }
+  if (rows->n_rows == 0 || rows->n_seqs == 0) return QMOE_OK;
+  if (!rows->k_dev || !rows->v_dev || !rows->cu_dev || !rows->start_dev) {
+    set_error("%s: null device pointer", fn);
+    return QMOE_ERR_INVALID_ARG;
+  }
   if (cache->kv_heads > 1024) {
-    set_error("%s: at most 1024 key heads", __func__);
+    set_error("%s: at most 1024 key heads", fn);
     return QMOE_ERR_UNSUPPORTED;
   }
+  a.k = a.k_out = rows->k_dev;
+  a.v = a.v_out = rows->v_dev;
+  a.k_row = rows->k_row;
+  a.k_head = rows->k_head;
+  a.v_row = rows->v_row;
+  a.v_head = rows->v_head;
+  a.cu = rows->cu_dev;
+  a.start = rows->start_dev;
+  a.n_seqs = rows->n_seqs;
+  a.n_rows = rows->n_rows;
+  // 16-byte accesses to the 16-bit tensors where every row begins on a 16-byte boundary
+  uintptr_t bits = reinterpret_cast<uintptr_t>(rows->k_dev) | reinterpret_cast<uintptr_t>(rows->v_dev);
+  bits |= READ ? (uintptr_t)(2 * cache->head_dim) : (uintptr_t)(2 * (a.k_row | a.k_head | a.v_row | a.v_head));
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_dev) | reinterpret_cast<uintptr_t>(v_dev) |
-                         (uintptr_t)(2 * (k_row | k_head | v_row | v_head));
-  return run_rows<false>(a, dtype, cache->format, (bits & 15u) == 0, device, reinterpret_cast<cudaStream_t>(stream));
+  return run_rows<READ>(a, rows->dtype, cache->format, (bits & 15u) == 0, device, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int qmoe_cache_read(const qmoe_quant_cache *cache, void *k_out_dev, void *v_out_dev, const int32_t *cu_dev,
-                    const int32_t *start_dev, const int32_t *page_table_dev, int32_t *status_dev, int n_seqs,
-                    int max_pages, int64_t n_rows, int dtype, int device, void *stream) {
-  RowsArgs a{};
-  const int rc = cache_view(__func__, cache, page_table_dev, status_dev, n_seqs, max_pages, dtype, &a.c);
-  if (rc != QMOE_OK) return rc;
-  QMOE_REQUIRE(n_rows >= 0 && n_rows <= 0x7fffffffLL, "bad number of rows");
-  if (n_rows == 0 || n_seqs == 0) return QMOE_OK;
-  QMOE_REQUIRE(k_out_dev && v_out_dev && cu_dev && start_dev, "null device pointer");
-  a.k_out = k_out_dev;
-  a.v_out = v_out_dev;
-  a.cu = cu_dev;
-  a.start = start_dev;
-  a.n_seqs = n_seqs;
-  a.n_rows = n_rows;
-  if (cache->kv_heads > 1024) {
-    set_error("%s: at most 1024 key heads", __func__);
-    return QMOE_ERR_UNSUPPORTED;
-  }
-  DeviceGuard guard(device);
-  if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_out_dev) | reinterpret_cast<uintptr_t>(v_out_dev);
-  return run_rows<true>(a, dtype, cache->format, (bits & 15u) == 0 && cache->head_dim % 8 == 0, device, reinterpret_cast<cudaStream_t>(stream));
+extern "C" {
+
+int qmoe_cache_append(const qmoe_quant_cache *cache, const qmoe_cache_rows *rows, int device, void *stream) {
+  return rows_entry<false>(__func__, cache, rows, device, stream);
+}
+
+int qmoe_cache_read(const qmoe_quant_cache *cache, const qmoe_cache_rows *rows, int device, void *stream) {
+  return rows_entry<true>(__func__, cache, rows, device, stream);
 }
 
 int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int head_dim, int device) {
@@ -1062,38 +1054,37 @@ int64_t qmoe_decode_paged_work_bytes(int n_seqs, int heads, int kv_heads, int he
   return prefix + (int64_t)paged_warps(shape.width, device) * 2 * shape.rows * (shape.width + 2) * 4;
 }
 
-int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const void *q_dev, int64_t q_row, int64_t q_head,
-                                void *out_dev, const int32_t *page_table_dev, const int32_t *lengths_dev,
-                                const float *rel_bias_dev, int n_dist, int32_t *status_dev, void *work_dev, int n_seqs,
-                                int heads, int max_pages, float scale, int dtype, int device, void *stream) {
+int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const qmoe_paged_args *args, int device, void *stream) {
+  QMOE_REQUIRE(args != nullptr, "null pointer");
+  const int n_seqs = args->n_seqs, heads = args->heads;
   PagedArgs a{};
-  const int rc = cache_view(__func__, cache, page_table_dev, status_dev, n_seqs, max_pages, dtype, &a.c);
+  const int rc = cache_view(__func__, cache, args->page_table_dev, args->status_dev, n_seqs, args->max_pages, args->dtype, &a.c);
   if (rc != QMOE_OK) return rc;
   QMOE_REQUIRE(heads >= 1 && heads % cache->kv_heads == 0, "heads must be a positive multiple of kv_heads");
-  QMOE_REQUIRE((rel_bias_dev == nullptr) == (n_dist == 0) && n_dist >= 0, "bias and n_dist do not agree");
-  QMOE_REQUIRE(isfinite(scale), "scale is not finite");
+  QMOE_REQUIRE((args->rel_bias_dev == nullptr) == (args->n_dist == 0) && args->n_dist >= 0, "bias and n_dist do not agree");
+  QMOE_REQUIRE(isfinite(args->scale), "scale is not finite");
   if (n_seqs == 0) return QMOE_OK;
-  QMOE_REQUIRE(q_dev && out_dev && lengths_dev && work_dev, "null device pointer");
-  QMOE_REQUIRE((reinterpret_cast<uintptr_t>(work_dev) & 15u) == 0, "workspace must be 16-byte aligned");
+  QMOE_REQUIRE(args->q_dev && args->out_dev && args->lengths_dev && args->work_dev, "null device pointer");
+  QMOE_REQUIRE((reinterpret_cast<uintptr_t>(args->work_dev) & 15u) == 0, "workspace must be 16-byte aligned");
   if (n_seqs > kPagedMaxSeqs || (int64_t)n_seqs * heads > 0x7fffffffLL) {
     set_error("%s: at most %d sequences", __func__, kPagedMaxSeqs);
     return QMOE_ERR_UNSUPPORTED;
   }
   const PagedShape shape = paged_shape(heads, cache->kv_heads, cache->head_dim);
-  a.q = q_dev;
-  a.out = out_dev;
-  a.q_row = q_row;
-  a.q_head = q_head;
-  a.lengths = lengths_dev;
-  a.bias = rel_bias_dev;
-  a.n_dist = n_dist;
+  a.q = args->q_dev;
+  a.out = args->out_dev;
+  a.q_row = args->q_row;
+  a.q_head = args->q_head;
+  a.lengths = args->lengths_dev;
+  a.bias = args->rel_bias_dev;
+  a.n_dist = args->n_dist;
   a.heads = heads;
   a.n_seqs = n_seqs;
-  a.dtype = dtype;
+  a.dtype = args->dtype;
   a.warps = paged_warps(shape.width, device);
-  a.prefix = reinterpret_cast<long long *>(work_dev);
-  a.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(work_dev) + ((int64_t)(n_seqs + 1) * 8 + 15) / 16 * 16);
-  a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
+  a.prefix = reinterpret_cast<long long *>(args->work_dev);
+  a.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(args->work_dev) + ((int64_t)(n_seqs + 1) * 8 + 15) / 16 * 16);
+  a.scale = args->scale > 0.f ? args->scale : 1.f / sqrtf((float)cache->head_dim);
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -808,21 +808,20 @@ __global__ void __launch_bounds__(kRowThreads) k_sample(const SampleArgs a, cons
 
 using namespace qmoe;
 
-extern "C" int qmoe_sample(const void *logits_dev, int64_t row_stride, int rows, int vocab, int dtype,
-                           const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev,
-                           const float *min_p_dev, const float *uniform_dev, int64_t *tokens_dev, float *logprob_dev,
-                           int device, void *stream) {
-  QMOE_REQUIRE(rows >= 0 && vocab >= 1 && row_stride >= 0, "bad shape");
+extern "C" int qmoe_sample(const qmoe_sample_args *args, int device, void *stream) {
+  QMOE_REQUIRE(args != nullptr, "null pointer");
+  const int rows = args->rows, vocab = args->vocab, dtype = args->dtype;
+  QMOE_REQUIRE(rows >= 0 && vocab >= 1 && args->row_stride >= 0, "bad shape");
   QMOE_REQUIRE(dtype == QMOE_FP32 || dtype == QMOE_BF16 || dtype == QMOE_FP16, "logits are fp32, bf16 or fp16");
   if (rows == 0) return QMOE_OK;
   QMOE_REQUIRE(rows <= 0x7fffffff / kMaxCluster, "too many rows");
-  QMOE_REQUIRE(logits_dev && uniform_dev && tokens_dev, "null device pointer");
+  QMOE_REQUIRE(args->logits_dev && args->uniform_dev && args->tokens_dev, "null device pointer");
   if (vocab > kMaxVocab) {
     set_error("%s: at most %d logits a row are supported", __func__, kMaxVocab);
     return QMOE_ERR_UNSUPPORTED;
   }
-  const SampleArgs a{logits_dev, row_stride, vocab, temperature_dev, top_p_dev, min_p_dev, uniform_dev, top_k_dev,
-                     reinterpret_cast<long long *>(tokens_dev), logprob_dev};
+  const SampleArgs a{args->logits_dev, args->row_stride, vocab, args->temperature_dev, args->top_p_dev, args->min_p_dev,
+                     args->uniform_dev, args->top_k_dev, reinterpret_cast<long long *>(args->tokens_dev), args->logprob_dev};
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

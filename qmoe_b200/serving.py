@@ -27,11 +27,16 @@ FORMATS = {"e4m3": (0, torch.float8_e4m3fn), "int8": (1, torch.int8)}
 
 
 def _stream(dev: torch.device) -> int:
-    return int(torch.cuda.current_stream(dev).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _need(t, name: str, dtypes, ndim: int, device: Optional[torch.device] = None, packed: bool = True) -> torch.Tensor:
     """Checks of one argument; ``packed`` False: only the last axis has to be contiguous."""
+    if (t.__class__ is torch.Tensor and (t.dtype is dtypes or (dtypes.__class__ is tuple and t.dtype in dtypes)) and t.dim() == ndim
+            and t.is_cuda and (t.is_contiguous() or (not packed and t.stride(-1) == 1))
+            and (device is None or t.get_device() == device.index)):
+        return t
+    # the same one after another, for the message
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
@@ -52,15 +57,15 @@ def _need(t, name: str, dtypes, ndim: int, device: Optional[torch.device] = None
 
 def _bias_args(rel_bias: Optional[torch.Tensor], heads: int, dev: torch.device):
     if rel_bias is None:
-        return None, 0
+        return 0, 0
     _need(rel_bias, "rel_bias", torch.float32, 2, dev)
     if rel_bias.shape[0] != heads or rel_bias.shape[1] < 1:
         raise ValueError(f"rel_bias must be [heads = {heads}, distances >= 1], got {tuple(rel_bias.shape)}")
     return rel_bias.data_ptr(), rel_bias.shape[1]
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -99,12 +104,17 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if out.shape != q.shape:
             raise ValueError("out must have the shape of q")
     bias, n_dist = _bias_args(rel_bias, heads, dev)
-    shape = _lib.PromptShape(total_q, total_k, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-                             v.stride(1), out.stride(0), out.stride(1), cu_q.numel() - 1, heads, kv_heads, hd,
-                             _DTYPES[q.dtype], n_dist, float(scale))
-    _lib.check(_lib.load().qmoe_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                                 cu_q.data_ptr(), cu_k.data_ptr(), bias, ctypes.byref(shape),
-                                                 dev.index, _stream(dev)))
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    fields = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), bias, 0,
+              total_q, total_k, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], cu_q.numel() - 1, heads, kv_heads,
+              hd, _DTYPES[q.dtype], n_dist, scale]
+    L, args = _lib.load(), _lib.PROMPT_ARGS.pack(*fields)
+    nbytes = L.qmoe_prompt_work_bytes(args)
+    if nbytes:
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        fields[7] = work.data_ptr()
+        args = _lib.PROMPT_ARGS.pack(*fields)
+    _lib.check(L.qmoe_prompt_attention(args, dev.index, _stream(dev)))
     return out
 
 
@@ -140,6 +150,8 @@ class QuantCache:
         self.device = self.k_codes.device
         self.desc = _lib.QuantCacheDesc(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(),
                                         self.v_scale.data_ptr(), n_pages, page_size, kv_heads, head_dim, code)
+        self._desc = ctypes.addressof(self.desc)
+        self._status = self.status.data_ptr()
 
     def refused(self, reset: bool = False) -> int:
         """Positions refused so far because the page table had no valid page for them (synchronises)."""
@@ -180,11 +192,10 @@ def cache_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor, cu: torch.
     _need(v, "v", k.dtype, 3, cache.device, packed=False)
     if k.shape != v.shape or tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
         raise ValueError(f"k and v must be [rows, {cache.kv_heads}, {cache.head_dim}], got {tuple(k.shape)}, {tuple(v.shape)}")
-    dev = cache.device
-    _lib.check(_lib.load().qmoe_cache_append(
-        ctypes.byref(cache.desc), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        cu.data_ptr(), start.data_ptr(), page_table.data_ptr(), cache.status.data_ptr(), n_seqs, max_pages, k.shape[0],
-        _DTYPES[k.dtype], dev.index, _stream(dev)))
+    dev, ks, vs = cache.device, k.stride(), v.stride()
+    args = _lib.CACHE_ROWS.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], cu.data_ptr(), start.data_ptr(),
+                                page_table.data_ptr(), cache._status, k.shape[0], n_seqs, max_pages, _DTYPES[k.dtype])
+    _lib.check(_lib.load().qmoe_cache_append(cache._desc, args, dev.index, _stream(dev)))
 
 
 def cache_read(cache: QuantCache, cu: torch.Tensor, start: torch.Tensor, page_table: torch.Tensor, rows: int,
@@ -200,9 +211,9 @@ def cache_read(cache: QuantCache, cu: torch.Tensor, start: torch.Tensor, page_ta
     dev = cache.device
     k = torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    _lib.check(_lib.load().qmoe_cache_read(
-        ctypes.byref(cache.desc), k.data_ptr(), v.data_ptr(), cu.data_ptr(), start.data_ptr(), page_table.data_ptr(),
-        cache.status.data_ptr(), n_seqs, max_pages, rows, _DTYPES[dtype], dev.index, _stream(dev)))
+    args = _lib.CACHE_ROWS.pack(k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, cu.data_ptr(), start.data_ptr(),
+                                page_table.data_ptr(), cache._status, rows, n_seqs, max_pages, _DTYPES[dtype])
+    _lib.check(_lib.load().qmoe_cache_read(cache._desc, args, dev.index, _stream(dev)))
     return k, v
 
 
@@ -225,13 +236,12 @@ def decode_attention_paged(q: torch.Tensor, cache: QuantCache, page_table: torch
     dev = cache.device
     bias, n_dist = _bias_args(rel_bias, heads, dev)
     out = torch.empty((n_seqs, heads, hd), dtype=q.dtype, device=dev)
-    L = _lib.load()
-    nbytes = int(L.qmoe_decode_paged_work_bytes(n_seqs, heads, cache.kv_heads, hd, dev.index))
+    L, qs = _lib.load(), q.stride()
+    nbytes = L.qmoe_decode_paged_work_bytes(n_seqs, heads, cache.kv_heads, hd, dev.index)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _lib.check(L.qmoe_decode_attention_paged(
-        ctypes.byref(cache.desc), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), page_table.data_ptr(),
-        lengths.data_ptr(), bias, n_dist, cache.status.data_ptr(), _ptr(work), n_seqs, heads, max_pages, float(scale),
-        _DTYPES[q.dtype], dev.index, _stream(dev)))
+    args = _lib.PAGED_ARGS.pack(q.data_ptr(), out.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), bias, cache._status,
+                                _ptr(work), qs[0], qs[1], n_dist, n_seqs, heads, max_pages, _DTYPES[q.dtype], scale)
+    _lib.check(L.qmoe_decode_attention_paged(cache._desc, args, dev.index, _stream(dev)))
     return out
 
 
@@ -271,13 +281,13 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: Unio
     _need(uniform, "uniform", torch.float32, 1, dev)
     if uniform.numel() != rows:
         raise ValueError("uniform must have an entry per row")
-    settings = [_per_row(temperature, "temperature", torch.float32, rows, dev),
-                _per_row(top_k, "top_k", torch.int32, rows, dev),
-                _per_row(top_p, "top_p", torch.float32, rows, dev),
-                _per_row(min_p, "min_p", torch.float32, rows, dev)]
+    t = _per_row(temperature, "temperature", torch.float32, rows, dev)
+    k = _per_row(top_k, "top_k", torch.int32, rows, dev)
+    p = _per_row(top_p, "top_p", torch.float32, rows, dev)
+    m = _per_row(min_p, "min_p", torch.float32, rows, dev)
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     logprob = torch.empty(rows, dtype=torch.float32, device=dev) if return_logprob else None
-    _lib.check(_lib.load().qmoe_sample(
-        logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, _DTYPES[logits.dtype],
-        *(_ptr(t) for t in settings), uniform.data_ptr(), tokens.data_ptr(), _ptr(logprob), dev.index, _stream(dev)))
+    args = _lib.SAMPLE_ARGS.pack(logits.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m), uniform.data_ptr(), tokens.data_ptr(),
+                                 _ptr(logprob), logits.stride(0) if rows > 1 else vocab, rows, vocab, _DTYPES[logits.dtype])
+    _lib.check(_lib.load().qmoe_sample(args, dev.index, _stream(dev)))
     return (tokens, logprob) if return_logprob else tokens

@@ -6,22 +6,34 @@ import torch
 
 from qmoe_b200 import _lib, serving
 
-FAKE = ctypes.c_void_p(256)
+FAKE = 256                                     # an address that nothing looks at: refusals come first
+PROMPT = ("q", "k", "v", "out", "cu_q", "cu_k", "bias", "work", "total_q", "total_k", "q_row", "q_head", "k_row", "k_head",
+          "v_row", "v_head", "out_row", "out_head", "n_seqs", "heads", "kv_heads", "head_dim", "dtype", "n_dist", "scale")
+ROWS = ("k", "v", "k_row", "k_head", "v_row", "v_head", "cu", "start", "table", "status", "n_rows", "n_seqs", "max_pages", "dtype")
+PAGED = ("q", "out", "table", "lengths", "bias", "status", "work", "q_row", "q_head", "n_dist", "n_seqs", "heads", "max_pages",
+         "dtype", "scale")
+SAMPLE = ("logits", "temperature", "top_k", "top_p", "min_p", "uniform", "tokens", "logprob", "row_stride", "rows", "vocab", "dtype")
+
+
+def _pack(layout, names, base, changes):
+    unknown = set(changes) - set(names)
+    assert not unknown, unknown
+    return layout.pack(*[changes.get(n, base.get(n, FAKE)) for n in names])
 
 
 def _shape(**kw):
-    base = dict(total_q=4, total_k=4, q_row=64, q_head=64, k_row=64, k_head=64, v_row=64, v_head=64, out_row=64,
-                out_head=64, n_seqs=1, heads=2, kv_heads=1, head_dim=64, dtype=0, n_dist=0, scale=0.0)
-    base.update(kw)
-    return _lib.PromptShape(*[base[name] for name, _ in _lib.PromptShape._fields_])
+    return _pack(_lib.PROMPT_ARGS, PROMPT, dict(bias=0, work=0, total_q=4, total_k=4, q_row=64, q_head=64, k_row=64, k_head=64,
+                                                v_row=64, v_head=64, out_row=64, out_head=64, n_seqs=1, heads=2, kv_heads=1,
+                                                head_dim=64, dtype=0, n_dist=0, scale=0.0), kw)
 
 
-def _prompt(shape, bias=None, q=FAKE):
-    return _lib.load().qmoe_prompt_attention(q, FAKE, FAKE, FAKE, FAKE, FAKE, bias, ctypes.byref(shape), 0, None)
+def _prompt(args):
+    return _lib.load().qmoe_prompt_attention(args, 0, None)
 
 
 def test_struct_layouts():
-    assert ctypes.sizeof(_lib.PromptShape) == 112 and _lib.PromptShape.scale.offset == 104
+    assert _lib.PROMPT_ARGS.size == 8 * 18 + 4 * 8 and _lib.CACHE_ROWS.size == 8 * 11 + 16
+    assert _lib.PAGED_ARGS.size == 8 * 9 + 24 and _lib.SAMPLE_ARGS.size == 8 * 9 + 16
     assert ctypes.sizeof(_lib.QuantCacheDesc) == 56
 
 
@@ -37,10 +49,22 @@ def test_prompt_refusals(bad, status):
 
 
 def test_prompt_null_pointers_and_empty_calls():
-    assert _prompt(_shape(), q=None) == _lib.ERR_INVALID_ARG
-    assert _prompt(_shape(), bias=FAKE) == _lib.ERR_INVALID_ARG
-    assert _lib.load().qmoe_prompt_attention(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, None, 0, None) == _lib.ERR_INVALID_ARG
+    assert _prompt(_shape(q=0)) == _lib.ERR_INVALID_ARG
+    assert _prompt(_shape(cu_k=0)) == _lib.ERR_INVALID_ARG
+    assert _prompt(_shape(bias=FAKE)) == _lib.ERR_INVALID_ARG
+    assert _prompt(None) == _lib.ERR_INVALID_ARG
     assert _prompt(_shape(n_seqs=0)) == _lib.OK and _prompt(_shape(total_q=0)) == _lib.OK
+
+
+def test_prompt_workspace():
+    size = lambda **kw: _lib.load().qmoe_prompt_work_bytes(_shape(**kw))  # noqa: E731
+    assert size() == 0
+    assert size(q=258) == 4 * 2 * 64 * 2                             # q off its boundary
+    assert size(k_row=65) == 4 * 64 * 2 and size(heads=4, q_head=0) == 4 * 4 * 64 * 2
+    assert size(k_head=3, v_head=0) == 0                             # the stride of one head is not used
+    assert size(head_dim=200, q_row=201) == 0                        # taken row by row
+    assert _prompt(_shape(k_row=65)) == _lib.ERR_INVALID_ARG         # needs a workspace
+    assert _prompt(_shape(k_row=65, work=258)) == _lib.ERR_INVALID_ARG
 
 
 def _cache(**kw):
@@ -56,36 +80,61 @@ def _cache(**kw):
     (dict(n_pages=-1), _lib.ERR_INVALID_ARG), (dict(k_codes=None), _lib.ERR_INVALID_ARG), (dict(v_scale=None), _lib.ERR_INVALID_ARG),
     (dict(k_codes=264), _lib.ERR_INVALID_ARG)])
 def test_cache_refusals(bad, status):
-    lib, c = _lib.load(), ctypes.byref(_cache(**bad))
-    assert lib.qmoe_cache_append(c, FAKE, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, FAKE, 1, 1, 1, 0, 0, None) == status
-    assert lib.qmoe_cache_read(c, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1, 1, 1, 0, 0, None) == status
-    assert lib.qmoe_decode_attention_paged(c, FAKE, 1, 1, FAKE, FAKE, FAKE, None, 0, FAKE, FAKE, 1, 2, 1, 0.0, 0, 0, None) == status
+    desc = _cache(**bad)
+    assert _append(desc) == status and _read(desc) == status and _decode(desc) == status
+
+
+def _rows(**kw):
+    return _pack(_lib.CACHE_ROWS, ROWS, dict(k_row=1, k_head=1, v_row=1, v_head=1, n_rows=1, n_seqs=1, max_pages=1, dtype=0), kw)
+
+
+def _append(desc, **kw):
+    return _lib.load().qmoe_cache_append(None if desc is None else ctypes.addressof(desc), _rows(**kw), 0, None)
+
+
+def _read(desc, **kw):
+    return _lib.load().qmoe_cache_read(None if desc is None else ctypes.addressof(desc), _rows(**kw), 0, None)
+
+
+def _decode(desc, **kw):
+    args = _pack(_lib.PAGED_ARGS, PAGED, dict(bias=0, q_row=1, q_head=1, n_dist=0, n_seqs=1, heads=2, max_pages=1, dtype=0, scale=0.0), kw)
+    return _lib.load().qmoe_decode_attention_paged(None if desc is None else ctypes.addressof(desc), args, 0, None)
 
 
 def test_cache_call_refusals():
-    lib, c = _lib.load(), ctypes.byref(_cache())
-    assert lib.qmoe_cache_append(None, FAKE, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, FAKE, 1, 1, 1, 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert lib.qmoe_cache_append(c, FAKE, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, None, 1, 1, 1, 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert lib.qmoe_cache_append(c, None, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, FAKE, 1, 1, 1, 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert lib.qmoe_cache_append(c, FAKE, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, FAKE, 1, 1, 1, 2, 0, None) == _lib.ERR_INVALID_ARG
-    assert lib.qmoe_cache_append(c, FAKE, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, FAKE, 1, 1, -1, 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert lib.qmoe_cache_append(c, FAKE, FAKE, 1, 1, 1, 1, FAKE, FAKE, FAKE, FAKE, 0, 1, 0, 0, 0, None) == _lib.OK
-    dec = lib.qmoe_decode_attention_paged
-    assert dec(c, FAKE, 1, 1, FAKE, FAKE, FAKE, None, 0, FAKE, FAKE, 1, 3, 1, 0.0, 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert dec(c, FAKE, 1, 1, FAKE, FAKE, FAKE, FAKE, 0, FAKE, FAKE, 1, 2, 1, 0.0, 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert dec(c, FAKE, 1, 1, FAKE, FAKE, FAKE, None, 0, FAKE, FAKE, 1, 2, 1, float("nan"), 0, 0, None) == _lib.ERR_INVALID_ARG
-    assert dec(c, FAKE, 1, 1, None, FAKE, FAKE, None, 0, FAKE, FAKE, 1, 2, 1, 0.0, 0, 0, None) == _lib.ERR_INVALID_ARG
+    c = _cache()
+    for call in (_append, _read):
+        assert call(None) == _lib.ERR_INVALID_ARG
+        for name in ("k", "v", "cu", "start", "table", "status"):
+            assert call(c, **{name: 0}) == _lib.ERR_INVALID_ARG, name
+        assert call(c, dtype=2) == _lib.ERR_INVALID_ARG
+        assert call(c, n_rows=-1) == _lib.ERR_INVALID_ARG and call(c, n_rows=1 << 31) == _lib.ERR_INVALID_ARG
+        assert call(c, n_seqs=-1) == _lib.ERR_INVALID_ARG and call(c, max_pages=-1) == _lib.ERR_INVALID_ARG
+        assert call(c, n_seqs=0, n_rows=0) == _lib.OK and call(c, n_rows=0) == _lib.OK
+        assert call(_cache(kv_heads=1025)) == _lib.ERR_UNSUPPORTED
+    assert _decode(None) == _lib.ERR_INVALID_ARG
+    for name in ("q", "out", "table", "lengths", "status", "work"):
+        assert _decode(c, **{name: 0}) == _lib.ERR_INVALID_ARG, name
+    for bad in (dict(heads=3), dict(heads=0), dict(bias=FAKE), dict(n_dist=3), dict(n_dist=-1), dict(scale=float("nan")),
+                dict(scale=float("-inf")), dict(dtype=2), dict(work=257), dict(n_seqs=-1)):
+        assert _decode(c, **bad) == _lib.ERR_INVALID_ARG, bad
+    assert _decode(c, n_seqs=4097) == _lib.ERR_UNSUPPORTED
+    assert _decode(c, n_seqs=0) == _lib.OK
+    size = _lib.load().qmoe_decode_paged_work_bytes
+    assert size(4, 8, 2, 64, 0) > 0 and size(0, 8, 2, 64, 0) == 0 and size(4, 8, 3, 64, 0) == 0 and size(4, 8, 2, 300, 0) == 0
 
 
 def test_sample_refusals():
-    f = _lib.load().qmoe_sample
-    ok = [FAKE, 8, 1, 8, 2, None, None, None, None, FAKE, FAKE, None, 0, None]
-    for at, value, status in ((0, None, _lib.ERR_INVALID_ARG), (9, None, _lib.ERR_INVALID_ARG), (10, None, _lib.ERR_INVALID_ARG),
-                              (2, -1, _lib.ERR_INVALID_ARG), (3, 0, _lib.ERR_INVALID_ARG), (4, 3, _lib.ERR_INVALID_ARG),
-                              (1, -8, _lib.ERR_INVALID_ARG), (3, 262145, _lib.ERR_UNSUPPORTED), (2, 0, _lib.OK)):
-        args = list(ok)
-        args[at] = value
-        assert f(*args) == status, (at, value)
+    def call(**kw):
+        base = dict(temperature=0, top_k=0, top_p=0, min_p=0, logprob=0, row_stride=8, rows=1, vocab=8, dtype=2)
+        return _lib.load().qmoe_sample(_pack(_lib.SAMPLE_ARGS, SAMPLE, base, kw), 0, None)
+
+    for bad in (dict(logits=0), dict(uniform=0), dict(tokens=0), dict(rows=-1), dict(vocab=0), dict(dtype=3), dict(row_stride=-8),
+                dict(rows=1 << 30)):
+        assert call(**bad) == _lib.ERR_INVALID_ARG, bad
+    assert call(vocab=262145) == _lib.ERR_UNSUPPORTED
+    assert call(rows=0) == _lib.OK
+    assert _lib.load().qmoe_sample(None, 0, None) == _lib.ERR_INVALID_ARG
 
 
 def test_python_refusals_on_cpu_tensors():
