@@ -14,6 +14,8 @@
 
 namespace qmoe {
 
+int allow_shared(const void *kernel, int bytes, int device, int regs);
+
 // ---- error plumbing -------------------------------------------------------------------------
 static thread_local char g_error[512] = "";
 
@@ -77,6 +79,24 @@ int *tile_status_word(int device) {
     word[device] = p;
   }
   return word[device];
+}
+
+int allow_shared(const void *kernel, int bytes, int device, int regs) {
+  static std::map<std::pair<const void *, int>, int> allowed;
+  std::lock_guard<std::mutex> lock(setup_mutex());
+  auto it = allowed.find({kernel, device});
+  if (it != allowed.end() && it->second >= bytes) return QMOE_OK;
+  if (regs > 0) {
+    cudaFuncAttributes attr;
+    QMOE_CUDA(cudaFuncGetAttributes(&attr, kernel));
+    if (attr.numRegs != regs) {
+      set_error("a kernel was built with %d registers a thread instead of %d", attr.numRegs, regs);
+      return QMOE_ERR_UNSUPPORTED;
+    }
+  }
+  QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  allowed[{kernel, device}] = bytes;
+  return QMOE_OK;
 }
 
 int sm_count(int device) {

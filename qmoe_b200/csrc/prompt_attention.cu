@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // All waits are bounded; when one runs out the CTA counts itself in d_prompt_timeouts, frees its tensor
 // memory and returns.
 constexpr int kPromptThreads = 512;
+constexpr int kPromptRegs = 128;  // at launch; the softmax warps then hold 192 and the others 64
 constexpr int kTileRows = 128;
 constexpr int kStages = 4;
 constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
@@ -633,7 +634,7 @@ static bool needs_packing(const void *base, int64_t rows, int heads, int64_t row
 static int64_t packed_bytes(int64_t rows, int heads, int d) { return (rows * heads * ((d + 7) / 8 * 16) + 255) / 256 * 256; }
 
 template <typename T>
-static int run_prompt(PromptArgs a, void *work, cudaStream_t stream) {
+static int run_prompt(PromptArgs a, void *work, int device, cudaStream_t stream) {
   if (a.s.head_dim > kTileRows) {
     const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 3) / 4));
     QMOE_LAUNCH((k_prompt_rows<T>), grid, 128, 0, stream, a);
@@ -674,13 +675,9 @@ static int run_prompt(PromptArgs a, void *work, cudaStream_t stream) {
                    make_map(&maps.v, a.v, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.v_head, a.s.v_row);
   const int smem = (2 + kStages) * ((a.s.head_dim + 63) / 64) * kBlockBytes + 1024;
   auto kernel = a.bias != nullptr ? k_prompt_tiles<T, true> : k_prompt_tiles<T, false>;
-  cudaFuncAttributes attr;
-  QMOE_CUDA(cudaFuncGetAttributes(&attr, kernel));
-  if (attr.numRegs * kPromptThreads < 65536) {  // the warpgroups' shares have to fit what the block is launched with
-    set_error("prompt attention: built with %d registers a thread, 128 are needed", attr.numRegs);
-    return QMOE_ERR_UNSUPPORTED;
-  }
-  QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the warpgroups' register shares have to fit what the block is launched with
+  const int allowed = allow_shared(reinterpret_cast<const void *>(kernel), smem, device, kPromptRegs);
+  if (allowed != QMOE_OK) return allowed;
   const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 2 * kTileRows - 1) / (2 * kTileRows) + a.s.n_seqs));
   QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, maps, tma);
   QMOE_CUDA(cudaGetLastError());
@@ -722,5 +719,6 @@ extern "C" int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, v
   DeviceGuard guard(device);
   if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return a.s.dtype == QMOE_BF16 ? run_prompt<__nv_bfloat16>(a, args->work_dev, st) : run_prompt<__half>(a, args->work_dev, st);
+  return a.s.dtype == QMOE_BF16 ? run_prompt<__nv_bfloat16>(a, args->work_dev, device, st)
+                                  : run_prompt<__half>(a, args->work_dev, device, st);
 }

@@ -1095,7 +1095,8 @@ int qmoe_decode_attention_paged(const qmoe_quant_cache *cache, const qmoe_paged_
     constexpr int NB = decltype(nb)::value;
     auto kernel = e4m3 ? (wide ? k_decode_paged<NB, QMOE_CACHE_E4M3, true> : k_decode_paged<NB, QMOE_CACHE_E4M3, false>)
                        : (wide ? k_decode_paged<NB, QMOE_CACHE_INT8, true> : k_decode_paged<NB, QMOE_CACHE_INT8, false>);
-    QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int allowed = allow_shared(reinterpret_cast<const void *>(kernel), (int)smem, device);
+    if (allowed != QMOE_OK) return allowed;
     QMOE_LAUNCH(kernel, grid, kPagedThreads, smem, st, a);
     QMOE_CUDA(cudaGetLastError());
     return QMOE_OK;

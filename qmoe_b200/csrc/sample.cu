@@ -833,7 +833,8 @@ extern "C" int qmoe_sample(const qmoe_sample_args *args, int device, void *strea
   const int slice = ((vocab + ranks - 1) / ranks + 7) / 8 * 8;
   auto kernel = dtype == QMOE_FP32 ? k_sample<float> : (dtype == QMOE_BF16 ? k_sample<__nv_bfloat16> : k_sample<__half>);
   const size_t smem = kRowSharedBytes + (size_t)slice * sizeof(float);
-  QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int allowed = allow_shared(reinterpret_cast<const void *>(kernel), (int)smem, device);
+  if (allowed != QMOE_OK) return allowed;
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = (unsigned)ranks;

@@ -71,6 +71,10 @@ __device__ __forceinline__ pair_t pair_mul(pair_t a, pair_t b) {
   return d;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory on a device; remembered, as the attribute call costs a
+// microsecond.  `regs` > 0: fails unless the kernel was built with that many registers a thread.
+int allow_shared(const void *kernel, int bytes, int device, int regs = 0);
+
 __host__ __device__ constexpr int cache_row_bytes(int head_dim) { return (head_dim + 15) & ~15; }
 
 }  // namespace qmoe
