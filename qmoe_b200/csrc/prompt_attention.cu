@@ -92,9 +92,11 @@ constexpr int kPromptThreads = 512;
 constexpr int kPromptRegs = 128;  // at launch; the softmax warps then hold 192 and the others 64
 constexpr int kTileRows = 128;
 constexpr int kStages = 4;
+constexpr int kItems = 4;         // decided ahead
+constexpr int kItemReaders = 10;  // arrivals that give an item back: eight softmax warps, one for products, one for copies
 constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
 constexpr int kPolyPairs = 2;
-constexpr uint32_t kPromptWait = 1u << 22;
+constexpr unsigned long long kPromptWait = 4000000000ull;  // ns; a row computed again key by key may take a while
 __device__ int d_prompt_timeouts;
 
 struct PromptMaps {
@@ -102,14 +104,20 @@ struct PromptMaps {
 };
 
 struct PromptBars {
-  uint64_t q_full, s_full[2], p_full[2][2], pv_done[2], kv_full[kStages], kv_empty[kStages], drain;
+  uint64_t q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], kv_full[kStages], kv_empty[kStages];
+  uint64_t item_full[kItems], item_empty[kItems], drain;
 };
 
+// Waits for a phase of a barrier for kPromptWait nanoseconds at most, or until another wait of the CTA ran out.
 __device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, volatile int *fail) {
-  for (uint32_t i = 0; i < kPromptWait; i++) {
+  if (mbar_wait(bar, parity, 2)) return true;
+  unsigned long long now, begin;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
+  do {
     if (mbar_wait(bar, parity, 2)) return true;
     if (*fail) return false;
-  }
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+  } while (now - begin < kPromptWait);
   *fail = 1;
   return false;
 }
@@ -210,65 +218,27 @@ __global__ void __launch_bounds__(256) k_prompt_pack(const PackArgs a) {
   }
 }
 
+// What a CTA works on next: 256 queries of one head.
+struct PromptItem {
+  int valid, head, q_row, n, k_row, m, row0;  // first query row of the tensor, queries, first key row, keys of the sequence
+  int steps[2];                               // key tiles that each query tile walks
+};
+
 template <typename T, bool BIAS>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    const bool tma) {
+                                                                    const bool tma, const int n_items) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // the swizzle repeats every 1024 bytes
   __shared__ PromptBars s_bar;
+  __shared__ PromptItem s_item[kItems];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
-  __shared__ int s_scan[kPromptThreads / 32];
-  __shared__ int s_seq, s_tile;
   __shared__ volatile int s_stop[2];
-  const int tid = threadIdx.x, lane = tid & 31, head = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-
-  // ---- which sequence and tile: blocks count the tiles of all sequences, the longest queries of each first
-  if (tid == 0) s_seq = -1;
-  int before = 0;
-  for (int s0 = 0; s0 < a.s.n_seqs; s0 += kPromptThreads) {
-    const int2 r = s0 + tid < a.s.n_seqs ? packed_rows(a.cu_q, s0 + tid, a.s.total_q) : make_int2(0, 0);
-    const int count = (r.y - r.x + 2 * kTileRows - 1) / (2 * kTileRows);
-    int upto = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = upto;
-    __syncthreads();
-    int all = 0, mine = before + upto;
-    for (int w = 0; w < kPromptThreads / 32; w++) {
-      if (w < warp) mine += s_scan[w];
-      all += s_scan[w];
-    }
-    const int block = blockIdx.y;
-    if (block < mine && block >= mine - count) {
-      s_seq = s0 + tid;
-      s_tile = mine - 1 - block;
-    }
-    before += all;
-    if (before > block) break;
-  }
-  __syncthreads();
-  const int seq = s_seq;
-  if (seq < 0) return;
-  const int2 rq = packed_rows(a.cu_q, seq, a.s.total_q), rk = packed_rows(a.cu_k, seq, a.s.total_k);
-  const int n = rq.y - rq.x, m = rk.y - rk.x, shift = m - n;
-  const int row0 = s_tile * 2 * kTileRows;
-  int steps[2];  // key tiles that each query tile walks
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int r = row0 + i * kTileRows, rows = min(kTileRows, n - r);
-    const int last = r + rows - 1 + shift;
-    steps[i] = rows <= 0 || last < 0 ? 0 : last / kTileRows + 1;
-  }
-  const int n_steps = max(steps[0], steps[1]);
   const int d = a.s.head_dim, chunks = 2 * ((d + 15) / 16), blocks = (d + 63) / 64, tile_bytes = blocks * kBlockBytes;
-  const int kv = head / (a.s.heads / a.s.kv_heads);
-  uint8_t *q_tile = smem, *ring = smem + 2 * tile_bytes;
+  const int group = a.s.heads / a.s.kv_heads;
+  uint8_t *q_tile = smem, *ring = smem + 2 * tile_bytes, *stage_out = ring + kStages * tile_bytes;
 
   auto bar = [&](uint64_t &b) { return smem_u32(&b); };
   if (tid == 0) {
@@ -282,86 +252,186 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       mbar_init(bar(s_bar.kv_full[i]), 1);
       mbar_init(bar(s_bar.kv_empty[i]), 1);
     }
+    for (int i = 0; i < kItems; i++) {
+      mbar_init(bar(s_bar.item_full[i]), 1);
+      mbar_init(bar(s_bar.item_empty[i]), kItemReaders);
+    }
     mbar_init(bar(s_bar.q_full), 1);
+    mbar_init(bar(s_bar.q_empty), 1);
     mbar_init(bar(s_bar.drain), 1);
     s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(smem_u32(&s_tmem), 512);
-  if (n_steps > 0 && !tma) {
-    for (int i = 0; i < 2; i++) {
-      const int r = row0 + i * kTileRows;
-      load_tile<T, kPromptThreads>(q_tile + i * tile_bytes,
-                                   reinterpret_cast<const T *>(a.q) + (rq.x + (r < n ? r : 0)) * a.s.q_row + head * a.s.q_head,
-                                   a.s.q_row, max(0, min(kTileRows, n - r)), d, chunks, tid);
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    fence_async_proxy();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  // Item number `x` of this CTA, by every thread that uses it; false when a wait ran out.  Given back by
+  // done_item, once per warp that reads items (the copying warps: once).
+  auto get_item = [&](int x, PromptItem &item) {
+    const bool ok = wait_or_fail(bar(s_bar.item_full[x % kItems]), (x / kItems) & 1, &s_fail);
+    item = s_item[x % kItems];
+    return ok;
+  };
+  auto done_item = [&](int x) { mbar_arrive(bar(s_bar.item_empty[x % kItems])); };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp >= 12) {
-      // ---- copies: K 0, V 0, K 1, V 1, ...
+      // ---- copies: Q, then K 0, V 0, K 1, V 1, ... of one item after another
       const int t = tid - 384;
-      const int n_tma = tma ? 2 * min(n_steps, m / kTileRows) : 0;  // whole key tiles come by bulk copies
       bool ok = true;
-      if (t == 0 && tma && n_steps > 0) {
-        const uint32_t q_full = bar(s_bar.q_full);
-        mbar_arrive_tx(q_full, (uint32_t)((steps[0] > 0) + (steps[1] > 0)) * tile_bytes);
-        for (int i = 0; i < 2; i++)
-          for (int b = 0; steps[i] > 0 && b < blocks; b++)
-            tma_load3(smem_u32(q_tile) + i * tile_bytes + b * kBlockBytes, &maps.q, 64 * b, head, rq.x + row0 + i * kTileRows, q_full);
-        int item = 0;
-        for (; item < n_tma; item++) {
-          const int stage = item % kStages;
-          ok = item < kStages || wait_or_fail(bar(s_bar.kv_empty[stage]), (item / kStages - 1) & 1, &s_fail);
-          if (!ok) break;
-          const uint32_t full = bar(s_bar.kv_full[stage]);
-          mbar_arrive_tx(full, tile_bytes);
-          for (int b = 0; b < blocks; b++)
-            tma_load3(smem_u32(ring) + stage * tile_bytes + b * kBlockBytes, (item & 1) ? &maps.v : &maps.k, 64 * b, kv,
-                      rk.x + (item >> 1) * kTileRows, full);
+      int copied = 0, first = 0;  // buffers filled so far, at the beginning of the item
+      for (int x = 0;; x++) {
+        PromptItem item;
+        ok = get_item(x, item) && ok;
+        // one decision for all: thread 0's
+        if (t == 0) s_stop[0] = !ok || !item.valid;
+        named_sync(1, kTileRows);
+        const bool stop = s_stop[0];
+        named_sync(1, kTileRows);
+        if (stop) break;
+        const int n_steps = max(item.steps[0], item.steps[1]), kv = item.head / group;
+        const int n_tma = tma ? 2 * min(n_steps, item.m / kTileRows) : 0;  // whole key tiles come by bulk copies
+        if (n_steps > 0) {
+          if (t == 0 && x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, &s_fail);
+          if (tma && t == 0 && ok) {
+            const uint32_t q_full = bar(s_bar.q_full);
+            mbar_arrive_tx(q_full, (uint32_t)((item.steps[0] > 0) + (item.steps[1] > 0)) * tile_bytes);
+            for (int i = 0; i < 2; i++)
+              for (int b = 0; item.steps[i] > 0 && b < blocks; b++)
+                tma_load3(smem_u32(q_tile) + i * tile_bytes + b * kBlockBytes, &maps.q, 64 * b, item.head,
+                          item.q_row + item.row0 + i * kTileRows, q_full);
+          }
+          if (!tma) {
+            named_sync(1, kTileRows);
+            for (int i = 0; i < 2; i++) {
+              const int r = item.row0 + i * kTileRows;
+              load_tile<T, kTileRows>(q_tile + i * tile_bytes,
+                                      reinterpret_cast<const T *>(a.q) + (item.q_row + (long long)(r < item.n ? r : 0)) * a.s.q_row + item.head * a.s.q_head,
+                                      a.s.q_row, max(0, min(kTileRows, item.n - r)), d, chunks, t);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_async_proxy();
+            named_sync(1, kTileRows);
+            if (t == 0) mbar_arrive(bar(s_bar.q_full));
+          }
+        } else if (t == 0) {
+          if (x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, &s_fail);
+          mbar_arrive(bar(s_bar.q_full));  // nothing to copy: the phases go on
         }
-        if (!ok || s_fail) {  // copies in flight land before the block ends
-          mbar_wait(q_full, 0);
-          for (int x = max(0, item - kStages); x < item; x++) mbar_wait(bar(s_bar.kv_full[x % kStages]), (x / kStages) & 1);
-        }
-      }
-      __syncwarp();
-      for (int item = n_tma; item < 2 * n_steps; item++) {
-        const int stage = item % kStages;
         if (t == 0) {
-          if (ok && item >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (item / kStages - 1) & 1, &s_fail);
-          s_stop[item & 1] = !ok;
+          for (int c = 0; ok && c < n_tma; c++) {
+            const int at = first + c, stage = at % kStages;
+            if (at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, &s_fail);
+            if (!ok) break;
+            const uint32_t full = bar(s_bar.kv_full[stage]);
+            mbar_arrive_tx(full, tile_bytes);
+            for (int b = 0; b < blocks; b++)
+              tma_load3(smem_u32(ring) + stage * tile_bytes + b * kBlockBytes, (c & 1) ? &maps.v : &maps.k, 64 * b, kv,
+                        item.k_row + (c >> 1) * kTileRows, full);
+            copied = at + 1;
+          }
         }
-        named_sync(1, kTileRows);
-        if (s_stop[item & 1]) break;  // one decision for all: the other entry is written next
-        const int key0 = (item >> 1) * kTileRows;
-        const bool is_v = item & 1;
-        const long long pitch = is_v ? a.s.v_row : a.s.k_row;
-        const T *src = reinterpret_cast<const T *>(is_v ? a.v : a.k) + (rk.x + (long long)key0) * pitch +
-                       kv * (is_v ? a.s.v_head : a.s.k_head);
-        load_tile<T, kTileRows>(ring + stage * tile_bytes, src, pitch, min(kTileRows, m - key0), d, chunks, t);
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_async_proxy();
-        named_sync(1, kTileRows);
-        if (t == 0) mbar_arrive(bar(s_bar.kv_full[stage]));
+        __syncwarp();
+        bool gave_up = false;
+        for (int c = n_tma; c < 2 * n_steps; c++) {
+          const int at = first + c, stage = at % kStages;
+          if (t == 0) {
+            if (ok && at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, &s_fail);
+            s_stop[c & 1] = !ok;
+          }
+          named_sync(1, kTileRows);
+          gave_up = s_stop[c & 1];  // one decision for all: the other entry is written next
+          if (gave_up) break;
+          const int key0 = (c >> 1) * kTileRows;
+          const bool is_v = c & 1;
+          const long long pitch = is_v ? a.s.v_row : a.s.k_row;
+          const T *src = reinterpret_cast<const T *>(is_v ? a.v : a.k) + (item.k_row + (long long)key0) * pitch +
+                         kv * (is_v ? a.s.v_head : a.s.k_head);
+          load_tile<T, kTileRows>(ring + stage * tile_bytes, src, pitch, min(kTileRows, item.m - key0), d, chunks, t);
+          cp_async_commit();
+          cp_async_wait<0>();
+          fence_async_proxy();
+          named_sync(1, kTileRows);
+          if (t == 0) mbar_arrive(bar(s_bar.kv_full[stage]));
+        }
+        named_sync(1, kTileRows);  // s_stop is written again; the item has been read by all
+        if (gave_up) break;
+        first += 2 * n_steps;
+        if (t == 0) done_item(x);
       }
-    } else if (warp == 8 && n_steps > 0) {
+      if (t == 0 && (!ok || s_fail)) {  // copies in flight land before the block ends
+        mbar_wait(bar(s_bar.q_full), 0);
+        for (int c = max(0, copied - kStages); c < copied; c++) mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
+      }
+    } else if (warp == 9) {
+      // ---- what to work on: tiles of all sequences counted through, the longest queries of each first, every
+      // tile for all heads; this CTA takes every gridDim.x-th
+      int s0 = 0, before = 0, all = 0, upto = 0, count = 0;
+      bool loaded = false;
+      for (int x = 0;; x++) {
+        const long long number = blockIdx.x + (long long)x * gridDim.x;
+        const int tile = (int)(number / a.s.heads), head = (int)(number - (long long)tile * a.s.heads);
+        PromptItem item{};
+        item.head = head;
+        while (number < n_items) {
+          if (!loaded) {
+            const int2 r = s0 + lane < a.s.n_seqs ? packed_rows(a.cu_q, s0 + lane, a.s.total_q) : make_int2(0, 0);
+            count = (r.y - r.x + 2 * kTileRows - 1) / (2 * kTileRows);
+            upto = count;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int y = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += y;
+            }
+            all = __shfl_sync(0xffffffffu, upto, 31);
+            loaded = true;
+          }
+          if (tile < before + all) {
+            const unsigned who = __ballot_sync(0xffffffffu, tile < before + upto);
+            const int l = __ffs(who) - 1;
+            const int end = __shfl_sync(0xffffffffu, before + upto, l);
+            const int2 rq = packed_rows(a.cu_q, s0 + l, a.s.total_q), rk = packed_rows(a.cu_k, s0 + l, a.s.total_k);
+            item.valid = 1;
+            item.q_row = rq.x;
+            item.n = rq.y - rq.x;
+            item.k_row = rk.x;
+            item.m = rk.y - rk.x;
+            item.row0 = (end - 1 - tile) * 2 * kTileRows;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int r = item.row0 + i * kTileRows, rows = min(kTileRows, item.n - r);
+              const int last = r + rows - 1 + item.m - item.n;
+              item.steps[i] = rows <= 0 || last < 0 ? 0 : last / kTileRows + 1;
+            }
+            break;
+          }
+          before += all;
+          s0 += 32;
+          loaded = false;
+          if (s0 >= a.s.n_seqs) break;
+        }
+        bool ok = x < kItems || wait_or_fail(bar(s_bar.item_empty[x % kItems]), (x / kItems - 1) & 1, &s_fail);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) {
+          s_item[x % kItems] = item;
+          mbar_arrive(bar(s_bar.item_full[x % kItems]));
+        }
+        __syncwarp();
+        if (!item.valid) break;
+      }
+    } else if (warp == 8) {
       // ---- matrix instructions: the whole warp walks along, one elected lane issues
       const bool bf16 = a.s.dtype == QMOE_BF16;
       const uint32_t idesc_s = make_instr_desc(kTileRows, kTileRows, bf16);
       const uint32_t idesc_o = make_instr_desc(kTileRows, 8 * chunks, bf16, true);
-      auto tile_addr = [&](int item) { return smem_u32(ring) + (item % kStages) * tile_bytes; };
-      auto wait_tile = [&](int item) {
-        return __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.kv_full[item % kStages]), (item / kStages) & 1, &s_fail));
+      int first = 0, done[2] = {0, 0};  // buffers used and products of each tile before this item
+      auto tile_addr = [&](int c) { return smem_u32(ring) + ((first + c) % kStages) * tile_bytes; };
+      auto wait_tile = [&](int c) {
+        return __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.kv_full[(first + c) % kStages]), ((first + c) / kStages) & 1, &s_fail));
       };
       auto scores = [&](int i, int j) {
         const uint64_t qa = make_swizzled_desc(smem_u32(q_tile) + i * tile_bytes, 16, 1024);
@@ -372,38 +442,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         }
         mma_commit_warp(bar(s_bar.s_full[i]));
       };
-      bool ok = !tma || __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.q_full), 0, &s_fail));
-      ok = ok && wait_tile(0);
-      if (ok) {
-        tc_fence_after();
-        for (int i = 0; i < 2; i++)
-          if (steps[i] > 0) scores(i, 0);
-        mma_commit_warp(bar(s_bar.kv_empty[0]));
-      }
-      for (int j = 0; ok && j < n_steps; j++) {
-        const bool more = j + 1 < n_steps;
-        ok = wait_tile(2 * j + 1) && (!more || wait_tile(2 * j + 2));
+      bool ok = true;
+      for (int x = 0;; x++) {
+        PromptItem item;
+        ok = __all_sync(0xffffffffu, get_item(x, item));
+        if (!ok || !item.valid) break;
+        const int n_steps = max(item.steps[0], item.steps[1]);
+        ok = __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.q_full), x & 1, &s_fail));
+        if (n_steps > 0) {
+          ok = ok && wait_tile(0);
+          if (!ok) break;
+          tc_fence_after();
+          for (int i = 0; i < 2; i++)
+            if (item.steps[i] > 0) scores(i, 0);
+          mma_commit_warp(bar(s_bar.kv_empty[first % kStages]));
+        }
+        if (!ok) break;
+        if (n_steps <= 1) mma_commit_warp(bar(s_bar.q_empty));
+        for (int j = 0; ok && j < n_steps; j++) {
+          const bool more = j + 1 < n_steps;
+          ok = wait_tile(2 * j + 1) && (!more || wait_tile(2 * j + 2));
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          if (!ok || j >= steps[i]) continue;
-          uint64_t va = make_swizzled_desc(tile_addr(2 * j + 1), kBlockBytes, 1024);
+          for (int i = 0; i < 2; i++) {
+            if (!ok || j >= item.steps[i]) continue;
+            uint64_t va = make_swizzled_desc(tile_addr(2 * j + 1), kBlockBytes, 1024);
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            ok = ok && __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i][half]), j & 1, &s_fail));
+            for (int half = 0; half < 2; half++) {
+              ok = ok && __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i][half]), (done[i] + j) & 1, &s_fail));
+              if (!ok) continue;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 4 * half; kk < 4 * half + 4; kk++, va += 2048 >> 4)  // 16 keys each
+                mma_f16_ta_warp(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * kk, va, idesc_o, j > 0 || kk > 0);
+            }
             if (!ok) continue;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 4 * half; k < 4 * half + 4; k++, va += 2048 >> 4)  // 16 keys each
-              mma_f16_ta_warp(tmem + 256 + i * kTileRows, tmem + i * kTileRows + 8 * k, va, idesc_o, j > 0 || k > 0);
+            mma_commit_warp(bar(s_bar.pv_done[i]));
+            if (j + 1 < item.steps[i]) scores(i, j + 1);
           }
-          if (!ok) continue;
-          mma_commit_warp(bar(s_bar.pv_done[i]));
-          if (j + 1 < steps[i]) scores(i, j + 1);
+          if (ok) {
+            mma_commit_warp(bar(s_bar.kv_empty[(first + 2 * j + 1) % kStages]));
+            if (more) mma_commit_warp(bar(s_bar.kv_empty[(first + 2 * j + 2) % kStages]));
+            if (j + 2 == n_steps) mma_commit_warp(bar(s_bar.q_empty));  // the last scores have been issued
+          }
         }
-        if (ok) {
-          mma_commit_warp(bar(s_bar.kv_empty[(2 * j + 1) % kStages]));
-          if (more) mma_commit_warp(bar(s_bar.kv_empty[(2 * j + 2) % kStages]));
-        }
+        if (!ok) break;
+        first += 2 * n_steps;
+        done[0] += item.steps[0];
+        done[1] += item.steps[1];
+        if (lane == 0) done_item(x);
       }
       if (!ok) {  // whatever is still in flight ends before tensor memory is freed
         mma_commit_warp(bar(s_bar.drain));
@@ -414,170 +500,187 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ---- softmax and output: thread t of the warpgroup owns query row t of its tile
     const int i = warp >> 2, t = tid & (kTileRows - 1);
-    const int row = row0 + i * kTileRows + t;
-    const bool live = row < n;
-    const int last = live ? row + shift : -1;  // last key that the query sees
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_s = lane_base + i * kTileRows, t_o = lane_base + 256 + i * kTileRows;
     const int o_cols = 8 * chunks;
     const float sl2 = a.s.scale * kLog2e;
-    const float *bias = BIAS ? a.bias + (size_t)head * a.s.n_dist : nullptr;
-    float top = -INFINITY, sum = 0.f;  // maximum that O and the sum are relative to, in units of log 2
+    int done = 0;  // key tiles before this item
     bool ok = true;
-    for (int j = 0; j < steps[i]; j++) {
-      ok = wait_or_fail(bar(s_bar.s_full[i]), j & 1, &s_fail);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      float s[kTileRows];
+    for (int x = 0;; x++) {
+      PromptItem item;
+      ok = __all_sync(0xffffffffu, get_item(x, item));
+      if (!ok || !item.valid) break;
+      __syncwarp();
+      if (lane == 0) done_item(x);
+      const int steps = item.steps[i], n = item.n, shift = item.m - item.n, head = item.head, row0 = item.row0;
+      const int row = row0 + i * kTileRows + t;
+      const bool live = row < n;
+      const int last = live ? row + shift : -1;  // last key that the query sees
+      const float *bias = BIAS ? a.bias + (size_t)head * a.s.n_dist : nullptr;
+      float top = -INFINITY, sum = 0.f;  // maximum that O and the sum are relative to, in units of log 2
+      for (int j = 0; j < steps; j++) {
+        ok = wait_or_fail(bar(s_bar.s_full[i]), (done + j) & 1, &s_fail);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        float s[kTileRows];
 #pragma unroll
-      for (int c = 0; c < 4; c++) tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
-      tmem_wait_ld();
-      const int key0 = j * kTileRows;
-      if (BIAS) {
-        // distances of the tile's keys from this query; all behind the last column: one value for all
-        const int first_row = row0 + i * kTileRows + shift;
-        if (first_row - (key0 + kTileRows - 1) >= a.s.n_dist - 1) {
-          const float b = in_log2(bias[a.s.n_dist - 1]);
+        for (int c = 0; c < 4; c++) tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+        tmem_wait_ld();
+        const int key0 = j * kTileRows;
+        if (BIAS) {
+          // distances of the tile's keys from this query; all behind the last column: one value for all
+          const int first_row = row0 + i * kTileRows + shift;
+          if (first_row - (key0 + kTileRows - 1) >= a.s.n_dist - 1) {
+            const float b = in_log2(bias[a.s.n_dist - 1]);
 #pragma unroll
-          for (int c = 0; c < kTileRows; c++) s[c] = fmaf(s[c], sl2, b);
-        } else {
+            for (int c = 0; c < kTileRows; c++) s[c] = fmaf(s[c], sl2, b);
+          } else {
 #pragma unroll
-          for (int c = 0; c < kTileRows; c++)
-            s[c] = fmaf(s[c], sl2, in_log2(__ldg(bias + max(0, min(last - key0 - c, a.s.n_dist - 1)))));
-        }
-      }
-      const int edge = last - key0;  // columns behind it are masked
-      const bool masked = __any_sync(0xffffffffu, edge < kTileRows - 1);
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < kTileRows; c++) s[c] = c <= edge ? s[c] : -INFINITY;
-      }
-      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
-#pragma unroll
-      for (int c = 4; c < kTileRows - 4; c += 8) {
-        m0 = max3(m0, s[c], s[c + 4]);
-        m1 = max3(m1, s[c + 1], s[c + 5]);
-        m2 = max3(m2, s[c + 2], s[c + 6]);
-        m3 = max3(m3, s[c + 3], s[c + 7]);
-      }
-      m0 = max3(m0, s[kTileRows - 4], s[kTileRows - 3]);
-      m1 = max3(m1, s[kTileRows - 2], s[kTileRows - 1]);
-      float tile_top = fmaxf(max3(m0, m1, m2), m3);
-      if (!BIAS) tile_top *= sl2;
-      const bool grow = tile_top > top + 8.f || (top == -INFINITY && tile_top > top);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float next = grow ? tile_top : top;
-        const float keep = grow ? exp2_approx(top - next) : 1.f;
-        top = next;
-        sum *= keep;
-        if (j > 0) {
-          ok = wait_or_fail(bar(s_bar.pv_done[i]), (j - 1) & 1, &s_fail);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          tc_fence_after();
-          for (int c = 0; c < o_cols; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(t_o + c, o);
-#pragma unroll
-            for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
-            tmem_st16(t_o + c, o);
+            for (int c = 0; c < kTileRows; c++)
+              s[c] = fmaf(s[c], sl2, in_log2(__ldg(bias + max(0, min(last - key0 - c, a.s.n_dist - 1)))));
           }
         }
-      }
-      const float base = top == -INFINITY ? 0.f : top;
-      const pair_t minus = pair_of(-base, -base), by = pair_of(sl2, sl2);
-      pair_t sums = pair_of(0.f, 0.f);
-      // `poly` of 8 pairs go through pair_exp2 (tiles without masked keys: it has no weight of exactly 0)
-      auto weights = [&](auto poly) {
+        const int edge = last - key0;  // columns behind it are masked
+        const bool masked = __any_sync(0xffffffffu, edge < kTileRows - 1);
+        if (masked) {
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
+          for (int c = 0; c < kTileRows; c++) s[c] = c <= edge ? s[c] : -INFINITY;
+        }
+        float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-          for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 32) {
-            uint32_t p[16];
+        for (int c = 4; c < kTileRows - 4; c += 8) {
+          m0 = max3(m0, s[c], s[c + 4]);
+          m1 = max3(m1, s[c + 1], s[c + 5]);
+          m2 = max3(m2, s[c + 2], s[c + 6]);
+          m3 = max3(m3, s[c + 3], s[c + 7]);
+        }
+        m0 = max3(m0, s[kTileRows - 4], s[kTileRows - 3]);
+        m1 = max3(m1, s[kTileRows - 2], s[kTileRows - 1]);
+        float tile_top = fmaxf(max3(m0, m1, m2), m3);
+        if (!BIAS) tile_top *= sl2;
+        const bool grow = tile_top > top + 8.f || (top == -INFINITY && tile_top > top);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float next = grow ? tile_top : top;
+          const float keep = grow ? exp2_approx(top - next) : 1.f;
+          top = next;
+          sum *= keep;
+          if (j > 0) {
+            ok = wait_or_fail(bar(s_bar.pv_done[i]), (done + j - 1) & 1, &s_fail);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+            for (int c = 0; c < o_cols; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
 #pragma unroll
-            for (int c = 0; c < 16; c++) {
-              const pair_t v = pair_of(s[c0 + 2 * c], s[c0 + 2 * c + 1]);
-              const pair_t x = BIAS ? pair_add(v, minus) : pair_fma(v, by, minus);
-              float lo, hi;
-              pair_t e;
-              if ((c * decltype(poly)::value) % 8 + decltype(poly)::value > 7 && decltype(poly)::value > 0) {
-                e = pair_exp2(x);
-                pair_split(e, lo, hi);
-              } else {
-                pair_split(x, lo, hi);
-                lo = exp2_approx(lo);
-                hi = exp2_approx(hi);
-                e = pair_of(lo, hi);
-              }
-              sums = pair_add(sums, e);
-              p[c] = pack2<T>(lo, hi);
+              for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+              tmem_st16(t_o + c, o);
             }
-            tmem_st16(t_s + c0 / 2, p);
           }
-          // the product over these 64 keys starts while the next are worked on
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(bar(s_bar.p_full[i][half]));
         }
-      };
-      if (BIAS || masked) weights(std::integral_constant<int, 0>());
-      else weights(std::integral_constant<int, kPolyPairs>());
-      float sum0, sum1;
-      pair_split(sums, sum0, sum1);
-      sum += sum0 + sum1;
-    }
-    if (ok && steps[i] > 0) {
-      ok = wait_or_fail(bar(s_bar.pv_done[i]), (steps[i] - 1) & 1, &s_fail);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
-    if (ok) {
-      // Rows go through shared memory (the query tile's, which nothing reads any more) so that a warp writes
-      // them one after another instead of one piece of 32 rows at a time.
+        const float base = top == -INFINITY ? 0.f : top;
+        const pair_t minus = pair_of(-base, -base), by = pair_of(sl2, sl2);
+        pair_t sums = pair_of(0.f, 0.f);
+        // `poly` of 8 pairs go through pair_exp2 (tiles without masked keys: it has no weight of exactly 0)
+        auto weights = [&](auto poly) {
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+#pragma unroll
+            for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 32) {
+              uint32_t p[16];
+#pragma unroll
+              for (int c = 0; c < 16; c++) {
+                const pair_t v = pair_of(s[c0 + 2 * c], s[c0 + 2 * c + 1]);
+                const pair_t x = BIAS ? pair_add(v, minus) : pair_fma(v, by, minus);
+                float lo, hi;
+                pair_t e;
+                if ((c * decltype(poly)::value) % 8 + decltype(poly)::value > 7 && decltype(poly)::value > 0) {
+                  e = pair_exp2(x);
+                  pair_split(e, lo, hi);
+                } else {
+                  pair_split(x, lo, hi);
+                  lo = exp2_approx(lo);
+                  hi = exp2_approx(hi);
+                  e = pair_of(lo, hi);
+                }
+                sums = pair_add(sums, e);
+                p[c] = pack2<T>(lo, hi);
+              }
+              tmem_st16(t_s + c0 / 2, p);
+            }
+            // the product over these 64 keys starts while the next are worked on
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(s_bar.p_full[i][half]));
+          }
+        };
+        if (BIAS || masked) weights(std::integral_constant<int, 0>());
+        else weights(std::integral_constant<int, kPolyPairs>());
+        float sum0, sum1;
+        pair_split(sums, sum0, sum1);
+        sum += sum0 + sum1;
+      }
+      if (!ok) break;
+      if (steps > 0) {
+        ok = wait_or_fail(bar(s_bar.pv_done[i]), (done + steps - 1) & 1, &s_fail);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (!ok) break;
+      done += steps;
+      // Rows go through shared memory, 64 columns at a time, so that a warp writes them one after another instead
+      // of one piece of 32 rows at a time.
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      uint8_t *stage = q_tile + i * tile_bytes;
-      bool finite = true;
-      for (int c = 0; c < o_cols; c += 16) {
-        uint32_t o[16], w[8];
-        if (steps[i] > 0) {
-          tmem_ld16(t_o + c, o);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 16; x++) o[x] = 0u;
-        }
-#pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const float lo = __uint_as_float(o[2 * x]) * inv, hi = __uint_as_float(o[2 * x + 1]) * inv;
-          finite = finite && fabsf(lo) <= FLT_MAX && fabsf(hi) <= FLT_MAX;
-          w[x] = pack2<T>(lo, hi);
-        }
-        *reinterpret_cast<uint4 *>(stage + tile_offset(t, c >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4 *>(stage + tile_offset(t, (c >> 3) + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      __syncwarp();
+      uint8_t *stage = stage_out + warp * 4096;
       const int t0 = t & ~31, rows = min(32, n - (row0 + i * kTileRows + t0));  // of this warp
-      T *out = reinterpret_cast<T *>(a.out) + (rq.x + (long long)(row0 + i * kTileRows + t0)) * a.s.out_row + head * a.s.out_head;
-      if (((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.s.out_row * 2) | (uintptr_t)(d * 2)) & 15u) == 0) {
-        const int units = d / 8, shift = units > 8 ? 4 : (units > 4 ? 3 : 2), u = lane & ((1 << shift) - 1);
-        for (int r = lane >> shift; r < rows && u < units; r += 32 >> shift)
-          *reinterpret_cast<uint4 *>(out + r * a.s.out_row + 8 * u) = *reinterpret_cast<const uint4 *>(stage + tile_offset(t0 + r, u));
-      } else {
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-          for (int c = lane; c < d; c += 32) {
-            T v[8];
+      T *out = reinterpret_cast<T *>(a.out) + (item.q_row + (long long)(row0 + i * kTileRows + t0)) * a.s.out_row + head * a.s.out_head;
+      const bool vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.s.out_row * 2) | (uintptr_t)(d * 2)) & 15u) == 0;
+      bool finite = true;
+      for (int c0 = 0; c0 < o_cols; c0 += 64) {
+        for (int c = c0; c < min(o_cols, c0 + 64); c += 16) {
+          uint32_t o[16], w[8];
+          if (steps > 0) {
+            tmem_ld16(t_o + c, o);
+          } else {
 #pragma unroll
-            for (int r = 0; r < 8; r++) v[r] = *reinterpret_cast<const T *>(stage + tile_offset(t0 + r0 + r, c >> 3) + 2 * (c & 7));
+            for (int y = 0; y < 16; y++) o[y] = 0u;
+          }
 #pragma unroll
-            for (int r = 0; r < 8; r++)
-              if (r0 + r < rows) out[(r0 + r) * a.s.out_row + c] = v[r];
+          for (int y = 0; y < 8; y++) {
+            const float lo = __uint_as_float(o[2 * y]) * inv, hi = __uint_as_float(o[2 * y + 1]) * inv;
+            finite = finite && fabsf(lo) <= FLT_MAX && fabsf(hi) <= FLT_MAX;
+            w[y] = pack2<T>(lo, hi);
+          }
+          const int unit = (c & 63) >> 3;
+          *reinterpret_cast<uint4 *>(stage + lane * 128 + ((unit ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4 *>(stage + lane * 128 + (((unit + 1) ^ (lane & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+        __syncwarp();
+        const int cols = min(64, d - c0);
+        if (vec) {
+          const int u = lane & 7;
+          for (int r = lane >> 3; r < rows && u < cols / 8; r += 4)
+            *reinterpret_cast<uint4 *>(out + r * a.s.out_row + c0 + 8 * u) = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+        } else {
+          for (int r0 = 0; r0 < rows; r0 += 8) {
+            for (int c = lane; c < cols; c += 32) {
+              T v[8];
+#pragma unroll
+              for (int r = 0; r < 8; r++)
+                v[r] = *reinterpret_cast<const T *>(stage + (r0 + r) * 128 + (((c >> 3) ^ (r & 7)) << 4) + 2 * (c & 7));
+#pragma unroll
+              for (int r = 0; r < 8; r++)
+                if (r0 + r < rows) out[(r0 + r) * a.s.out_row + c0 + c] = v[r];
+            }
           }
         }
+        __syncwarp();
       }
-      __syncwarp();
+      tc_fence_before();
       unsigned again = __ballot_sync(0xffffffffu, live && !finite);
       while (again != 0) {
         const int l = __ffs(again) - 1;
         again &= again - 1;
-        attend_row<T, 4>(a, head, rq.x + row0 + i * kTileRows + (t & ~31) + l, rq, rk);
+        attend_row<T, 4>(a, head, item.q_row + row0 + i * kTileRows + t0 + l, make_int2(item.q_row, item.q_row + n), make_int2(item.k_row, item.k_row + item.m));
       }
     }
   }
@@ -673,13 +776,15 @@ static int run_prompt(PromptArgs a, void *work, int device, cudaStream_t stream)
   const bool tma = make_map(&maps.q, a.q, a.s.dtype, a.s.head_dim, a.s.heads, a.s.total_q, a.s.q_head, a.s.q_row) &&
                    make_map(&maps.k, a.k, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.k_head, a.s.k_row) &&
                    make_map(&maps.v, a.v, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.v_head, a.s.v_row);
-  const int smem = (2 + kStages) * ((a.s.head_dim + 63) / 64) * kBlockBytes + 1024;
+  const int smem = (2 + kStages) * ((a.s.head_dim + 63) / 64) * kBlockBytes + 8 * 4096 + 1024;
   auto kernel = a.bias != nullptr ? k_prompt_tiles<T, true> : k_prompt_tiles<T, false>;
   // the warpgroups' register shares have to fit what the block is launched with
   const int allowed = allow_shared(reinterpret_cast<const void *>(kernel), smem, device, kPromptRegs);
   if (allowed != QMOE_OK) return allowed;
-  const dim3 grid((unsigned)a.s.heads, (unsigned)((a.s.total_q + 2 * kTileRows - 1) / (2 * kTileRows) + a.s.n_seqs));
-  QMOE_LAUNCH(kernel, grid, kPromptThreads, smem, stream, a, maps, tma);
+  const long long n_items = a.s.heads * ((a.s.total_q + 2 * kTileRows - 1) / (2 * kTileRows) + a.s.n_seqs);  // at most
+  QMOE_REQUIRE(n_items <= 0x7fffffff, "too many heads");
+  const long long ctas = n_items < sm_count(device) ? n_items : sm_count(device);
+  QMOE_LAUNCH(kernel, (unsigned)ctas, kPromptThreads, smem, stream, a, maps, tma, (int)n_items);
   QMOE_CUDA(cudaGetLastError());
   return QMOE_OK;
 }
