@@ -68,14 +68,23 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 }
 
 // ---- tensor-core tiles ----------------------------------------------------------------------------
-// One CTA owns 256 queries of one head as two tiles of 128 and walks the keys 128 at a time:
+// One CTA per SM takes items of work one after another: 256 queries of one head as two tiles of 128, the keys
+// walked 128 at a time:
 //   S[128 queries, 128 keys] = Q K^T        both from shared memory, fp32 in tensor memory
 //   P = exp2(S * scale * log2 e - m)        by a warpgroup per query tile, one thread per query; P
 //                                           replaces S in tensor memory as 16-bit values
 //   O[128 queries, head_dim] += P V         P from tensor memory, V from shared memory
-// Roles: warps 0-3 and 4-7 the two softmax warpgroups, warp 8 issues the matrix instructions, warps
-// 12-15 copy key and value tiles into a ring of four buffers.  While one query tile's softmax runs, the
-// tensor core works for the other.
+// Roles: warps 0-3 and 4-7 the two softmax warpgroups, which also write the output; warp 8 issues the matrix
+// instructions; warp 9 finds out from the offsets what the items are; warps 12-15 copy queries, and keys and
+// values into a ring of four buffers.  While one query tile's softmax runs, the tensor core works for the other,
+// and the next item's tiles come in while this one's output is written (one CTA per item instead: 126 against
+// 110 us for 16 uneven prompts of 8192 tokens together, 32 heads of 128).
+//
+// Bound by the chain scores -> softmax -> product of each tile: a step of 2 x 128 queries by 128 keys takes 3200
+// to 3600 clocks, of which the tensor core works 2048 at head_dim 128.  The exponentials are the softmax's
+// largest part (a special function unit gives 16 results a clock and SM: 2048 clocks a step), so two pairs of
+// eight are polynomials on the FMA units (1165 instead of 1143 TFLOP/s over one prompt of 8192 tokens).
+// One prompt of 16384 tokens, 32 heads of 128: 1.96 to 2.01 ms, 1.1 PFLOP/s.
 // Every tile lies in shared memory as rows of 64 columns (128 bytes) under the 128-byte swizzle, one block
 // of 128 rows per 64 columns: K-major for Q and K, and the same bytes with the head axis contiguous for V.
 // Tiles come by bulk tensor copies, a sequence's last, partial key tile by the copying warps, which write zeros
@@ -86,8 +95,8 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // weight); the sum is taken from the unrounded fp32 weights.
 // A value row that is not finite would spoil queries that give it weight 0 (0 * inf): a query row whose
 // result is not finite is computed again key by key.
-// All waits are bounded; when one runs out the CTA counts itself in d_prompt_timeouts, frees its tensor
-// memory and returns.
+// All waits are bounded (kPromptWait); when one runs out the CTA counts itself in d_prompt_timeouts, waits for its
+// copies in flight, frees its tensor memory and returns.
 constexpr int kPromptThreads = 512;
 constexpr int kPromptRegs = 128;  // at launch; the softmax warps then hold 192 and the others 64
 constexpr int kTileRows = 128;
@@ -109,13 +118,19 @@ struct PromptBars {
 };
 
 // Waits for a phase of a barrier for kPromptWait nanoseconds at most, or until another wait of the CTA ran out.
+// `fail[1]` counts what takes long by design: while it moves, the wait begins again.
 __device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, volatile int *fail) {
   if (mbar_wait(bar, parity, 2)) return true;
   unsigned long long now, begin;
+  int seen = fail[1];
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
   do {
     if (mbar_wait(bar, parity, 2)) return true;
     if (*fail) return false;
+    if (seen != fail[1]) {
+      seen = fail[1];
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
+    }
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
   } while (now - begin < kPromptWait);
   *fail = 1;
@@ -195,7 +210,7 @@ __device__ __forceinline__ void load_tile(uint8_t *tile, const T *src, long long
 // Copies of tensors whose rows do not begin on 16-byte boundaries, as [rows][heads][pitch] with pitch = head_dim
 // rounded up to 8 (what stands behind the head's values is not read).  A pass over the inputs is little next to
 // the attention itself; copying such rows value by value inside it was slower even for one tile of 128 queries
-// (25 us against PACKED us for 32 heads of 65).
+// (25 us against 13 us for 32 heads of 65).
 struct PackArgs {
   const void *src[3];
   void *dst[3];
@@ -232,7 +247,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
   __shared__ PromptBars s_bar;
   __shared__ PromptItem s_item[kItems];
   __shared__ uint32_t s_tmem;
-  __shared__ volatile int s_fail;
+  __shared__ volatile int s_fail[2];
   __shared__ volatile int s_stop[2];
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -259,7 +274,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
     mbar_init(bar(s_bar.q_full), 1);
     mbar_init(bar(s_bar.q_empty), 1);
     mbar_init(bar(s_bar.drain), 1);
-    s_fail = 0;
+    s_fail[0] = s_fail[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(smem_u32(&s_tmem), 512);
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
   // Item number `x` of this CTA, by every thread that uses it; false when a wait ran out.  Given back by
   // done_item, once per warp that reads items (the copying warps: once).
   auto get_item = [&](int x, PromptItem &item) {
-    const bool ok = wait_or_fail(bar(s_bar.item_full[x % kItems]), (x / kItems) & 1, &s_fail);
+    const bool ok = wait_or_fail(bar(s_bar.item_full[x % kItems]), (x / kItems) & 1, s_fail);
     item = s_item[x % kItems];
     return ok;
   };
@@ -295,7 +310,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         const int n_steps = max(item.steps[0], item.steps[1]), kv = item.head / group;
         const int n_tma = tma ? 2 * min(n_steps, item.m / kTileRows) : 0;  // whole key tiles come by bulk copies
         if (n_steps > 0) {
-          if (t == 0 && x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, &s_fail);
+          if (t == 0 && x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, s_fail);
           if (tma && t == 0 && ok) {
             const uint32_t q_full = bar(s_bar.q_full);
             mbar_arrive_tx(q_full, (uint32_t)((item.steps[0] > 0) + (item.steps[1] > 0)) * tile_bytes);
@@ -319,13 +334,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
             if (t == 0) mbar_arrive(bar(s_bar.q_full));
           }
         } else if (t == 0) {
-          if (x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, &s_fail);
+          if (x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, s_fail);
           mbar_arrive(bar(s_bar.q_full));  // nothing to copy: the phases go on
         }
         if (t == 0) {
           for (int c = 0; ok && c < n_tma; c++) {
             const int at = first + c, stage = at % kStages;
-            if (at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, &s_fail);
+            if (at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, s_fail);
             if (!ok) break;
             const uint32_t full = bar(s_bar.kv_full[stage]);
             mbar_arrive_tx(full, tile_bytes);
@@ -340,7 +355,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         for (int c = n_tma; c < 2 * n_steps; c++) {
           const int at = first + c, stage = at % kStages;
           if (t == 0) {
-            if (ok && at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, &s_fail);
+            if (ok && at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, s_fail);
             s_stop[c & 1] = !ok;
           }
           named_sync(1, kTileRows);
@@ -363,13 +378,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         first += 2 * n_steps;
         if (t == 0) done_item(x);
       }
-      if (t == 0 && (!ok || s_fail)) {  // copies in flight land before the block ends
+      if (t == 0 && (!ok || s_fail[0])) {  // copies in flight land before the block ends
         mbar_wait(bar(s_bar.q_full), 0);
         for (int c = max(0, copied - kStages); c < copied; c++) mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
       }
     } else if (warp == 9) {
       // ---- what to work on: tiles of all sequences counted through, the longest queries of each first, every
-      // tile for all heads; this CTA takes every gridDim.x-th
+      // tile for all heads; this CTA takes every gridDim.x-th.  (Every second round backwards, or CTAs that have
+      // not started taken over by those that run, ended within 2 % of this: 110 to 117 us, and 1976 to 2014 us for
+      // one prompt of 16384 tokens.)
       int s0 = 0, before = 0, all = 0, upto = 0, count = 0;
       bool loaded = false;
       for (int x = 0;; x++) {
@@ -414,7 +431,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
           loaded = false;
           if (s0 >= a.s.n_seqs) break;
         }
-        bool ok = x < kItems || wait_or_fail(bar(s_bar.item_empty[x % kItems]), (x / kItems - 1) & 1, &s_fail);
+        bool ok = x < kItems || wait_or_fail(bar(s_bar.item_empty[x % kItems]), (x / kItems - 1) & 1, s_fail);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) {
           s_item[x % kItems] = item;
@@ -431,7 +448,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       int first = 0, done[2] = {0, 0};  // buffers used and products of each tile before this item
       auto tile_addr = [&](int c) { return smem_u32(ring) + ((first + c) % kStages) * tile_bytes; };
       auto wait_tile = [&](int c) {
-        return __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.kv_full[(first + c) % kStages]), ((first + c) / kStages) & 1, &s_fail));
+        return __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.kv_full[(first + c) % kStages]), ((first + c) / kStages) & 1, s_fail));
       };
       auto scores = [&](int i, int j) {
         const uint64_t qa = make_swizzled_desc(smem_u32(q_tile) + i * tile_bytes, 16, 1024);
@@ -448,7 +465,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         ok = __all_sync(0xffffffffu, get_item(x, item));
         if (!ok || !item.valid) break;
         const int n_steps = max(item.steps[0], item.steps[1]);
-        ok = __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.q_full), x & 1, &s_fail));
+        ok = __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.q_full), x & 1, s_fail));
         if (n_steps > 0) {
           ok = ok && wait_tile(0);
           if (!ok) break;
@@ -468,7 +485,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
             uint64_t va = make_swizzled_desc(tile_addr(2 * j + 1), kBlockBytes, 1024);
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-              ok = ok && __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i][half]), (done[i] + j) & 1, &s_fail));
+              ok = ok && __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.p_full[i][half]), (done[i] + j) & 1, s_fail));
               if (!ok) continue;
               tc_fence_after();
 #pragma unroll
@@ -519,7 +536,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       const float *bias = BIAS ? a.bias + (size_t)head * a.s.n_dist : nullptr;
       float top = -INFINITY, sum = 0.f;  // maximum that O and the sum are relative to, in units of log 2
       for (int j = 0; j < steps; j++) {
-        ok = wait_or_fail(bar(s_bar.s_full[i]), (done + j) & 1, &s_fail);
+        ok = wait_or_fail(bar(s_bar.s_full[i]), (done + j) & 1, s_fail);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         float s[kTileRows];
@@ -565,7 +582,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
           top = next;
           sum *= keep;
           if (j > 0) {
-            ok = wait_or_fail(bar(s_bar.pv_done[i]), (done + j - 1) & 1, &s_fail);
+            ok = wait_or_fail(bar(s_bar.pv_done[i]), (done + j - 1) & 1, s_fail);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
             for (int c = 0; c < o_cols; c += 16) {
@@ -621,7 +638,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       }
       if (!ok) break;
       if (steps > 0) {
-        ok = wait_or_fail(bar(s_bar.pv_done[i]), (done + steps - 1) & 1, &s_fail);
+        ok = wait_or_fail(bar(s_bar.pv_done[i]), (done + steps - 1) & 1, s_fail);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
@@ -680,13 +697,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       while (again != 0) {
         const int l = __ffs(again) - 1;
         again &= again - 1;
+        s_fail[1] = s_fail[1] + 1;  // any change will do
         attend_row<T, 4>(a, head, item.q_row + row0 + i * kTileRows + t0 + l, make_int2(item.q_row, item.q_row + n), make_int2(item.k_row, item.k_row + item.m));
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && s_fail) atomicAdd(&d_prompt_timeouts, 1);
+  if (tid == 0 && s_fail[0]) atomicAdd(&d_prompt_timeouts, 1);
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
@@ -814,8 +832,8 @@ extern "C" int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, v
   QMOE_REQUIRE(isfinite(a.s.scale), "scale is not finite");
   if (a.s.n_seqs == 0 || a.s.total_q == 0) return QMOE_OK;
   QMOE_REQUIRE(a.q && a.out && (a.s.total_k == 0 || (a.k && a.v)), "null device pointer");
-  if (a.s.head_dim > 256 || a.s.total_q > (1 << 18) - 4 || a.s.total_k > 0x7fffffffLL || a.s.n_seqs > 32768) {
-    set_error("%s: head_dim <= 256, 262140 query rows, 2^31 - 1 key rows and 32768 sequences are supported", __func__);
+  if (a.s.head_dim > 256 || a.s.total_q > (1 << 18) - 4 || a.s.total_k > (1 << 25) || a.s.n_seqs > 32768) {
+    set_error("%s: head_dim <= 256, 262140 query rows, 2^25 key rows and 32768 sequences are supported", __func__);
     return QMOE_ERR_UNSUPPORTED;
   }
   QMOE_REQUIRE(qmoe_prompt_work_bytes(args) == 0 || (args->work_dev != nullptr && (reinterpret_cast<uintptr_t>(args->work_dev) & 255u) == 0),

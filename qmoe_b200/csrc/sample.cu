@@ -97,6 +97,9 @@ __device__ __forceinline__ V block_total(V v, V *scratch) {
 // the row to sample_by_radix, which reads it again from global memory.
 // What bounds it: the 64-bit exponentials where the whole row is kept (eleven operations a logit at 64 a clock
 // and SM), exchanges between the CTAs (a microsecond each) for few rows.
+// 256 rows of 131072 fp32 logits (134 MB): 85 us for the largest alone, 157 with the masses of the whole row, 164 with a
+// top_k of 50, 353 with a top_p of 0.9; of that about 11 us go to the start and end of each wave of clusters.  Four
+// rows of 32128: 8 us.
 constexpr int kRowThreads = 512;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kBins = 1024;
