@@ -288,8 +288,12 @@ class SwitchDecoderLM:
             raise ValueError("start_batch needs at least one prompt, and no empty one")
         if n_new < 0 or max(lens) + n_new > self.max_len:
             raise ValueError(f"prompt and new tokens must fit max_len = {self.max_len}")
+        ids = torch.cat([p.reshape(-1) for p in prompts]).to(self.dev)
+        lowest, highest = (int(v) for v in ids.aminmax())
+        if lowest < 0 or highest >= self.embed.shape[0]:
+            raise ValueError(f"prompt ids must lie in [0, {self.embed.shape[0]}), got {lowest} to {highest}")
         state = BatchState(self, lens, n_new, cache_format, page_size)
-        x = self.embed[torch.cat([p.reshape(-1) for p in prompts]).to(self.dev)]
+        x = self.embed[ids]
         n = x.shape[0]
         for b, cache in zip(self.blocks, state.caches):
             qkv = (_rms_norm(x, b["ln1"]) @ b["wqkv"].t()).view(n, 3, self.h, self.hd)
@@ -305,8 +309,11 @@ class SwitchDecoderLM:
     def step_batch(self, state: "BatchState", tokens: torch.Tensor) -> torch.Tensor:
         """One more token (int64[n]) for every sequence of ``state``; returns the logits fp32 ``[n, vocab]``
         behind them.  The position is ``state.lengths``, which the caller moves on (``+= 1``), so that the call
-        can be captured and replayed."""
-        x = self.embed[tokens]
+        can be captured and replayed.  Ids outside the vocabulary (the -1 of a row that could not be sampled)
+        are read as the nearest one inside."""
+        if tokens.shape != state.lengths.shape:
+            raise ValueError(f"tokens must have an entry per sequence ({state.lengths.numel()}), got {tuple(tokens.shape)}")
+        x = self.embed[tokens.clamp(0, self.embed.shape[0] - 1)]
         n = x.shape[0]
         seen = state.lengths + 1
         for b, cache in zip(self.blocks, state.caches):
@@ -326,6 +333,8 @@ class SwitchDecoderLM:
         a CUDA graph for this call when there are enough steps."""
         if n_new < 1:
             raise ValueError("n_new must be at least 1")
+        if not 0.0 <= temperature < float("inf"):
+            raise ValueError(f"temperature must be finite and not negative, got {temperature}")
         n = len(prompts)
         if uniform is None:
             uniform = torch.rand((n_new, n), device=self.dev)
@@ -362,7 +371,11 @@ class SwitchDecoderLM:
         refused = sum(c.refused() for c in state.caches)
         if refused:
             raise RuntimeError(f"{refused} cache positions had no page")
-        return torch.stack(out, 1)
+        tokens = torch.stack(out, 1)
+        lost = (tokens < 0).any(1).nonzero().flatten().tolist()
+        if lost:
+            raise RuntimeError(f"logits of sequences {lost} were no distribution (NaN or infinite)")
+        return tokens
 
     def close(self) -> None:
         """Destroy the captured decode graph (before tearing down a process group it captured)."""

@@ -68,6 +68,28 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _check_out(out: torch.Tensor, inputs) -> None:
+    """Refuses an output whose rows share memory with each other or with an input."""
+    if out.numel() == 0:
+        return
+    reach = out.shape[2]  # values of what is laid out so far: a head's row, then the axes from the smaller stride up
+    for stride, size in sorted((st, n) for st, n in zip(out.stride()[:2], out.shape[:2]) if n > 1):
+        if stride < reach:
+            raise ValueError("rows of out must not share memory")
+        reach += stride * (size - 1)
+    end = out.data_ptr() + out.element_size() * reach
+    for name, t in inputs:
+        if t.numel() and t.data_ptr() < end and out.data_ptr() < t.data_ptr() + t.element_size() * (
+                1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))):
+            raise ValueError(f"out must lie apart from {name}")
+
+
+def _scale(scale: float) -> float:
+    if not scale >= 0.0:
+        raise ValueError(f"scale must not be negative (0: 1 / sqrt(head_dim)), got {scale}")
+    return scale
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
                      cu_k: Optional[torch.Tensor] = None, scale: float = 0.0,
                      rel_bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -80,8 +102,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     sequence; a query that sees no key gives zeros.  ``scale`` multiplies the scores (0:
     ``1 / sqrt(head_dim)``; T5 / Switch attention uses 1); ``rel_bias`` fp32 ``[heads, n]`` is added
     to them at column ``min(distance, n - 1)``, the distance between query and key.  Keys whose bias
-    is ``-inf`` are masked, whatever they hold.  Returns ``out`` ``[total_q, heads, head_dim]``; rows
-    that no sequence owns are left as they were (uninitialised when ``out`` is not given)."""
+    is ``-inf`` are masked, whatever they hold.  Returns ``out`` ``[total_q, heads, head_dim]`` (any strides
+    over the first two axes, memory apart from the inputs'); rows that no sequence owns are left as they
+    were (uninitialised when ``out`` is not given)."""
     _need(q, "q", (torch.bfloat16, torch.float16), 3, packed=False)
     dev = q.device
     for name, t in (("k", k), ("v", v)):
@@ -103,11 +126,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         _need(out, "out", q.dtype, 3, dev, packed=False)
         if out.shape != q.shape:
             raise ValueError("out must have the shape of q")
+        _check_out(out, (("q", q), ("k", k), ("v", v)))
     bias, n_dist = _bias_args(rel_bias, heads, dev)
     qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
     fields = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), bias, 0,
               total_q, total_k, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], cu_q.numel() - 1, heads, kv_heads,
-              hd, _DTYPES[q.dtype], n_dist, scale]
+              hd, _DTYPES[q.dtype], n_dist, _scale(scale)]
     L, args = _lib.load(), _lib.PROMPT_ARGS.pack(*fields)
     nbytes = L.qmoe_prompt_work_bytes(args)
     if nbytes:
@@ -127,7 +151,16 @@ class QuantCache:
     ``scale = max(amax / 448, 2^-126)`` (e4m3) or ``max(amax / 127, 2^-126)`` (int8) over the row of one
     head, the code is the nearest one.  A row with an infinity or NaN reads back as NaN.  Which pages
     hold which sequence is the caller's page table, int32 ``[n_seqs, max_pages]``.  ``status``
-    (int32[1] on the device) counts refused positions: see :meth:`refused`."""
+    (int32[1] on the device) counts refused positions: see :meth:`refused`.  The tensors are written in
+    place (``copy_``), not replaced: calls use the memory they had at the beginning."""
+
+    _fixed = frozenset(("k_codes", "v_codes", "k_scale", "v_scale", "status", "n_pages", "page_size", "kv_heads",
+                        "head_dim", "fmt", "device", "desc"))
+
+    def __setattr__(self, name, value):
+        if name in self._fixed and name in self.__dict__:
+            raise AttributeError(f"{name} of a QuantCache cannot be replaced (write into its tensors instead)")
+        super().__setattr__(name, value)
 
     def __init__(self, n_pages: int, page_size: int, kv_heads: int, head_dim: int, device, fmt: str = "e4m3"):
         if fmt not in FORMATS:
@@ -240,7 +273,7 @@ def decode_attention_paged(q: torch.Tensor, cache: QuantCache, page_table: torch
     nbytes = L.qmoe_decode_paged_work_bytes(n_seqs, heads, cache.kv_heads, hd, dev.index)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     args = _lib.PAGED_ARGS.pack(q.data_ptr(), out.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), bias, cache._status,
-                                _ptr(work), qs[0], qs[1], n_dist, n_seqs, heads, max_pages, _DTYPES[q.dtype], scale)
+                                _ptr(work), qs[0], qs[1], n_dist, n_seqs, heads, max_pages, _DTYPES[q.dtype], _scale(scale))
     _lib.check(L.qmoe_decode_attention_paged(cache._desc, args, dev.index, _stream(dev)))
     return out
 

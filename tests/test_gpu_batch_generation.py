@@ -135,3 +135,22 @@ def test_batch_refusals():
         model.generate_batch([one], 2, cache_format="fp4")
     assert model.generate_batch([one], 93).shape == (1, 93)               # up to max_len exactly
     assert isinstance(serving.QuantCache(0, 16, 1, 8, model.dev), serving.QuantCache)
+
+
+def test_ids_and_logits_that_cannot_be_used():
+    model = _model(n_layers=1)
+    one = torch.zeros(3, dtype=torch.int64)
+    for bad in (-1, VOCAB):
+        with pytest.raises(ValueError):
+            model.start_batch([one, one + bad], 1)
+    for temperature in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            model.generate_batch([one], 2, temperature=temperature)
+    state = model.start_batch([one, one], 4)
+    with pytest.raises(ValueError):
+        model.step_batch(state, torch.zeros(1, dtype=torch.int64, device=model.dev))
+    ids = torch.tensor([-1, VOCAB + 7], device=model.dev)          # the nearest inside
+    assert torch.equal(model.step_batch(state, ids), model.step_batch(state, torch.tensor([0, VOCAB - 1], device=model.dev)))
+    model.lm_head.fill_(float("nan"))
+    with pytest.raises(RuntimeError, match="no distribution"):
+        model.generate_batch([one, one], 6, temperature=1.0)

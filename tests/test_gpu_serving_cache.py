@@ -1,4 +1,5 @@
 """The quantised cache: append, read back and the attention over it, against plain 64-bit statements."""
+import copy
 import math
 
 import pytest
@@ -312,3 +313,26 @@ def test_offsets_beyond_32_bits():
     got = serving.decode_attention_paged(q, cache, table, _ints([1500]))
     kq = value * scale.double()[..., None]
     _check_decode(got, q, kq, kq, [1500], d ** -0.5)
+
+
+def test_the_cache_keeps_its_memory():
+    cache = serving.QuantCache(4, 16, 1, 64, DEV)
+    for name in ("k_codes", "v_codes", "k_scale", "v_scale", "status"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros_like(getattr(cache, name)))
+    with pytest.raises(AttributeError):
+        cache.page_size = 32
+    with pytest.raises(ValueError):
+        copy.deepcopy(cache)
+
+
+def test_a_cache_without_pages():
+    cache = serving.QuantCache(0, 16, 2, 64, DEV)
+    x = torch.randn(3, 2, 64, device=DEV).bfloat16()
+    for table in (_ints([[0, 1]]), torch.empty((1, 0), dtype=torch.int32, device=DEV)):
+        serving.cache_append(cache, x, x, _cu([3]), _ints([0]), table)
+        assert cache.refused(reset=True) == 3
+        k, v = serving.cache_read(cache, _cu([3]), _ints([0]), table, 3)
+        assert bool((k == 0).all()) and bool((v == 0).all()) and cache.refused(reset=True) == 3
+        assert bool((serving.decode_attention_paged(x[:1], cache, table, _ints([3])) == 0).all())
+        assert cache.refused(reset=True) == 2             # one tile, or one sequence, by two key heads

@@ -1,5 +1,6 @@
 """Prompt attention against a plain 64-bit statement: head layouts, lengths, strides, masks."""
 import math
+import random
 
 import pytest
 import torch
@@ -203,3 +204,49 @@ def test_same_bits_again_on_another_stream_and_in_a_replayed_graph():
         q.copy_(src)
         graph.replay()
         assert torch.equal(held, w)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_items_of_every_kind(d):
+    """More pieces of work than the GPU has multiprocessors, pieces without a key between long ones, and rows that
+    are computed again: one CTA works through all kinds."""
+    r = random.Random(d)
+    lens_q = [r.choice([0, 1, 3, 40, 128, 200, 300, 600]) for _ in range(150)]
+    lens_k = [max(0, n + r.choice([-n, -200, 0, 0, 0, 1, 130, 700])) for n in lens_q]
+    q, k, v = _case(lens_q, lens_k, 4, 2, d, torch.bfloat16, seed=14)
+    got = serving.prompt_attention(q, k, v, _cu(lens_q), _cu(lens_k))
+    _check(got, q, k, v, lens_q, lens_k, d ** -0.5)
+    # the last key of every fifth sequence is infinite: only the sequence's last query sees it
+    first, rows = 0, []
+    spoiled = v.clone()
+    for i, m in enumerate(lens_k):
+        if i % 5 == 0 and m > 0 and lens_q[i] > 0:
+            spoiled[first + m - 1] = math.inf
+            rows.append(sum(lens_q[:i + 1]) - 1)
+        first += m
+    again = serving.prompt_attention(q, k, spoiled, _cu(lens_q), _cu(lens_k))
+    keep = torch.ones(q.shape[0], dtype=torch.bool, device=DEV)
+    keep[rows] = False
+    _check(again.where(keep[:, None, None], got), q, k, v, lens_q, lens_k, d ** -0.5)
+    assert not bool(again[~keep].isfinite().any())
+
+
+@pytest.mark.parametrize("d", [64, 65])
+def test_key_rows_far_apart(d):
+    """Strides that carry the last rows more than 2^32 values behind the first."""
+    n, far = 40, (1 << 27) + 8
+    pool = torch.empty(far * (n - 1) + 2 * d, dtype=torch.bfloat16, device=DEV)
+    q, k0, v0 = _case([n], [n], 2, 1, d, torch.bfloat16, seed=15)
+    k, v = (pool[i * d:].as_strided((n, 1, d), (far, d, 1)) for i in range(2))
+    k.copy_(k0)
+    v.copy_(v0)
+    _check(serving.prompt_attention(q, k, v, _cu([n])), q, k0, v0, [n], [n], d ** -0.5)
+
+
+def test_output_refusals():
+    q, k, v = _case([8], [8], 2, 1, 64, torch.bfloat16)
+    for bad in (q, k.expand(8, 2, 64), torch.empty(1, 2, 64, dtype=q.dtype, device=DEV).expand(8, 2, 64), q.float(), q[:4]):
+        with pytest.raises((ValueError, TypeError)):
+            serving.prompt_attention(q, k, v, _cu([8]), out=bad)
+    with pytest.raises(ValueError):
+        serving.prompt_attention(q, k, v, _cu([8]), scale=-0.5)

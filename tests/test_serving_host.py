@@ -1,5 +1,6 @@
 """Refusals of the serving entry points, before any device is touched."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -159,3 +160,23 @@ def test_python_refusals_on_cpu_tensors():
             serving.QuantCache(**args)
     with pytest.raises(TypeError):
         serving.decode_attention_paged(x, None, cu, cu)
+
+
+def test_prompt_output_has_to_lie_apart():
+    buffer = torch.zeros(4, 3, 2, 64)
+    q, k, v = buffer[:, 0], buffer[:, 1], buffer[:, 2]
+    inputs = (("q", q), ("k", k), ("v", v))
+    for out in (q, v, buffer[:, 1].clone().expand(4, 2, 64)[:1].expand(4, 2, 64), torch.zeros(4, 1, 64).expand(4, 2, 64),
+                torch.zeros(4 * 64 + 64).as_strided((4, 2, 64), (64, 64, 1))):
+        with pytest.raises(ValueError):
+            serving._check_out(out, inputs)
+    for out in (torch.zeros(4, 2, 64), torch.zeros(2, 4, 64).transpose(0, 1), torch.zeros(4, 2, 80)[..., :64], torch.zeros(0, 2, 64)):
+        serving._check_out(out, inputs)
+    flat = torch.zeros(3 * 128)                                           # neighbours
+    serving._check_out(flat[128:256].view(1, 2, 64), (("q", flat[:128].view(1, 2, 64)), ("k", flat[256:].view(1, 2, 64))))
+
+
+@pytest.mark.parametrize("scale", [-1.0, float("nan"), -math.inf])
+def test_scale_is_not_negative(scale):
+    with pytest.raises(ValueError):
+        serving._scale(scale)
