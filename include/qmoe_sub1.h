@@ -444,8 +444,8 @@ typedef struct qmoe_prompt_args {
  * being i + m - n - j: the one-directional relative bias of T5 / Switch (scale 1).  Statistics and
  * sums are fp32.  At most 262140 query rows, 2^25 key rows and 32768 sequences a call.  A wait of the tensor-core kernel
  * that runs out is counted by qmoe_moe_tile_timeouts.  out_dev must not overlap q, k or v.  work_dev: qmoe_prompt_work_bytes bytes for the same
- * arguments (0 where every row of q, k and v begins on a 16-byte boundary), 256-byte aligned, not shared by
- * calls that may overlap. */
+ * arguments (0 where every row of q, k and v begins on a 16-byte boundary and there are queries enough to keep
+ * the GPU busy), 256-byte aligned, not shared by calls that may overlap. */
 int64_t qmoe_prompt_work_bytes(const qmoe_prompt_args *args);
 int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, void *stream);
 

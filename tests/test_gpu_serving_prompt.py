@@ -250,3 +250,73 @@ def test_output_refusals():
             serving.prompt_attention(q, k, v, _cu([8]), out=bad)
     with pytest.raises(ValueError):
         serving.prompt_attention(q, k, v, _cu([8]), scale=-0.5)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,dtype", [(8, 1, 128, torch.bfloat16), (3, 3, 65, torch.float16), (2, 1, 40, torch.bfloat16),
+                                                    (4, 4, 64, torch.float16), (1, 1, 127, torch.bfloat16)])
+@pytest.mark.parametrize("lens_q,lens_k", [([1], [5000]), ([130], [2100]), ([300], [1204]), ([600], [600]),
+                                           ([40, 0, 3], [3000, 700, 2]), ([129, 200], [4000, 90])])
+def test_few_queries_of_many_keys(lens_q, lens_k, heads, kv_heads, d, dtype):
+    """Calls whose keys are split among CTAs; some parts hold no key of a sequence."""
+    q, k, v = _case(lens_q, lens_k, heads, kv_heads, d, dtype, seed=16)
+    _check(serving.prompt_attention(q, k, v, _cu(lens_q), _cu(lens_k)), q, k, v, lens_q, lens_k, d ** -0.5)
+
+
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min])
+def test_parts_that_a_bias_masks(low):
+    """All keys but the nearest 100 are masked (whole parts of them), or all but the far ones."""
+    n, m, heads, d = 70, 3100, 2, 64
+    q, k, v = _case([n], [m], heads, 1, d, torch.bfloat16, seed=17)
+    g = torch.Generator(device=DEV).manual_seed(18)
+    bias = torch.randn(heads, 400, generator=g, device=DEV)
+    bias[0, 100:] = low
+    bias[1, :399] = low
+    got = serving.prompt_attention(q, k, v, _cu([n]), _cu([m]), scale=1.0, rel_bias=bias)
+    _check(got, q, k, v, [n], [m], 1.0, bias, exact_fn=ref.attention)
+    nothing = torch.full((heads, 3), -math.inf, device=DEV)
+    assert bool((serving.prompt_attention(q, k, v, _cu([n]), _cu([m]), rel_bias=nothing) == 0).all())
+
+
+def test_parts_with_values_that_are_not_finite():
+    n, m, heads, d = 200, 2500, 2, 128
+    q, k, v = _case([n], [m], heads, 1, d, torch.bfloat16, seed=19)
+    k[2400:] = math.nan                                      # seen by the last hundred queries only
+    v[2450:] = math.inf
+    got = serving.prompt_attention(q, k, v, _cu([n]), _cu([m]))
+    _check(got[:100], q[:100], k[:2400], v[:2400], [100], [2400], d ** -0.5)
+    assert bool(got[100:].isnan().all())
+
+
+def test_split_calls_leave_other_rows_and_follow_replayed_offsets():
+    heads, d, total = 2, 64, 150
+    q, k, v = _case([total], [4000], heads, 2, d, torch.bfloat16, seed=20)
+    wide = torch.full((total, heads, d + 9), 7.0, dtype=q.dtype, device=DEV)      # rows off 16-byte boundaries
+    cu_q, cu_k = _cu([90], first=20), _cu([3500], first=300)
+    graph = torch.cuda.CUDAGraph()
+    serving.prompt_attention(q, k, v, cu_q, cu_k, out=wide[..., 3:3 + d])
+    with torch.cuda.graph(graph):
+        serving.prompt_attention(q, k, v, cu_q, cu_k, out=wide[..., 3:3 + d])
+    for first_q, n, first_k, m in ((20, 90, 300, 3500), (0, 150, 0, 4000), (149, 1, 17, 130), (3, 5, 9, 0)):
+        cu_q.copy_(_cu([n], first=first_q))
+        cu_k.copy_(_cu([m], first=first_k))
+        wide.fill_(7.0)
+        graph.replay()
+        got = wide[first_q:first_q + n, :, 3:3 + d]
+        rows = slice(first_q, first_q + n), slice(first_k, first_k + m)
+        _check(got, q[rows[0]], k[rows[1]], v[rows[1]], [n], [m], d ** -0.5)
+        wide[first_q:first_q + n, :, 3:3 + d] = 7.0
+        assert bool((wide == 7.0).all())
+
+
+def test_split_calls_on_two_streams_at_once():
+    q, k, v = _case([64], [6000], 2, 1, 64, torch.bfloat16, seed=21)
+    cu_q, cu_k = _cu([64]), _cu([6000])
+    want = serving.prompt_attention(q, k, v, cu_q, cu_k)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(serving.prompt_attention(q, k, v, cu_q, cu_k))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)

@@ -180,3 +180,18 @@ def test_prompt_output_has_to_lie_apart():
 def test_scale_is_not_negative(scale):
     with pytest.raises(ValueError):
         serving._scale(scale)
+
+
+def test_prompt_workspace_of_split_keys():
+    size = lambda **kw: _lib.load().qmoe_prompt_work_bytes(_shape(**kw))  # noqa: E731
+    one = dict(n_seqs=1, heads=2, kv_heads=2, total_q=128, total_k=8192, q_row=128, k_row=128, v_row=128, q_head=64, k_head=64, v_head=64)
+    parts = lambda n, rows=128, heads=2: n * rows * heads * (64 + 2) * 4    # noqa: E731
+    assert size(**one) == parts(32)                                         # 64 key tiles, at most 32 parts
+    assert size(**{**one, "total_k": 1024}) == parts(4)                     # two tiles a part
+    assert size(**{**one, "total_k": 255}) == 0 and size(**{**one, "total_k": 0}) == 0
+    assert size(**{**one, "total_q": 20000}) == 0                           # queries enough
+    assert size(**{**one, "n_seqs": 64}) == 0                               # of 128 keys each
+    assert size(**{**one, "heads": 20, "kv_heads": 10, "total_q": 1280}) == 0
+    assert _prompt(_shape(**one)) == _lib.ERR_INVALID_ARG                   # needs a workspace
+    for bad in (dict(heads=0), dict(kv_heads=0), dict(n_seqs=0), dict(n_seqs=-1), dict(total_q=-1), dict(total_k=-1)):
+        assert size(**{**one, **bad}) == 0
