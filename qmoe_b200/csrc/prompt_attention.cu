@@ -252,7 +252,7 @@ struct PromptItem {
 
 template <typename T, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    const bool tma, const int n_items) {
+                                                                    const bool tma) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // the swizzle repeats every 1024 bytes
   __shared__ PromptBars s_bar;
@@ -394,44 +394,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         for (int c = max(0, copied - kStages); c < copied; c++) mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
       }
     } else if (warp == 9) {
-      // ---- what to work on: tiles of all sequences counted through, the longest queries of each first, every
-      // tile for all heads; this CTA takes every gridDim.x-th.  (Every second round backwards, or CTAs that have
-      // not started taken over by those that run, ended within 2 % of this: 110 to 117 us, and 1976 to 2014 us for
-      // one prompt of 16384 tokens.)
+      // ---- what to work on.  Of 32 sequences at a time, the tiles with the most key tiles first, every tile for all
+      // heads (and parts); dealt out to the CTAs forwards and backwards in turn.  Lane l holds sequence s0 + l and its
+      // next tile, counted from the sequence's end.
+      // (Sequence after sequence and only forwards, 16 uneven prompts of 8192 tokens took 125 us instead of 109, one of
+      // 8192 tokens 551 instead of 506; in this order but only forwards 120 and 552.  Taking over CTAs that had not been
+      // started, item by item, was no better than forwards.)
       const int item_rows = kTileRows + a.row_step, item_heads = 1 + a.head_step;
-      int s0 = 0, before = 0, all = 0, upto = 0, count = 0;
+      const int of_heads = a.s.heads / item_heads, per_tile = SPLIT ? of_heads * a.n_parts : of_heads;
+      int s0 = 0, next = -1, level = -1;
+      int2 rq = make_int2(0, 0), rk = rq;
+      long long before = 0;
       bool loaded = false;
+      auto key_tiles = [&](int i) {  // of the last row of tile i
+        const int last = min((i + 1) * item_rows, rq.y - rq.x) - 1 + (rk.y - rk.x) - (rq.y - rq.x);
+        return i < 0 ? -1 : (last < 0 ? 0 : last / kTileRows + 1);
+      };
       for (int x = 0;; x++) {
-        const long long number = blockIdx.x + (long long)x * gridDim.x;
-        const int of_heads = a.s.heads / item_heads, per_tile = SPLIT ? of_heads * a.n_parts : of_heads;
-        const int tile = (int)(number / per_tile), in_tile = (int)(number - (long long)tile * per_tile);
+        const long long number = (long long)x * gridDim.x + ((x & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         PromptItem item{};
-        item.part = SPLIT ? in_tile / of_heads : 0;
-        item.head = (in_tile - item.part * of_heads) * item_heads;
-        while (number < n_items) {
+        while (s0 < a.s.n_seqs) {
           if (!loaded) {
-            const int2 r = s0 + lane < a.s.n_seqs ? packed_rows(a.cu_q, s0 + lane, a.s.total_q) : make_int2(0, 0);
-            count = (r.y - r.x + item_rows - 1) / item_rows;
-            upto = count;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const int y = __shfl_up_sync(0xffffffffu, upto, o);
-              if (lane >= o) upto += y;
-            }
-            all = __shfl_sync(0xffffffffu, upto, 31);
+            const bool in = s0 + lane < a.s.n_seqs;
+            rq = in ? packed_rows(a.cu_q, s0 + lane, a.s.total_q) : make_int2(0, 0);
+            rk = in ? packed_rows(a.cu_k, s0 + lane, a.s.total_k) : make_int2(0, 0);
+            next = (rq.y - rq.x + item_rows - 1) / item_rows - 1;
+            level = key_tiles(next);
             loaded = true;
           }
-          if (tile < before + all) {
-            const unsigned who = __ballot_sync(0xffffffffu, tile < before + upto);
-            const int l = __ffs(who) - 1;
-            const int end = __shfl_sync(0xffffffffu, before + upto, l);
-            const int2 rq = packed_rows(a.cu_q, s0 + l, a.s.total_q), rk = packed_rows(a.cu_k, s0 + l, a.s.total_k);
+          const int top = __reduce_max_sync(0xffffffffu, level);
+          if (top < 0) {
+            s0 += 32;
+            loaded = false;
+            continue;
+          }
+          const unsigned who = __ballot_sync(0xffffffffu, level == top);
+          const long long count = (long long)__popc(who) * per_tile;
+          if (number < before + count) {
+            const long long in_level = number - before;
+            const int in_tile = (int)(in_level % per_tile), l = __fns(who, 0, (int)(in_level / per_tile) + 1);
             item.valid = 1;
-            item.q_row = rq.x;
-            item.n = rq.y - rq.x;
-            item.k_row = rk.x;
-            item.m = rk.y - rk.x;
-            item.row0 = (end - 1 - tile) * item_rows;
+            item.part = SPLIT ? in_tile / of_heads : 0;
+            item.head = (in_tile - item.part * of_heads) * item_heads;
+            item.q_row = __shfl_sync(0xffffffffu, rq.x, l);
+            item.n = __shfl_sync(0xffffffffu, rq.y, l) - item.q_row;
+            item.k_row = __shfl_sync(0xffffffffu, rk.x, l);
+            item.m = __shfl_sync(0xffffffffu, rk.y, l) - item.k_row;
+            item.row0 = __shfl_sync(0xffffffffu, next, l) * item_rows;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
               const int r = item.row0 + i * a.row_step, rows = min(kTileRows, item.n - r);
@@ -446,10 +455,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
             }
             break;
           }
-          before += all;
-          s0 += 32;
-          loaded = false;
-          if (s0 >= a.s.n_seqs) break;
+          before += count;
+          if (level == top) level = key_tiles(--next);
         }
         bool ok = x < kItems || wait_or_fail(bar(s_bar.item_empty[x % kItems]), (x / kItems - 1) & 1, s_fail);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -562,8 +569,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         if (BIAS) {
           // Distances of the tile's keys from the warp's queries: where all are behind the last column, one value for
           // all; else the 32 + 127 values that they can have, looked up while the scores are computed.  Query t
-          // and key c find theirs at t + 127 - c.  (Looked up by every query for every key instead, 2049 queries with 2826 keys and 12 heads of
-          // 64 took 45 us, now 37.)
+          // and key c find theirs at t + 127 - c.  (Looked up by every query for every key instead, 2049 queries
+          // with 2826 keys and 12 heads of 64 took 45 us instead of 37.)
           const int nearest = tile0 + (t & ~31) + shift - ((SPLIT ? item.tile0 : 0) + j) * kTileRows - (kTileRows - 1);
           far = nearest >= a.s.n_dist - 1;
           if (!far) {
@@ -946,7 +953,7 @@ static int run_prompt(PromptArgs a, void *work, int device, cudaStream_t stream)
   const long long n_items = most_items(a.s, a.s.n_seqs) * a.n_parts;
   QMOE_REQUIRE(n_items <= 0x7fffffff, "too many heads");
   const long long ctas = n_items < sm_count(device) ? n_items : sm_count(device);
-  QMOE_LAUNCH(kernel, (unsigned)ctas, kPromptThreads, smem, stream, a, maps, tma, (int)n_items);
+  QMOE_LAUNCH(kernel, (unsigned)ctas, kPromptThreads, smem, stream, a, maps, tma);
   QMOE_CUDA(cudaGetLastError());
   if (split) {
     cudaLaunchAttribute overlap{};
