@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // instructions; warp 9 finds out from the offsets what the items are; warps 12-15 copy queries, and keys and
 // values into a ring of four buffers.  While one query tile's softmax runs, the tensor core works for the other,
 // and the next item's tiles come in while this one's output is written (one CTA per item instead: 126 against
-// 110 us for 16 uneven prompts of 8192 tokens together, 32 heads of 128; 105 with two heads an item).
+// 110 us for 16 uneven prompts of 8192 tokens together, 32 heads of 128; 105 with two heads an item, 93 with the items in order).
 // Few items with many keys are split along the keys (key_parts): every part leaves its unfinished rows, maximum and
 // sum in the workspace, and a second kernel joins them.
 //
@@ -92,7 +92,9 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // to 3600 clocks, of which the tensor core works 2048 at head_dim 128.  The exponentials are the softmax's
 // largest part (a special function unit gives 16 results a clock and SM: 2048 clocks a step), so two pairs of
 // eight are polynomials on the FMA units (1165 instead of 1143 TFLOP/s over one prompt of 8192 tokens).
-// One prompt of 16384 tokens, 32 heads of 128: 1.96 to 2.01 ms, 1.1 PFLOP/s.
+// One prompt of 16384 tokens, 32 heads of 128: 1.88 to 1.98 ms, 1.11 to 1.17 PFLOP/s; 16 uneven prompts of 8192 tokens
+// together 93 us.
+//
 // Every tile lies in shared memory as rows of 64 columns (128 bytes) under the 128-byte swizzle, one block
 // of 128 rows per 64 columns: K-major for Q and K, and the same bytes with the head axis contiguous for V.
 // Tiles come by bulk tensor copies, a sequence's last, partial key tile by the copying warps, which write zeros
@@ -251,8 +253,7 @@ struct PromptItem {
 };
 
 template <typename T, bool BIAS, bool SPLIT>
-__global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    const bool tma) {
+__global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const PromptArgs a, const __grid_constant__ PromptMaps maps) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // the swizzle repeats every 1024 bytes
   __shared__ PromptBars s_bar;
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       // ---- copies: Q, then K 0, V 0, K 1, V 1, ... of one item after another
       const int t = tid - 384;
       bool ok = true;
-      int copied = 0, first = 0;  // buffers filled so far, at the beginning of the item
+      int copied = 0, first = 0, q_item = -1;  // buffers filled so far, at the beginning of the item; last item whose queries came
       for (int x = 0;; x++) {
         PromptItem item;
         ok = get_item(x, item) && ok;
@@ -319,30 +320,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         named_sync(1, kTileRows);
         if (stop) break;
         const int n_steps = max(item.steps[0], item.steps[1]), kv = item.head / group;
-        const int n_tma = tma ? 2 * max(0, min(n_steps, item.m / kTileRows - (SPLIT ? item.tile0 : 0))) : 0;  // whole key tiles come by bulk copies
+        const int n_tma = 2 * max(0, min(n_steps, item.m / kTileRows - (SPLIT ? item.tile0 : 0)));  // whole key tiles come by bulk copies
         if (n_steps > 0) {
           if (t == 0 && x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, s_fail);
-          if (tma && t == 0 && ok) {
+          if (t == 0 && ok) {
             const uint32_t q_full = bar(s_bar.q_full);
             mbar_arrive_tx(q_full, (uint32_t)((item.steps[0] > 0) + (item.steps[1] > 0)) * tile_bytes);
             for (int i = 0; i < 2; i++)
               for (int b = 0; item.steps[i] > 0 && b < blocks; b++)
                 tma_load3(smem_u32(q_tile) + i * tile_bytes + b * kBlockBytes, &maps.q, 64 * b, item.head + i * a.head_step,
                           item.q_row + item.row0 + i * a.row_step, q_full);
-          }
-          if (!tma) {
-            named_sync(1, kTileRows);
-            for (int i = 0; i < 2; i++) {
-              const int r = item.row0 + i * a.row_step;
-              load_tile<T, kTileRows>(q_tile + i * tile_bytes,
-                                      reinterpret_cast<const T *>(a.q) + (item.q_row + (long long)(r < item.n ? r : 0)) * a.s.q_row + (item.head + i * a.head_step) * a.s.q_head,
-                                      a.s.q_row, max(0, min(kTileRows, item.n - r)), d, chunks, t);
-            }
-            cp_async_commit();
-            cp_async_wait<0>();
-            fence_async_proxy();
-            named_sync(1, kTileRows);
-            if (t == 0) mbar_arrive(bar(s_bar.q_full));
+            q_item = x;
           }
         } else if (t == 0) {
           if (x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, s_fail);
@@ -390,7 +378,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         if (t == 0) done_item(x);
       }
       if (t == 0 && (!ok || s_fail[0])) {  // copies in flight land before the block ends
-        mbar_wait(bar(s_bar.q_full), 0);
+        if (q_item >= 0) mbar_wait(bar(s_bar.q_full), q_item & 1);
         for (int c = max(0, copied - kStages); c < copied; c++) mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
       }
     } else if (warp == 9) {
@@ -838,7 +826,7 @@ int prompt_timeouts(int reset, int *count) {
 }
 
 // Tensor map of [rows][heads][head_dim] with boxes of 64 values, one head and 128 rows; false where the
-// driver has no such map (a stride of 0, for one): the tiles are then copied by threads.
+// driver has no such map.
 static bool make_map(CUtensorMap *map, const void *base, int dtype, int d, int heads, int64_t rows, int64_t head_stride,
                      int64_t row_stride) {
   using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -860,7 +848,6 @@ static bool make_map(CUtensorMap *map, const void *base, int dtype, int d, int h
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
   const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
   const cuuint32_t box[3] = {64, 1, (cuuint32_t)kTileRows}, steps[3] = {1, 1, 1};
-  if (strides[0] == 0 || strides[1] == 0) return false;
   return encode(map, dtype == QMOE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                 const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -941,9 +928,14 @@ static int run_prompt(PromptArgs a, void *work, int device, cudaStream_t stream)
   a.part_out = reinterpret_cast<float *>(at);
   a.part_stat = reinterpret_cast<float2 *>(a.part_out + a.s.total_q * a.s.heads * a.n_parts * (16 * ((a.s.head_dim + 15) / 16)));
   PromptMaps maps{};
-  const bool tma = make_map(&maps.q, a.q, a.s.dtype, a.s.head_dim, a.s.heads, a.s.total_q, a.s.q_head, a.s.q_row) &&
+  // without keys no tile is copied
+  if (a.s.total_k > 0 &&
+      !(make_map(&maps.q, a.q, a.s.dtype, a.s.head_dim, a.s.heads, a.s.total_q, a.s.q_head, a.s.q_row) &&
                    make_map(&maps.k, a.k, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.k_head, a.s.k_row) &&
-                   make_map(&maps.v, a.v, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.v_head, a.s.v_row);
+                   make_map(&maps.v, a.v, a.s.dtype, a.s.head_dim, a.s.kv_heads, a.s.total_k, a.s.v_head, a.s.v_row))) {
+    set_error("qmoe_prompt_attention: the driver took no tensor map of q, k or v");
+    return QMOE_ERR_UNSUPPORTED;
+  }
   const int smem = (2 + kStages) * ((a.s.head_dim + 63) / 64) * kBlockBytes + 8 * 4096 + 1024;
   auto kernel = a.bias != nullptr ? (split ? k_prompt_tiles<T, true, true> : k_prompt_tiles<T, true, false>)
                                   : (split ? k_prompt_tiles<T, false, true> : k_prompt_tiles<T, false, false>);
@@ -953,7 +945,7 @@ static int run_prompt(PromptArgs a, void *work, int device, cudaStream_t stream)
   const long long n_items = most_items(a.s, a.s.n_seqs) * a.n_parts;
   QMOE_REQUIRE(n_items <= 0x7fffffff, "too many heads");
   const long long ctas = n_items < sm_count(device) ? n_items : sm_count(device);
-  QMOE_LAUNCH(kernel, (unsigned)ctas, kPromptThreads, smem, stream, a, maps, tma);
+  QMOE_LAUNCH(kernel, (unsigned)ctas, kPromptThreads, smem, stream, a, maps);
   QMOE_CUDA(cudaGetLastError());
   if (split) {
     cudaLaunchAttribute overlap{};
