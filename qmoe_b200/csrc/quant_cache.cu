@@ -120,17 +120,20 @@ struct RowsArgs {
 // Both directions are bounded by memory: 2 bytes read or written per value of the 16-bit side, 1 of the codes,
 // 4 per row for the scale; what is left to do is to spend few instructions on a value.  A CTA takes `tokens`
 // tokens with all their heads, keys and values: their places in the cache are looked up once, one thread a
-// token, then every thread moves pieces of 16 values.  A row of one head is shared by LANES neighbouring lanes
-// (a power of two), heads run fastest, so that 16-bit rows are read or written in order.
-// Where the 16-bit tensors' rows do not begin on 16-byte boundaries (VEC false) a warp moves them value by
-// value, neighbouring lanes neighbouring values, through shared memory: [row of the warp][16 * LANES values].
+// token, then every thread moves pieces of 16 values.  A row of one head is shared by LANES neighbouring lanes,
+// heads run fastest, so that 16-bit rows are read or written in order.  Rows of 3, 5 and 6 pieces have their own
+// kernels with 30 of 32 lanes at work (17408 tokens of 12 heads of 80 enter the cache in 33 us, with the next power of
+// two lanes a row in 54).
+// Where the 16-bit tensors' rows do not begin on 16-byte boundaries (VEC false) they are read in words of 4 bytes
+// (7680 tokens of 32 heads of 65: 52 us, value by value 93) and written value by value, neighbouring lanes neighbouring values, through shared memory:
+// [row of the warp][16 * LANES values].
 // 16384 tokens of 8 heads of 128 in bf16 enter an e4m3 cache in 33 us (3.1 TB/s: the rounding, some twenty
 // instructions a value, takes as long as the memory); 65536 of them come back in 75 us (5.4 TB/s).
 constexpr int kRowsThreads = 256;
 constexpr int kRowsPieces = 8;  // of a thread, at most
 constexpr int kRowsTokens = 64;
 
-__host__ __device__ constexpr int row_lanes(int width) { return width <= 16 ? 1 : (width <= 32 ? 2 : (width <= 64 ? 4 : (width <= 128 ? 8 : 16))); }
+__host__ __device__ constexpr int row_lanes(int width) { return width <= 96 ? (width + 15) / 16 : (width <= 128 ? 8 : 16); }
 
 // Places of the CTA's tokens: index of (page, head 0, place); -1 without a valid page, -2 when nobody owns the
 // row.
@@ -154,13 +157,15 @@ struct CacheRow {
   int head;
   bool is_v;
 };
+template <int LANES>
 __device__ __forceinline__ CacheRow cache_row(const RowsArgs &a, const long long *s_slot, int r) {
   CacheRow c;
   const int token = (int)__umulhi((uint32_t)r, a.per_token_inverse), in_token = r - token * 2 * a.c.kv_heads;
   c.is_v = in_token >= a.c.kv_heads;
   c.head = in_token - (c.is_v ? a.c.kv_heads : 0);
   c.row = (long long)blockIdx.x * a.tokens + token;
-  c.slot = token < a.tokens ? s_slot[token] : -2;
+  const bool idle = (threadIdx.x & 31) >= 32 / LANES * LANES;  // lanes that are left over own no row
+  c.slot = token < a.tokens && !idle ? s_slot[token] : -2;
   if (c.slot >= 0) c.slot += (long long)c.head << a.c.page_shift;
   return c;
 }
@@ -186,9 +191,8 @@ __device__ __forceinline__ float2 pair_values<__half>(uint32_t v) { return __hal
 
 template <typename T, int FMT, int LANES, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) k_cache_append(const RowsArgs a) {
-  constexpr int kPerWarp = 32 / LANES;
+  constexpr int kPerWarp = 32 / LANES, kStep = kRowsThreads / 32 * kPerWarp;
   __shared__ long long s_slot[kRowsTokens];
-  __shared__ __align__(16) T s_rows[VEC ? 1 : kRowsThreads / 32][VEC ? 1 : 512];
   const int lane = threadIdx.x & 31, at = 16 * (lane % LANES);
   const int d = a.c.head_dim, width = cache_row_bytes(d), rows = a.tokens * 2 * a.c.kv_heads;
   find_slots(a, s_slot);
@@ -202,7 +206,8 @@ __global__ void __launch_bounds__(kRowsThreads) k_cache_append(const RowsArgs a)
 #pragma unroll
     for (int i = 0; i < 8; i++) m = abs_max2(m, w[i], T());
 #pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) m = abs_max2(m, __shfl_xor_sync(0xffffffffu, m, o), T());
+    for (int o = 1; o < LANES; o <<= 1)  // of the row's lanes, taken round
+      m = abs_max2(m, __shfl_sync(0xffffffffu, m, lane - lane % LANES + (lane % LANES + o) % LANES), T());
     const float2 m2 = pair_values<T>(m);
     const bool finite = m2.x <= FLT_MAX && m2.y <= FLT_MAX;  // NaN and infinity stay in the maximum
     if (c.slot < 0 || at >= width) return;
@@ -229,66 +234,71 @@ __global__ void __launch_bounds__(kRowsThreads) k_cache_append(const RowsArgs a)
     *reinterpret_cast<uint4 *>((c.is_v ? a.c.v_codes : a.c.k_codes) + c.slot * width + at) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
     if (at == 0) (c.is_v ? a.c.v_scale : a.c.k_scale)[c.slot] = finite ? stored : __int_as_float(0x7fffffff);
   };
-  if (VEC) {
-    // two pieces at a time: both loads are under way before the first is used
-    for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += 2 * kRowsThreads / LANES) {
-      const int r0 = base + lane / LANES;
-      CacheRow c[2];
-      uint4 v[2][2];
+  auto load = [&](const CacheRow &c, uint4 (&v)[2]) {
+    v[0] = v[1] = make_uint4(0u, 0u, 0u, 0u);
+    if (c.slot < 0) return;
+    const T *src = source(c) + at;
+    if (VEC && at + 16 <= d) {
+      v[0] = __ldg(reinterpret_cast<const uint4 *>(src));
+      v[1] = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
+    } else if (VEC) {
+      T *to = reinterpret_cast<T *>(v);
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        c[b] = cache_row(a, s_slot, r0 + b * (kRowsThreads / LANES));
-        v[b][0] = v[b][1] = make_uint4(0u, 0u, 0u, 0u);
-        const T *src = source(c[b]) + at;
-        if (c[b].slot >= 0 && at + 16 <= d) {
-          v[b][0] = __ldg(reinterpret_cast<const uint4 *>(src));
-          v[b][1] = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
-        } else if (c[b].slot >= 0) {
-          T *to = reinterpret_cast<T *>(v[b]);
+      for (int i = 0; i < 16; i++)
+        if (at + i < d) to[i] = src[i];
+    } else {
+      // the nine 4-byte words that the 16 values lie in, shifted by half a word where they begin in its middle;
+      // of words that reach over the row's ends only the row's half is read
+      const int odd = (int)(reinterpret_cast<uintptr_t>(src) >> 1) & 1;
+      const uint16_t *from = reinterpret_cast<const uint16_t *>(src) - odd;
+      uint32_t w[9];
 #pragma unroll
-          for (int i = 0; i < 16; i++)
-            if (at + i < d) to[i] = src[i];
-        }
+      for (int x = 0; x < 9; x++) {
+        const int first = at + 2 * x - odd;
+        const bool lo = first >= 0 && first < d && (x < 8 || odd), hi = first + 1 < d && x < 8;
+        w[x] = 0u;
+        if (lo && hi) w[x] = __ldg(reinterpret_cast<const uint32_t *>(from) + x);
+        else if (lo) w[x] = __ldg(from + 2 * x);
+        else if (hi) w[x] = (uint32_t)__ldg(from + 2 * x + 1) << 16;
       }
+      uint32_t o[8];
 #pragma unroll
-      for (int b = 0; b < 2; b++) finish(c[b], v[b]);
+      for (int x = 0; x < 8; x++) o[x] = odd ? __funnelshift_r(w[x], w[x + 1], 16) : w[x];
+      v[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      v[1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
-  } else {
-    T *stage = s_rows[threadIdx.x >> 5];
-    for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += kRowsThreads / LANES) {
-      const CacheRow c = cache_row(a, s_slot, base + lane / LANES);
-      const T *src = source(c);
+  };
+  // two pieces at a time: both loads are under way before the first is used
+  for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += 2 * kStep) {
+    const int r0 = base + lane / LANES;
+    CacheRow c[2];
+    uint4 v[2][2];
 #pragma unroll
-      for (int i = 0; i < kPerWarp; i++) {
-        const T *from = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, (unsigned long long)src, i * LANES));
-        const bool in = __shfl_sync(0xffffffffu, (int)(c.slot >= 0), i * LANES);
-        for (int col = lane; col < 16 * LANES; col += 32) stage[i * 16 * LANES + col] = in && col < d ? from[col] : from_f32<T>(0.f);
-      }
-      __syncwarp();
-      const uint4 *from = reinterpret_cast<const uint4 *>(stage + (lane / LANES) * 16 * LANES + at);
-      const uint4 v[2] = {from[0], from[1]};
-      finish(c, v);
-      __syncwarp();
+    for (int b = 0; b < 2; b++) {
+      c[b] = cache_row<LANES>(a, s_slot, r0 + b * kStep);
+      load(c[b], v[b]);
     }
+#pragma unroll
+    for (int b = 0; b < 2; b++) finish(c[b], v[b]);
   }
 }
 
 template <typename T, int FMT, int LANES, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) k_cache_read(const RowsArgs a) {
-  constexpr int kPerWarp = 32 / LANES;
+  constexpr int kPerWarp = 32 / LANES, kStep = kRowsThreads / 32 * kPerWarp;
   __shared__ long long s_slot[kRowsTokens];
   __shared__ __align__(16) T s_rows[VEC ? 1 : kRowsThreads / 32][VEC ? 1 : 512];
   const int lane = threadIdx.x & 31, at = 16 * (lane % LANES);
   const int d = a.c.head_dim, width = cache_row_bytes(d), rows = a.tokens * 2 * a.c.kv_heads;
   find_slots(a, s_slot);
-  for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += 2 * kRowsThreads / LANES) {  // uniform in a warp
+  for (int base = (threadIdx.x >> 5) * kPerWarp; base < rows; base += 2 * kStep) {  // uniform in a warp
     const int r0 = base + lane / LANES;
     CacheRow c[2];
     uint4 codes[2];
     float scale[2];
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-      c[b] = cache_row(a, s_slot, r0 + b * (kRowsThreads / LANES));
+      c[b] = cache_row<LANES>(a, s_slot, r0 + b * kStep);
       codes[b] = make_uint4(0u, 0u, 0u, 0u);
       scale[b] = 0.f;
       if (c[b].slot >= 0 && at < width) {
@@ -970,6 +980,9 @@ using namespace qmoe;
 #define QMOE_ROWS_KERNELS(kernel, T, FMT, vec)                                                                  \
   (lanes == 1   ? (vec ? kernel<T, FMT, 1, true> : kernel<T, FMT, 1, false>)                                    \
    : lanes == 2 ? (vec ? kernel<T, FMT, 2, true> : kernel<T, FMT, 2, false>)                                    \
+   : lanes == 3 ? (vec ? kernel<T, FMT, 3, true> : kernel<T, FMT, 3, false>)                                    \
+   : lanes == 5 ? (vec ? kernel<T, FMT, 5, true> : kernel<T, FMT, 5, false>)                                    \
+   : lanes == 6 ? (vec ? kernel<T, FMT, 6, true> : kernel<T, FMT, 6, false>)                                    \
    : lanes == 4 ? (vec ? kernel<T, FMT, 4, true> : kernel<T, FMT, 4, false>)                                    \
    : lanes == 8 ? (vec ? kernel<T, FMT, 8, true> : kernel<T, FMT, 8, false>)                                    \
                 : (vec ? kernel<T, FMT, 16, true> : kernel<T, FMT, 16, false>))
