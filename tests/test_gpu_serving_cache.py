@@ -336,3 +336,22 @@ def test_a_cache_without_pages():
         assert bool((k == 0).all()) and bool((v == 0).all()) and cache.refused(reset=True) == 3
         assert bool((serving.decode_attention_paged(x[:1], cache, table, _ints([3])) == 0).all())
         assert cache.refused(reset=True) == 2             # one tile, or one sequence, by two key heads
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.bfloat16), ("int8", torch.float16)])
+@pytest.mark.parametrize("d", [2, 15, 16, 31, 33, 48, 63, 66, 72, 79, 80, 81, 95, 96, 97, 112, 127, 129])
+def test_every_row_width_and_alignment(fmt, dtype, d):
+    """Rows of 1 to 9 pieces that begin on any 2-byte boundary, infinities right before and behind them."""
+    n, heads, page = 70, 3, 16
+    table = _table([n], page, 8)
+    g = torch.Generator(device=DEV).manual_seed(d)
+    for shift in range(0, 9, 1 if d < 90 else 3):
+        pool = torch.full((n * 2 * heads * (d + 3) + 16,), math.inf, dtype=dtype, device=DEV)
+        rows = pool[shift:shift + n * 2 * heads * (d + 3)].view(n, 2, heads, d + 3)[..., 1:1 + d]
+        rows.copy_(torch.randn(n, 2, heads, d, generator=g, device=DEV))
+        cache = serving.QuantCache(8, page, heads, d, DEV, fmt=fmt)
+        serving.cache_append(cache, rows[:, 0], rows[:, 1], _cu([n]), _ints([0]), table)
+        k, v = serving.cache_read(cache, _cu([n]), _ints([0]), table, n, dtype=dtype)
+        for x, back in ((rows[:, 0], k), (rows[:, 1], v)):
+            value, scale = ref.quantise(x, fmt)
+            assert torch.equal(back, (value.float() * scale[..., None]).to(dtype)), shift
