@@ -95,7 +95,10 @@ int allow_shared(const void *kernel, int bytes, int device, int regs) {
     }
   }
   QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  allowed[{kernel, device}] = bytes;
+  try {
+    allowed[{kernel, device}] = bytes;
+  } catch (...) {  // no memory to remember it: asked for again next time
+  }
   return QMOE_OK;
 }
 
