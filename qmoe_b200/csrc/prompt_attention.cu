@@ -575,7 +575,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         float s[kTileRows];
 #pragma unroll
         for (int c = 0; c < 4; c++) tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
-        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_wait_ld32(reinterpret_cast<uint32_t *>(s) + 32 * c);
         const int key0 = ((SPLIT ? item.tile0 : 0) + j) * kTileRows;
         if (BIAS) {
           if (far) {

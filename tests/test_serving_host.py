@@ -195,3 +195,20 @@ def test_prompt_workspace_of_split_keys():
     assert _prompt(_shape(**one)) == _lib.ERR_INVALID_ARG                   # needs a workspace
     for bad in (dict(heads=0), dict(kv_heads=0), dict(n_seqs=0), dict(n_seqs=-1), dict(total_q=-1), dict(total_k=-1)):
         assert size(**{**one, **bad}) == 0
+
+
+def test_waits_for_tensor_memory_name_the_values_they_guard():
+    """A wait for loads from tensor memory that stands in a statement without the loaded registers does not keep the
+    compiler from moving arithmetic on them in front of it."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(serving.__file__), "csrc")
+    found = 0
+    for name in os.listdir(csrc):
+        with open(os.path.join(csrc, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for statement in re.findall(r"asm volatile\(.*?\);", text, re.S):
+            if "tcgen05.wait::ld" in statement:
+                found += 1
+                assert '"+r"(v[0])' in statement or '"=r"(v[0])' in statement, (name, statement)
+    assert found > 0
