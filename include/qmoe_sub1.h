@@ -442,12 +442,16 @@ typedef struct qmoe_prompt_args {
  *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j] + bias) v[j]
  * with bias = rel_bias_dev[h * n_dist + min(distance, n_dist - 1)] (fp32, may be NULL), the distance
  * being i + m - n - j: the one-directional relative bias of T5 / Switch (scale 1).  Statistics and
- * sums are fp32.  At most 262140 query rows, 2^25 key rows and 32768 sequences a call.  A wait of the tensor-core kernel
- * that runs out is counted by qmoe_moe_tile_timeouts.  out_dev must not overlap q, k or v.  work_dev: qmoe_prompt_work_bytes bytes for the same
+ * sums are fp32.  At most 262140 query rows, 2^25 key rows and 32768 sequences a call.  Every wait of the
+ * tensor-core kernel is bounded (4 s without progress); a CTA whose wait runs out leaves the output rows that it has not
+ * finished as they were (of split keys: anything) and is counted by qmoe_moe_tile_timeouts.  qmoe_prompt_set_wait_limit(ns)
+ * lowers the bound (1: give up without polling; 0: back to the default), so that a test can make a wait run out.
+ * out_dev must not overlap q, k or v.  work_dev: qmoe_prompt_work_bytes bytes for the same
  * arguments (0 where every row of q, k and v begins on a 16-byte boundary and there are queries enough to keep
  * the GPU busy), 256-byte aligned, not shared by calls that may overlap. */
 int64_t qmoe_prompt_work_bytes(const qmoe_prompt_args *args);
 int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, void *stream);
+int qmoe_prompt_set_wait_limit(int64_t ns);
 
 /* A paged cache whose keys and values are held in 8 bits.  codes: [n_pages][kv_heads][page_size]
  * [row_bytes], row_bytes = head_dim rounded up to 16, the padding zero; scales: fp32

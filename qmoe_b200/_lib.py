@@ -121,6 +121,7 @@ SIGNATURES = {
     # the argument structures are passed as packed bytes: one argument is converted instead of twenty
     "qmoe_prompt_work_bytes": (_L, [ctypes.c_char_p]),
     "qmoe_prompt_attention": (_I, [ctypes.c_char_p, _I, _P]),
+    "qmoe_prompt_set_wait_limit": (_I, [_L]),
     "qmoe_cache_append": (_I, [_P, ctypes.c_char_p, _I, _P]),
     "qmoe_cache_read": (_I, [_P, ctypes.c_char_p, _I, _P]),
     "qmoe_decode_paged_work_bytes": (_L, [_I, _I, _I, _I, _I]),

@@ -128,6 +128,7 @@ void set_items_per_matrix(int wi, int wo);
 int set_fused_phases(int on);
 int set_tile_wait_limit(uint32_t spins);
 int prompt_timeouts(int reset, int *count);
+int set_prompt_wait_limit(int64_t ns);
 int work_summary(const void *work, int max_slots, int d_ff, int32_t *out, cudaStream_t stream);
 int launch_grouped_ffn(const SparseTable &tab, const int32_t *dec, const uint16_t *codes,
                        const int32_t *row_off, const void *minmax, const qmoe_matrix_desc *descs,
@@ -984,6 +985,8 @@ int qmoe_sub1_forget(const int32_t *dec_dev, int device) {
 }
 
 int qmoe_moe_set_tile_wait_limit(uint32_t spins) { return set_tile_wait_limit(spins); }
+
+int qmoe_prompt_set_wait_limit(int64_t ns) { return set_prompt_wait_limit(ns); }
 
 int qmoe_moe_tile_timeouts(int device, int reset, int *count_out) {
   QMOE_REQUIRE(count_out != nullptr, "null output pointer");

@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "serving.cuh"
@@ -21,6 +22,7 @@ struct PromptArgs {
   float2 *part_stat;  // [row][head][part]
   int n_parts;
   int row_step, head_step;  // of an item's second query tile from its first: 128 rows further on, or the next head
+  unsigned long long wait_ns;  // bound of the waits that decide to give up
 };
 
 // One query row of one head by one warp, keys one after another with a running maximum; 32 lanes share
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // A value row that is not finite would spoil queries that give it weight 0 (0 * inf): a query row whose
 // result is not finite is computed again key by key.
 // All waits are bounded (kPromptWait); when one runs out the CTA counts itself in d_prompt_timeouts, waits for its
-// copies in flight, frees its tensor memory and returns.
+// copies and products in flight, frees its tensor memory and returns.
 constexpr int kPromptThreads = 512;
 constexpr int kPromptRegs = 128;  // at launch; the softmax warps then hold 192 and the others 64
 constexpr int kTileRows = 128;
@@ -129,14 +131,18 @@ struct PromptBars {
   uint64_t item_full[kItems], item_empty[kItems], drain;
 };
 
-// Waits for a phase of a barrier for kPromptWait nanoseconds at most, or until another wait of the CTA ran out.
+// The bound in use: tests lower it so that waits run out without anything hanging (1: give up without polling;
+// 0: kPromptWait).  The clean-up waits before a block ends have their own, which stays.
+static std::atomic<long long> g_prompt_wait_ns{0};
+
+// Waits for a phase of a barrier for `limit` nanoseconds at most, or until another wait of the CTA ran out.
 // `fail[1]` counts what takes long by design: while it moves, the wait begins again.
-__device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, volatile int *fail) {
-  if (mbar_wait(bar, parity, 2)) return true;
+__device__ __forceinline__ bool wait_until(uint32_t bar, uint32_t parity, volatile int *fail, unsigned long long limit) {
+  if (limit != 1 && mbar_wait(bar, parity, 2)) return true;
   unsigned long long now, begin;
   int seen = fail[1];
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
-  do {
+  while (limit != 1) {
     if (mbar_wait(bar, parity, 2)) return true;
     if (*fail) return false;
     if (seen != fail[1]) {
@@ -144,7 +150,8 @@ __device__ __forceinline__ bool wait_or_fail(uint32_t bar, uint32_t parity, vola
       asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
     }
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-  } while (now - begin < kPromptWait);
+    if (now - begin >= limit) break;
+  }
   *fail = 1;
   return false;
 }
@@ -268,6 +275,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
   uint8_t *q_tile = smem, *ring = smem + 2 * tile_bytes, *stage_out = ring + kStages * tile_bytes;
 
   auto bar = [&](uint64_t &b) { return smem_u32(&b); };
+  auto wait_or_fail = [&](uint32_t at, uint32_t parity, volatile int *fail) { return wait_until(at, parity, fail, a.wait_ns); };
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(bar(s_bar.s_full[i]), 1);
@@ -312,11 +320,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       int copied = 0, first = 0, q_item = -1;  // buffers filled so far, at the beginning of the item; last item whose queries came
       for (int x = 0;; x++) {
         PromptItem item;
-        ok = get_item(x, item) && ok;
-        // one decision for all: thread 0's
-        if (t == 0) s_stop[0] = !ok || !item.valid;
+        // one decision for all, thread 0's: how often the threads meet below depends on the item, which must not have
+        // come to some of them only
+        if (t == 0) {
+          ok = get_item(x, item) && ok;
+          s_stop[0] = !ok || !item.valid;
+        }
         named_sync(1, kTileRows);
         const bool stop = s_stop[0];
+        item = s_item[x % kItems];
         named_sync(1, kTileRows);
         if (stop) break;
         const int n_steps = max(item.steps[0], item.steps[1]), kv = item.head / group;
@@ -334,7 +346,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
           }
         } else if (t == 0) {
           if (x > 0) ok = wait_or_fail(bar(s_bar.q_empty), (x - 1) & 1, s_fail);
-          mbar_arrive(bar(s_bar.q_full));  // nothing to copy: the phases go on
+          if (ok) {
+            mbar_arrive(bar(s_bar.q_full));  // nothing to copy: the phases go on
+            q_item = x;
+          }
         }
         if (t == 0) {
           for (int c = 0; ok && c < n_tma; c++) {
@@ -370,14 +385,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
           cp_async_wait<0>();
           fence_async_proxy();
           named_sync(1, kTileRows);
-          if (t == 0) mbar_arrive(bar(s_bar.kv_full[stage]));
+          if (t == 0) {
+            mbar_arrive(bar(s_bar.kv_full[stage]));
+            copied = at + 1;
+          }
         }
         named_sync(1, kTileRows);  // s_stop is written again; the item has been read by all
         if (gave_up) break;
         first += 2 * n_steps;
         if (t == 0) done_item(x);
       }
-      if (t == 0 && (!ok || s_fail[0])) {  // copies in flight land before the block ends
+      // Copies in flight land before the block ends, whoever gave up and whenever; of every buffer its last filling.
+      if (t == 0) {
         if (q_item >= 0) mbar_wait(bar(s_bar.q_full), q_item & 1);
         for (int c = max(0, copied - kStages); c < copied; c++) mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
       }
@@ -523,10 +542,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         done[1] += item.steps[1];
         if (lane == 0) done_item(x);
       }
-      if (!ok) {  // whatever is still in flight ends before tensor memory is freed
-        mma_commit_warp(bar(s_bar.drain));
-        mbar_wait(bar(s_bar.drain), 0);
-      }
+      // Whatever is still in flight ends before tensor memory is freed, also when only the softmax warps gave up.
+      mma_commit_warp(bar(s_bar.drain));
+      mbar_wait(bar(s_bar.drain), 0);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
@@ -819,6 +837,12 @@ __global__ void __launch_bounds__(kPartsThreads) k_prompt_join(const PromptArgs 
   }
 }
 
+int set_prompt_wait_limit(int64_t ns) {
+  QMOE_REQUIRE(ns >= 0, "a wait cannot be negative");
+  g_prompt_wait_ns.store(ns, std::memory_order_relaxed);
+  return QMOE_OK;
+}
+
 int prompt_timeouts(int reset, int *count) {
   QMOE_CUDA(cudaMemcpyFromSymbol(count, d_prompt_timeouts, sizeof(int)));
   const int zero = 0;
@@ -926,6 +950,8 @@ static int run_prompt(PromptArgs a, void *work, int device, cudaStream_t stream)
   a.row_step = two_heads(a.s) ? 0 : kTileRows;
   a.head_step = two_heads(a.s) ? 1 : 0;
   const bool split = a.n_parts > 1;
+  const long long wait_ns = g_prompt_wait_ns.load(std::memory_order_relaxed);
+  a.wait_ns = wait_ns > 0 ? (unsigned long long)wait_ns : kPromptWait;
   a.part_out = reinterpret_cast<float *>(at);
   a.part_stat = reinterpret_cast<float2 *>(a.part_out + a.s.total_q * a.s.heads * a.n_parts * (16 * ((a.s.head_dim + 15) / 16)));
   PromptMaps maps{};

@@ -588,10 +588,11 @@ def work_plan(work: torch.Tensor, max_slots: int, d_ff: int) -> Dict[str, int]:
 
 
 def tile_timeouts(device, reset: bool = False) -> int:
-    """Number of tensor-core tile CTAs on ``device`` whose bounded wait gave up since the last reset
+    """Number of tensor-core tile CTAs on ``device`` (of the grouped FFN and of
+    :func:`qmoe_b200.serving.prompt_attention`) whose bounded wait gave up since the last reset
     (0 in normal operation).  Synchronises the device: call it where the caller synchronises anyway.
-    A non-zero value means that grouped-FFN outputs produced since the last reset hold zeros for the
-    rows those CTAs did not finish."""
+    A non-zero value means that outputs produced since the last reset are incomplete: of the grouped FFN
+    the rows those CTAs did not finish hold zeros, of prompt attention they were not written."""
     count = ctypes.c_int(0)
     _lib.check(_lib.load().qmoe_moe_tile_timeouts(_dev_index(device), 1 if reset else 0, ctypes.byref(count)))
     return int(count.value)

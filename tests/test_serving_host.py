@@ -212,3 +212,8 @@ def test_waits_for_tensor_memory_name_the_values_they_guard():
                 found += 1
                 assert '"+r"(v[0])' in statement or '"=r"(v[0])' in statement, (name, statement)
     assert found > 0
+
+
+def test_wait_limit_is_not_negative():
+    assert _lib.load().qmoe_prompt_set_wait_limit(-1) == _lib.ERR_INVALID_ARG
+    assert _lib.load().qmoe_prompt_set_wait_limit(0) == _lib.OK
