@@ -27,8 +27,10 @@ struct PromptArgs {
 
 // One query row of one head by one warp, keys one after another with a running maximum; 32 lanes share
 // the head's values.  A key whose weight is 0 contributes nothing, whatever its value row holds.
+// `progress`, if given, moves at least every kProgressKeys keys: others of the CTA wait meanwhile.
+constexpr int kProgressKeys = 1024;
 template <typename T, int J>  // J >= ceil(head_dim / 32)
-__device__ __forceinline__ void attend_row(const PromptArgs &a, int head, int row, int2 rq, int2 rk) {
+__device__ __forceinline__ void attend_row(const PromptArgs &a, int head, int row, int2 rq, int2 rk, int *progress = nullptr) {
   const int lane = threadIdx.x & 31;
   const int last = row - rq.x + (rk.y - rk.x) - (rq.y - rq.x);  // last key that the query sees
   const int kv = head / (a.s.heads / a.s.kv_heads), d = a.s.head_dim;
@@ -42,6 +44,7 @@ __device__ __forceinline__ void attend_row(const PromptArgs &a, int head, int ro
   }
   float m = -INFINITY, sum = 0.f;
   for (int t = 0; t <= last; t++) {
+    if (progress != nullptr && t % kProgressKeys == 0 && lane == 0) atomicAdd(progress, 1);
     const T *k = reinterpret_cast<const T *>(a.k) + (rk.x + (long long)t) * a.s.k_row + kv * a.s.k_head;
     const T *v = reinterpret_cast<const T *>(a.v) + (rk.x + (long long)t) * a.s.v_row + kv * a.s.v_head;
     float dot = 0.f;
@@ -119,7 +122,7 @@ constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
 constexpr int kPolyPairs = 2;
 constexpr int kWave = 148;      // CTAs at a time
 constexpr int kMaxParts = 32;   // a warp's lanes look after one each when they are joined
-constexpr unsigned long long kPromptWait = 4000000000ull;  // ns; a row computed again key by key may take a while
+constexpr unsigned long long kPromptWait = 4000000000ull;  // ns without progress
 __device__ int d_prompt_timeouts;
 
 struct PromptMaps {
@@ -136,7 +139,8 @@ struct PromptBars {
 static std::atomic<long long> g_prompt_wait_ns{0};
 
 // Waits for a phase of a barrier for `limit` nanoseconds at most, or until another wait of the CTA ran out.
-// `fail[1]` counts what takes long by design: while it moves, the wait begins again.
+// `fail[1]` moves while rows are computed again key by key, which takes as long as it takes (up to some seconds for a
+// row of 2^25 keys): when it has moved, the wait begins again.
 __device__ __forceinline__ bool wait_until(uint32_t bar, uint32_t parity, volatile int *fail, unsigned long long limit) {
   if (limit != 1 && mbar_wait(bar, parity, 2)) return true;
   unsigned long long now, begin;
@@ -773,8 +777,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       while (again != 0) {
         const int l = __ffs(again) - 1;
         again &= again - 1;
-        s_fail[1] = s_fail[1] + 1;  // any change will do
-        attend_row<T, 4>(a, head, item.q_row + tile0 + t0 + l, make_int2(item.q_row, item.q_row + n), make_int2(item.k_row, item.k_row + item.m));
+        attend_row<T, 4>(a, head, item.q_row + tile0 + t0 + l, make_int2(item.q_row, item.q_row + n), make_int2(item.k_row, item.k_row + item.m),
+                         const_cast<int *>(&s_fail[1]));
       }
     }
   }

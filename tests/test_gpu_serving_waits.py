@@ -48,3 +48,18 @@ def test_waits_that_run_out_are_counted_and_leave_the_gpu_usable(lens, heads, kv
     for _ in range(3):                                     # and the next calls are whole again
         assert torch.equal(serving.prompt_attention(q, k, v, cu, rel_bias=bias), want)
     assert sub1.tile_timeouts(DEV) == 0
+
+
+def test_rows_computed_again_take_longer_than_a_wait():
+    """An infinite value sends every row to the key by key path, 100000 keys a row: far longer than the bound, which
+    the tiles themselves keep to.  More items than multiprocessors, so that the next one waits."""
+    heads, m = 640, 100000
+    q, k, v, _ = _rows([m], heads, 1, 64)
+    q = q[:1].contiguous()
+    v[0] = float("inf")
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device=DEV) for n in (1, m))
+    assert sub1.tile_timeouts(DEV, reset=True) == 0
+    with wait_limit(4_000_000):
+        got = serving.prompt_attention(q, k, v, cu_q, cu_k, out=torch.zeros_like(q))
+    assert sub1.tile_timeouts(DEV, reset=True) == 0
+    assert bool((got == float("inf")).all())
