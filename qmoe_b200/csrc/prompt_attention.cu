@@ -53,7 +53,8 @@ __device__ __forceinline__ void attend_row(const PromptArgs &a, int head, int ro
       if (lane + 32 * j < d) dot += qv[j] * to_f32(k[lane + 32 * j]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float s = dot * a.s.scale + (bias != nullptr ? bias[min(last - t, a.s.n_dist - 1)] : 0.f);
+    const float b = bias != nullptr ? bias[min(last - t, a.s.n_dist - 1)] : 0.f;
+    const float s = b == -INFINITY ? b : dot * a.s.scale + b;  // masked, whatever the key holds
     const float m_new = fmaxf(m, s);
     const float base = m_new == -INFINITY ? 0.f : m_new;  // scores of -inf only so far
     const float keep = expf(m - base), p = expf(s - base);
@@ -576,6 +577,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       const float far_bias = BIAS ? in_log2(bias[a.s.n_dist - 1]) : 0.f;
       for (int j = 0; j < steps; j++) {
         bool far = true;
+        uint32_t gone[5];  // of the 160 distances from the largest on: the bias is -inf
         if (BIAS) {
           // Distances of the tile's keys from the warp's queries: where all are behind the last column, one value for
           // all; else the 32 + 127 values that they can have, looked up while the scores are computed.  Query t
@@ -586,9 +588,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
           if (!far) {
             __syncwarp();  // the last ones have been read
 #pragma unroll
-            for (int x = lane; x < kTileRows + 32; x += 32)
-              near_bias[x] = in_log2(__ldg(bias + max(0, min(nearest + x, a.s.n_dist - 1))));
+            for (int x = 0; x < 5; x++) {
+              const float b = in_log2(__ldg(bias + max(0, min(nearest + lane + 32 * x, a.s.n_dist - 1))));
+              near_bias[lane + 32 * x] = b;
+              gone[4 - x] = __brev(__ballot_sync(0xffffffffu, b == -INFINITY));
+            }
             __syncwarp();
+          } else {
+#pragma unroll
+            for (int x = 0; x < 5; x++) gone[x] = far_bias == -INFINITY ? 0xffffffffu : 0u;
           }
         }
         ok = wait_or_fail(bar(s_bar.s_full[i]), (done + j) & 1, s_fail);
@@ -607,6 +615,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
           } else {
 #pragma unroll
             for (int c = 0; c < kTileRows; c++) s[c] = fmaf(s[c], sl2, near_bias[lane + kTileRows - 1 - c]);
+          }
+          // A key that the bias masks may hold anything: its score is replaced, not added to.
+          if ((gone[0] | gone[1] | gone[2] | gone[3] | gone[4]) != 0u) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+              const uint32_t mine = __funnelshift_l(gone[w], gone[w + 1], lane);  // bit c: key 32 w + c
+#pragma unroll
+              for (int c = 0; c < 32; c++) s[32 * w + c] = (mine >> c) & 1u ? -INFINITY : s[32 * w + c];
+            }
           }
         }
         const int edge = last - key0;  // columns behind it are masked

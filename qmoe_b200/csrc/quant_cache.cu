@@ -700,7 +700,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
           for (int i = 0; i < 4; i++) {
             const int row = min(8 * r + 2 * q + (i & 1), n_heads - 1);
             const int far = a.lengths[seq] - 1 - (pos0 + 8 * (i >> 1) + g);
-            s[i] += paged_log2(__ldg(a.bias + (size_t)(head0 + row) * a.n_dist + max(0, min(far, a.n_dist - 1))));
+            const float b = paged_log2(__ldg(a.bias + (size_t)(head0 + row) * a.n_dist + max(0, min(far, a.n_dist - 1))));
+            s[i] = b == -INFINITY ? b : s[i] + b;  // chosen, not added: a masked key may hold anything
           }
         }
         if (pos0 + 16 > seen) {

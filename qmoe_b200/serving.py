@@ -103,7 +103,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     sequence; a query that sees no key gives zeros.  ``scale`` multiplies the scores (0:
     ``1 / sqrt(head_dim)``; T5 / Switch attention uses 1); ``rel_bias`` fp32 ``[heads, n]`` is added
     to them at column ``min(distance, n - 1)``, the distance between query and key.  Keys whose bias
-    is ``-inf`` are masked, whatever they hold.  Returns ``out`` ``[total_q, heads, head_dim]`` (any strides
+    is ``-inf`` are masked, whatever they and their values hold.  Returns ``out`` ``[total_q, heads, head_dim]`` (any strides
     over the first two axes, memory apart from the inputs'); rows that no sequence owns are left as they
     were (uninitialised when ``out`` is not given)."""
     _need(q, "q", (torch.bfloat16, torch.float16), 3, packed=False)

@@ -355,3 +355,21 @@ def test_every_row_width_and_alignment(fmt, dtype, d):
         for x, back in ((rows[:, 0], k), (rows[:, 1], v)):
             value, scale = ref.quantise(x, fmt)
             assert torch.equal(back, (value.float() * scale[..., None]).to(dtype)), shift
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("group", [2, 12])
+def test_decode_keys_that_a_bias_masks_may_hold_anything(fmt, group):
+    lens = [100, 3000, 64]
+    cache, table, _, _ = _filled(lens, 16, 2, 64, fmt, 210)
+    q = torch.randn(3, 2 * group, 64, device=DEV).bfloat16()
+    bias = torch.randn(2 * group, 60, device=DEV)
+    bias[:, 59] = -math.inf
+    want = serving.decode_attention_paged(q, cache, table, _ints(lens), rel_bias=bias)
+    assert bool(torch.isfinite(want).all())
+    for value in (math.nan, math.inf):
+        for seq, pos in ((0, 30), (1, 2000), (1, 2940), (2, 4)):
+            at, inside = _slots(table, 16, seq, pos)
+            cache.k_scale[at, 1, inside] = value
+            cache.v_scale[at, 0, inside] = value
+        assert torch.equal(serving.decode_attention_paged(q, cache, table, _ints(lens), rel_bias=bias), want)

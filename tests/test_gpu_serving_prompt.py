@@ -320,3 +320,29 @@ def test_split_calls_on_two_streams_at_once():
             outs.append(serving.prompt_attention(q, k, v, cu_q, cu_k))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("d,n,m,heads,n_dist", [(64, 400, 400, 2, 41), (65, 300, 300, 80, 41), (64, 70, 3100, 2, 41), (128, 2000, 2000, 40, 300),
+                                                (200, 150, 150, 2, 41)])
+def test_keys_that_a_bias_masks_may_hold_anything(d, n, m, heads, n_dist, value):
+    """Keys and values outside a window, in the tiles, with split keys and row by row."""
+    q, k, v = _case([n], [m], heads, 1, d, torch.bfloat16, seed=22)
+    bias = torch.randn(heads, n_dist, generator=torch.Generator(device=DEV).manual_seed(23), device=DEV)
+    bias[:, -1] = -math.inf
+    spoiled = torch.zeros(m, dtype=torch.bool, device=DEV)
+    at = max(0, m - n) + 7
+    spoiled[[0, 5, at]] = True                                        # seen by queries up to n_dist - 2 positions on
+    reach = at + n_dist - 1 - (m - n)                                 # the first query that sees none of them
+    cu_q, cu_k = _cu([n]), _cu([m])
+    clean = serving.prompt_attention(q, k.masked_fill(spoiled[:, None, None], 0), v, cu_q, cu_k, scale=d ** -0.5, rel_bias=bias)
+    k[spoiled] = value
+    got = serving.prompt_attention(q, k, v, cu_q, cu_k, scale=d ** -0.5, rel_bias=bias)
+    assert 0 < reach < n and torch.equal(got[reach:], clean[reach:])
+    v[spoiled] = value
+    got = serving.prompt_attention(q, k, v, cu_q, cu_k, scale=d ** -0.5, rel_bias=bias)[reach:]
+    some = torch.linspace(0, n - reach - 1, 12, device=DEV).long()
+    k, v = (t.masked_fill(spoiled[:, None, None], 0) for t in (k, v))
+    for i in some.tolist():
+        _check(got[i:i + 1], q[reach + i:reach + i + 1], k[:m - n + reach + i + 1], v[:m - n + reach + i + 1], [1],
+               [m - n + reach + i + 1], d ** -0.5, bias)
