@@ -358,9 +358,12 @@ __global__ void __launch_bounds__(kRowsThreads) k_cache_read(const RowsArgs a) {
 // (g = lane / 4, c = lane % 4) holds bytes 16 c .. 16 c + 15 of every 64 of keys g and g + 8, and columns 16 g ..
 // of values 2c, 2c + 1, 2c + 8, 2c + 9.  Q is brought to fp16 by a power of two per head.  W comes out of S with
 // positions along g and heads along c and is turned by movmatrix.
-// Weights: p = exp2(s - m), w = p * value scale / r with r the largest p * value scale so far, so that rows of
-// small and large scale keep their accuracy in fp16.  m and r only move when p or w grew by more than 2^8 or
-// 2^12.
+// Weights: p = exp2(s - m), w = p * value scale / r in fp16, r being 2^-7 of the largest p * value scale so far, so
+// that rows of small and large scale keep their accuracy: half a step of fp16, and where w is subnormal 2^-32 of that
+// largest one.  m only moves when p grew by more than 2^8, and r moves with it: p and r are relative to the same m, so
+// the sums stay as they are.  r grows, and the sums are taken down, when w would pass 2^15.  (r left behind when m
+// moves would belong to weights that have just become small: a later row that has all the weight but a scale
+// 2^-20 of an earlier one's would be rounded to a few bits, or to nothing.)
 //
 // Measured: 64 sequences, 32 query and 8 key heads of 128, 554 MB of e4m3 codes and scales in 130 us (4.3
 // TB/s; int8 codes, which take fewer conversion instructions, 121 us).  Bound by the turning of codes into fp16
@@ -382,6 +385,8 @@ struct PagedArgs {
 constexpr int kPagedThreads = 128;
 constexpr int kPagedMaxSeqs = 4096;
 constexpr int kPagedMinTiles = 2;  // per warp
+constexpr float kUnitFloor = FLT_MIN;  // of r: 1 / r is finite
+constexpr float kUnitShare = 0x1p-7f, kWeightLimit = 0x1p15f;
 __host__ __device__ constexpr int paged_ctas(int nb) { return nb <= 5 ? 4 : (nb <= 8 ? 3 : 2); }  // per SM
 
 struct PagedShape {
@@ -407,6 +412,12 @@ __device__ __forceinline__ float paged_log2(float b) {  // a bias in units of lo
 __device__ __forceinline__ float paged_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float paged_inverse(float x) {  // to 2^-23; x and 1 / x are normal numbers
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -640,7 +651,9 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         m[r][h] = -INFINITY;
-        sum[r][h] = unit[r][h] = inv[r][h] = 0.f;
+        sum[r][h] = 0.f;
+        unit[r][h] = kUnitFloor;
+        inv[r][h] = 1.f / kUnitFloor;
         by_head[r][h] = __shfl_sync(0xffffffffu, factor[r], 4 * (2 * q + h));
       }
     }
@@ -714,11 +727,18 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
           const float next0 = fmaxf(m[r][0], column_max(top0)), next1 = fmaxf(m[r][1], column_max(top1));
           const float keep0 = next0 == -INFINITY ? 1.f : paged_exp2(m[r][0] - next0);
           const float keep1 = next1 == -INFINITY ? 1.f : paged_exp2(m[r][1] - next1);
+          const float moved0 = unit[r][0] * keep0, moved1 = unit[r][1] * keep1;
+          // below the least r the sums go down after all; without a maximum so far they are 0
+          const bool low = (moved0 < kUnitFloor && m[r][0] != -INFINITY) || (moved1 < kUnitFloor && m[r][1] != -INFINITY);
           m[r][0] = next0;
           m[r][1] = next1;
           sum[r][0] *= keep0;
           sum[r][1] *= keep1;
-          rescale(r, keep0, keep1);
+          unit[r][0] = fmaxf(moved0, kUnitFloor);
+          unit[r][1] = fmaxf(moved1, kUnitFloor);
+          inv[r][0] = paged_inverse(unit[r][0]);
+          inv[r][1] = paged_inverse(unit[r][1]);
+          if (__any_sync(0xffffffffu, low)) rescale(r, moved0 * inv[r][0], moved1 * inv[r][1]);
         }
         const float base0 = m[r][0] == -INFINITY ? 0.f : m[r][0], base1 = m[r][1] == -INFINITY ? 0.f : m[r][1];
         const float p0 = paged_exp2(s[0] - base0), p1 = paged_exp2(s[1] - base1);
@@ -729,14 +749,14 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         const float u0 = p0 != 0.f ? p0 * vs0 : 0.f, u1 = p1 != 0.f ? p1 * vs0 : 0.f;
         const float u2 = p2 != 0.f ? p2 * vs8 : 0.f, u3 = p3 != 0.f ? p3 * vs8 : 0.f;
         const float large0 = fmaxf(u0, u2), large1 = fmaxf(u1, u3);
-        if (__any_sync(0xffffffffu, large0 > unit[r][0] * 4096.f || large1 > unit[r][1] * 4096.f)) {
-          const float next0 = fmaxf(fmaxf(column_max(large0), unit[r][0]), 0x1p-100f);
-          const float next1 = fmaxf(fmaxf(column_max(large1), unit[r][1]), 0x1p-100f);
-          rescale(r, unit[r][0] / next0, unit[r][1] / next1);
+        if (__any_sync(0xffffffffu, large0 > unit[r][0] * kWeightLimit || large1 > unit[r][1] * kWeightLimit)) {
+          const float next0 = fmaxf(column_max(large0) * kUnitShare, unit[r][0]);
+          const float next1 = fmaxf(column_max(large1) * kUnitShare, unit[r][1]);
+          inv[r][0] = paged_inverse(next0);
+          inv[r][1] = paged_inverse(next1);
+          rescale(r, unit[r][0] * inv[r][0], unit[r][1] * inv[r][1]);
           unit[r][0] = next0;
           unit[r][1] = next1;
-          inv[r][0] = 1.f / next0;
-          inv[r][1] = 1.f / next1;
         }
         const __half2 h0 = __floats2half2_rn(u0 * inv[r][0], u1 * inv[r][1]);
         const __half2 h8 = __floats2half2_rn(u2 * inv[r][0], u3 * inv[r][1]);
@@ -814,7 +834,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
       for (int h = 0; h < 2; h++) {
         const int row = 8 * r + 2 * q + h;
         const float l = column_sum(sum[r][h]);
-        const float by = l == 0.f ? 0.f : unit[r][h] / l;
+        const float by = l == 0.f ? 0.f : 1.f / l, of = unit[r][h];  // of / l may be subnormal
         if (row >= n_heads) continue;
         const long long at = ((long long)seq * a.heads + head0 + row) * d;
         float *p = part + (size_t)row * row_floats;
@@ -826,7 +846,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
         for (int n = 0; n < 2 * NB; n++) {
           const int col = value_column<NB>(n, g);
           if (col >= d) continue;
-          const float v = o[n >> 1][r][2 * (n & 1) + h] * by;
+          const float v = o[n >> 1][r][2 * (n & 1) + h] * by * of;
           if (!whole) p[2 + col] = v;
           else if (a.dtype == QMOE_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[at + col] = from_f32<__nv_bfloat16>(v);
           else reinterpret_cast<__half *>(a.out)[at + col] = from_f32<__half>(v);

@@ -373,3 +373,40 @@ def test_decode_keys_that_a_bias_masks_may_hold_anything(fmt, group):
             cache.k_scale[at, 1, inside] = value
             cache.v_scale[at, 0, inside] = value
         assert torch.equal(serving.decode_attention_paged(q, cache, table, _ints(lens), rel_bias=bias), want)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("low,high", [(-30, 30), (-110, -80), (-110, 100)])
+def test_decode_value_rows_of_very_different_size(fmt, dtype, low, high):
+    """Three times in every sequence and head the scores rise by 40 units of log 2 and the value rows' size changes,
+    at other positions everywhere, so that they lie in the middle of a warp's run of tiles."""
+    if dtype == torch.float16 and high != 30:
+        pytest.skip("fp16 does not hold such values")
+    n_seqs, n, kv_heads, group, d, page = 40, 1000, 8, 2, 64, 64
+    g = torch.Generator(device=DEV).manual_seed(31)
+    direction = torch.where(torch.rand(kv_heads, d, generator=g, device=DEV) < 0.5, -1.0, 1.0)
+    at = torch.randint(1, n, (n_seqs, kv_heads, 3), generator=g, device=DEV).sort(-1).values
+    level = (torch.arange(n, device=DEV)[None, :, None, None] >= at[:, None]).sum(-1)               # [sequence, position, head]
+    size = torch.randint(low, high + 1, (n_seqs, kv_heads, 4), generator=g, device=DEV).gather(2, level.transpose(1, 2)).transpose(1, 2)
+    # q = direction / 8, |q|^2 = 1: a step of 40 * ln 2 in the scores (scale 1) is one of 40 * ln 2 * direction / 8 in k
+    k = direction / 8 * (level * 40 * math.log(2.0))[..., None] + 0.05 * torch.randn(n_seqs, n, kv_heads, d, generator=g, device=DEV)
+    v = torch.randn(n_seqs, n, kv_heads, d, generator=g, device=DEV) * torch.exp2(size.float())[..., None]
+    if dtype == torch.float16:
+        v = v / 2 ** 18                                                      # 2^-48 .. 2^14: what is too small is rounded away here
+    k, v = k.to(dtype).flatten(0, 1), v.to(dtype).flatten(0, 1)
+    q = (direction / 8).repeat_interleave(group, 0)[None].expand(n_seqs, -1, -1).to(dtype)
+    cache = serving.QuantCache(n_seqs * 16, page, kv_heads, d, DEV, fmt=fmt)
+    table = torch.arange(n_seqs * 16, dtype=torch.int32, device=DEV).view(n_seqs, 16)
+    serving.cache_append(cache, k, v, _cu([n] * n_seqs), _ints([0] * n_seqs), table)
+    got = serving.decode_attention_paged(q, cache, table, _ints([n] * n_seqs), scale=1.0).double()
+    kq, vq = ((value * scale.double()[..., None]).view(n_seqs, n, kv_heads, d) for value, scale in (ref.quantise(t, fmt) for t in (k, v)))
+    p = torch.softmax(torch.einsum("sphd,hd->shp", kq, (direction / 8).double()), -1)
+    out, mean = torch.einsum("shp,sphd->shd", p, vq), torch.einsum("shp,sphd->shd", p, vq.abs())
+    largest = torch.einsum("shp,sph->sh", p, vq.abs().amax(-1))[..., None]
+    # half a step of the output and of the fp16 weights, 2^-12 for scores of up to 2^7, and 2^-32 of the largest
+    # weight * row for each of the keys (weights that are subnormal in fp16); what the output type rounds to zero
+    bound = torch.finfo(dtype).eps / 2 * out.abs() + (2.0 ** -11 + 2.0 ** -12) * mean + n * 2.0 ** -32 * largest
+    bound = bound * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    err = (got.view(n_seqs, kv_heads, group, d) - out[:, :, None]).abs()
+    assert float((err / bound[:, :, None]).max()) <= 1
