@@ -143,7 +143,7 @@ __device__ __forceinline__ void find_slots(const RowsArgs &a, long long *s_slot)
     long long slot = -2;
     const int seq = row < a.n_rows ? packed_seq(a.cu, a.n_seqs, (int)row) : -1;
     if (seq >= 0) {
-      slot = cache_slot(a.c, seq, (long long)a.start[seq] + (row - a.cu[seq]));
+      slot = cache_slot(a.c, seq, (long long)a.start[seq] + (row - max(a.cu[seq], 0)));  // offsets are clamped to the tensor
       if (slot < 0) atomicAdd(a.c.status, 1);
     }
     s_slot[threadIdx.x] = slot;

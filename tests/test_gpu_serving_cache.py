@@ -410,3 +410,18 @@ def test_decode_value_rows_of_very_different_size(fmt, dtype, low, high):
     bound = bound * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
     err = (got.view(n_seqs, kv_heads, group, d) - out[:, :, None]).abs()
     assert float((err / bound[:, :, None]).max()) <= 1
+
+
+def test_cache_offsets_outside_the_rows_are_clamped():
+    x = torch.randn(20, 2, 64, device=DEV).bfloat16()
+    table, start = _ints([[0, 2], [1, 3]]), _ints([3, 5])
+    bad, good = _ints([-7, 12, 1 << 30]), _ints([0, 12, 20])
+    caches = [serving.QuantCache(4, 16, 2, 64, DEV) for _ in range(2)]
+    for cache, cu in zip(caches, (bad, good)):
+        serving.cache_append(cache, x, x, cu, start, table)
+        assert cache.refused() == 0
+    assert torch.equal(caches[0].k_scale, caches[1].k_scale)
+    assert torch.equal(caches[0].k_codes.view(torch.uint8), caches[1].k_codes.view(torch.uint8))
+    for a, b in zip(*(serving.cache_read(caches[1], cu, start, table, 20) for cu in (bad, good))):
+        assert torch.equal(a, b)
+    assert caches[1].refused() == 0
