@@ -106,6 +106,21 @@ def _rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6) -> torch.Tens
     return (v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps)).to(x.dtype) * w
 
 
+def common_uniform(uniform: Optional[torch.Tensor], n_new: int, n: int, device, world: int = 1, group=None) -> torch.Tensor:
+    """Random numbers fp32 ``[n_new, n]`` for sampling: ``uniform``, or drawn from torch's generator of ``device``.
+    Ranks that hold the same tokens have to draw the same ones, whatever the state of their generators: with
+    ``world`` > 1 all take those of the group's first rank (a collective call)."""
+    if uniform is None:
+        uniform = torch.rand((n_new, n), device=device)
+    if uniform.shape != (n_new, n) or uniform.dtype != torch.float32:
+        raise ValueError(f"uniform must be fp32 [{n_new}, {n}], got {uniform.dtype} {tuple(uniform.shape)}")
+    uniform = uniform.to(device).contiguous()
+    if world > 1:
+        uniform = uniform.clone()                   # the caller's stays as it is
+        dist.broadcast(uniform, group=group, group_src=0)
+    return uniform
+
+
 class SwitchDecoderLM:
     """``n_layers`` blocks of (self-attention, MoE FFN); greedy generation with a static KV cache."""
 
@@ -113,7 +128,7 @@ class SwitchDecoderLM:
                  max_len: int, device, seed: int = 0, rank: int = 0, world: int = 1, group=None,
                  drop_reference_layout: bool = True):
         self.d, self.h, self.hd, self.L, self.vocab, self.max_len = d_model, n_heads, d_model // n_heads, n_layers, vocab, max_len
-        self.dev = torch.device(device)
+        self.dev, self.world, self.group = torch.device(device), world, group
         g = torch.Generator().manual_seed(seed * 9973 + 1)
 
         def dense(*shape):
@@ -329,18 +344,15 @@ class SwitchDecoderLM:
                        cache_format: str = "e4m3", page_size: int = 64, use_graph: bool = True) -> torch.Tensor:
         """``n_new`` tokens for every prompt, int64 ``[n, n_new]``.  Tokens are sampled as
         :func:`qmoe_b200.serving.sample_tokens` does (``temperature`` 0: the largest logit) from ``uniform``
-        fp32 ``[n_new, n]``, by default torch's generator of the device.  The decoding step is captured into
+        fp32 ``[n_new, n]``, by default torch's generator of the device.  With several ranks every rank makes
+        the same call, and all sample from the first rank's numbers.  The decoding step is captured into
         a CUDA graph for this call when there are enough steps."""
         if n_new < 1:
             raise ValueError("n_new must be at least 1")
         if not 0.0 <= temperature < float("inf"):
             raise ValueError(f"temperature must be finite and not negative, got {temperature}")
         n = len(prompts)
-        if uniform is None:
-            uniform = torch.rand((n_new, n), device=self.dev)
-        if uniform.shape != (n_new, n) or uniform.dtype != torch.float32:
-            raise ValueError(f"uniform must be fp32 [{n_new}, {n}], got {uniform.dtype} {tuple(uniform.shape)}")
-        uniform = uniform.to(self.dev).contiguous()
+        uniform = common_uniform(uniform, n_new, n, self.dev, self.world, self.group)
         fixed = {"temperature": torch.full((n,), temperature, dtype=torch.float32, device=self.dev),
                  "top_k": torch.full((n,), top_k, dtype=torch.int32, device=self.dev),
                  "top_p": torch.full((n,), top_p, dtype=torch.float32, device=self.dev),
