@@ -15,7 +15,7 @@ small all-reduce per layer instead of two all-to-alls.
 from __future__ import annotations
 
 import math
-from typing import List, Optional
+from typing import List, Optional, Sequence
 
 import torch
 import torch.distributed as dist
@@ -47,19 +47,37 @@ class ReplicatedTokenMoE:
             return self(hidden, residual=x, logits=logits)
         return self(sub1.rms_norm(x, ln_weight), residual=x)
 
+    def _kept(self, choice: torch.Tensor, lens: Sequence[int]) -> torch.Tensor:
+        """``choice`` with -1 for the tokens that the capacity rule drops within their sequence; sequences of at
+        most ``capacity`` tokens lose none."""
+        kept, at = choice, 0
+        for count in lens:
+            if count > self.capacity:
+                kept = choice.clone() if kept is choice else kept
+                kept[at:at + count] = sub1.capacity_rule(choice[at:at + count], self.n_experts, count, self.capacity)
+            at += count
+        return kept
+
     def __call__(self, hidden: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                 logits: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """MoE output for ``hidden``; with ``residual`` (single-rank only) ``residual + output``."""
+                 logits: Optional[torch.Tensor] = None, lens: Optional[Sequence[int]] = None) -> torch.Tensor:
+        """MoE output for ``hidden``; with ``residual`` (single-rank only) ``residual + output``.  ``lens``: the
+        lengths of the sequences whose tokens ``hidden`` holds one after another (default: one sequence); the
+        capacity rule counts within a sequence (sub1.py:306-309)."""
         n, d = hidden.shape
+        capacity, ragged = self.capacity, False
+        if lens is not None and len(lens) > 1:
+            assert sum(lens) == n
+            # counted here, within each sequence; the steps below then drop nothing more
+            capacity, ragged = n, max(lens) > self.capacity
         if logits is None:
             logits = self.router(hidden).contiguous()
         if self.force is not None and n == 1:
             # measurement aid: the step's expert is given (a large logit), whatever the router computed
             logits = logits.index_fill(1, self.force, 1e4)
-        if n <= 32:
+        if n <= 32 and not ragged:
             # a decode step: routing, ranking and permutation in one launch (every rank does the same
             # routing on the same replicated token)
-            prob, offsets, slot, xs = sub1.route_small(logits, hidden, self.n_experts, self.capacity)
+            prob, offsets, slot, xs = sub1.route_small(logits, hidden, self.n_experts, capacity)
             if self.trace is not None and n == 1:                # decode steps only, not a short prefill
                 self.trace += offsets[1:] - offsets[:-1]
             if self.world == 1:
@@ -75,16 +93,18 @@ class ReplicatedTokenMoE:
                 return sub1.combine_add(ys, hidden, slot, prob, residual)
             return sub1.combine(ys, hidden, slot, prob)
         choice, prob = sub1.route_top1(logits)
+        if ragged:
+            choice = self._kept(choice, lens)
         if self.world == 1:
             # all experts are local: the single-GPU layer (route, rank, permute, FFN, combine)
-            bucket, rank, _, offsets = sub1.rank_buckets(choice, self.n_experts, n, self.capacity)
+            bucket, rank, _, offsets = sub1.rank_buckets(choice, self.n_experts, n, capacity)
             xs = torch.empty_like(hidden)
             slot = sub1.permute_rows(bucket, rank, offsets, hidden, xs)
             ys = sub1.grouped_ffn(self.store, offsets, xs, n)
             if residual is not None:
                 return sub1.combine_add(ys, hidden, slot, prob, residual)
             return sub1.combine(ys, hidden, slot, prob)
-        expert, _, _, _ = sub1.rank_buckets(choice, self.n_experts, n, self.capacity)
+        expert, _, _, _ = sub1.rank_buckets(choice, self.n_experts, n, capacity)
         lo = self.rank * self.local
         mine = (expert >= lo) & (expert < lo + self.local)
         local_choice = torch.where(mine, expert - lo, torch.full_like(expert, -1))
@@ -297,7 +317,7 @@ class SwitchDecoderLM:
         """Prefill ``prompts`` (int64 id vectors of any lengths) as one packed batch: causal attention within
         every prompt, keys and values into paged 8-bit caches (one per block, one page table for all) with
         room for ``n_new`` more tokens per sequence.  ``state.logits`` fp32 ``[n, vocab]`` are those behind
-        the prompts.  All tokens of a step count as one sequence for the router's capacity rule."""
+        the prompts.  The router's capacity rule counts within a prompt, as if it had come alone."""
         lens = [int(p.numel()) for p in prompts]
         if not lens or min(lens) < 1:
             raise ValueError("start_batch needs at least one prompt, and no empty one")
@@ -316,7 +336,7 @@ class SwitchDecoderLM:
             att = serving.prompt_attention(q, k, v, state.cu)
             serving.cache_append(cache, k, v, state.cu, state.start, state.table)
             x = x + att.view(n, -1) @ b["wo"].t()
-            x = x + b["moe"](_rms_norm(x, b["ln2"]).contiguous())
+            x = x + b["moe"](_rms_norm(x, b["ln2"]).contiguous(), lens=lens)
         last = x[state.cu[1:].long() - 1]
         state.logits = (_rms_norm(last, self.final_norm) @ self.lm_head.t()).float()
         return state
@@ -330,13 +350,13 @@ class SwitchDecoderLM:
             raise ValueError(f"tokens must have an entry per sequence ({state.lengths.numel()}), got {tuple(tokens.shape)}")
         x = self.embed[tokens.clamp(0, self.embed.shape[0] - 1)]
         n = x.shape[0]
-        seen = state.lengths + 1
+        seen, alone = state.lengths + 1, [1] * n        # one token of every sequence: none is over the capacity
         for b, cache in zip(self.blocks, state.caches):
             q, k, v = (sub1.rms_norm(x, b["ln1"]) @ b["wqkv"].t()).view(n, 3, self.h, self.hd).unbind(1)
             serving.cache_append(cache, k, v, state.one_each, state.lengths, state.table)
             att = serving.decode_attention_paged(q, cache, state.table, seen)
             x = x + att.view(n, -1) @ b["wo"].t()
-            x = x + b["moe"](sub1.rms_norm(x, b["ln2"]))
+            x = x + b["moe"](sub1.rms_norm(x, b["ln2"]), lens=alone)
         return (sub1.rms_norm(x, self.final_norm) @ self.lm_head.t()).float()
 
     def generate_batch(self, prompts: List[torch.Tensor], n_new: int, temperature: float = 0.0, top_k: int = 0,

@@ -3,7 +3,7 @@ together, against a plain re-statement of the stack."""
 import pytest
 import torch
 
-from qmoe_b200 import serving
+from qmoe_b200 import serving, sub1
 from qmoe_b200.decoder import SwitchDecoderLM, _rms_norm
 from tests import serving_ref as ref
 from tests.test_gpu_decoder import _dense_expert
@@ -154,3 +154,57 @@ def test_ids_and_logits_that_cannot_be_used():
     model.lm_head.fill_(float("nan"))
     with pytest.raises(RuntimeError, match="no distribution"):
         model.generate_batch([one, one], 6, temperature=1.0)
+
+
+def _capacity(model, tokens):
+    for b in model.blocks:
+        b["moe"].capacity = tokens
+
+
+@pytest.mark.parametrize("lens", [[5, 9, 1], [5, 40, 1, 3, 17], [2, 2], [60]])
+@pytest.mark.parametrize("capacity", [1, 3, 1024])
+def test_capacity_counts_within_a_sequence(lens, capacity):
+    """Packed sequences through an MoE block against each by itself."""
+    model = _model(n_layers=1)
+    _capacity(model, capacity)
+    moe = model.blocks[0]["moe"]
+    hidden = torch.randn(sum(lens), model.d, generator=torch.Generator().manual_seed(4)).bfloat16().to(model.dev)
+    got = moe(hidden, lens=lens)
+    rows = hidden.split(lens)
+    want = torch.cat([moe(h.contiguous()) for h in rows])
+    assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+    choice, _ = sub1.route_top1(moe.router(hidden).contiguous())
+    dropped = torch.cat([sub1.capacity_rule(c.contiguous(), moe.n_experts, c.numel(), capacity) for c in choice.split(lens)]) < 0
+    if max(lens) > capacity * moe.n_experts or max(lens) <= capacity:     # some expert has more than it takes; none can have
+        assert bool(dropped.any()) == (max(lens) > capacity)
+    assert torch.equal(got[dropped], want[dropped])                    # passed through
+    residual = torch.randn_like(hidden)
+    again = moe(hidden, residual=residual, lens=lens)
+    assert float((again.float() - (residual + got).float()).abs().max()) <= 2.0 ** -7 * float((residual + got).float().abs().max())
+
+
+@pytest.mark.parametrize("lens", [[7, 3, 8], [8, 8, 8, 8, 8, 8]])
+def test_prompts_lose_no_tokens_to_each_other(lens):
+    """Prompts of at most the capacity, together far over it: as if there were none.  Longer ones: as if alone."""
+    model = _model(n_layers=1)
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in lens]
+    unlimited = model.start_batch(prompts, 1).logits
+    _capacity(model, max(lens))
+    assert torch.equal(model.start_batch(prompts, 1).logits, unlimited)
+    _capacity(model, 2)
+    alone = torch.cat([model.start_batch([p], 1).logits for p in prompts])
+    together = model.start_batch(prompts, 1).logits
+    assert float((together - alone).abs().max()) <= 2e-2 * float(alone.abs().max())
+    assert not torch.equal(together, unlimited)
+
+
+@pytest.mark.parametrize("n", [6, 40])
+def test_a_step_is_one_token_of_every_sequence(n):
+    model = _model(n_layers=1)
+    g = torch.Generator().manual_seed(6)
+    state = model.start_batch([torch.randint(0, VOCAB, (3,), generator=g) for _ in range(n)], 2)
+    ids = torch.randint(0, VOCAB, (n,), generator=g).to(model.dev)
+    want = model.step_batch(state, ids)
+    _capacity(model, 1)
+    assert torch.equal(model.step_batch(state, ids), want)
