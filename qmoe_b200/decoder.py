@@ -141,6 +141,16 @@ def common_uniform(uniform: Optional[torch.Tensor], n_new: int, n: int, device, 
     return uniform
 
 
+def worst_of_ranks(counts: Sequence[int], device, world: int = 1, group=None) -> List[int]:
+    """The largest of every count over the ranks (with ``world`` > 1 a collective call), so that all of them raise
+    when one has to."""
+    if world > 1:
+        t = torch.tensor(list(counts), dtype=torch.int64, device=device)
+        dist.all_reduce(t, op=dist.ReduceOp.MAX, group=group)
+        counts = t.tolist()
+    return list(counts)
+
+
 class SwitchDecoderLM:
     """``n_layers`` blocks of (self-attention, MoE FFN); greedy generation with a static KV cache."""
 
@@ -377,6 +387,7 @@ class SwitchDecoderLM:
                  "top_k": torch.full((n,), top_k, dtype=torch.int32, device=self.dev),
                  "top_p": torch.full((n,), top_p, dtype=torch.float32, device=self.dev),
                  "min_p": torch.full((n,), min_p, dtype=torch.float32, device=self.dev)}
+        waits_before = sub1.tile_timeouts(self.dev)
         state = self.start_batch(prompts, n_new, cache_format, page_size)
         tokens = serving.sample_tokens(state.logits, uniform[0], **fixed)
         out = [tokens.clone()]
@@ -400,7 +411,10 @@ class SwitchDecoderLM:
         finally:
             if graph is not None:
                 graph.close()
-        refused = sum(c.refused() for c in state.caches)
+        refused, gave_up = worst_of_ranks([sum(c.refused() for c in state.caches), sub1.tile_timeouts(self.dev) - waits_before],
+                                          self.dev, self.world, self.group)
+        if gave_up > 0:
+            raise RuntimeError(f"{gave_up} CTA(s) gave up waiting: the tokens are not to be used")
         if refused:
             raise RuntimeError(f"{refused} cache positions had no page")
         tokens = torch.stack(out, 1)

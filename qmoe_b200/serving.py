@@ -105,7 +105,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     to them at column ``min(distance, n - 1)``, the distance between query and key.  Keys whose bias
     is ``-inf`` are masked, whatever they and their values hold.  Returns ``out`` ``[total_q, heads, head_dim]`` (any strides
     over the first two axes, memory apart from the inputs'); rows that no sequence owns are left as they
-    were (uninitialised when ``out`` is not given)."""
+    were (uninitialised when ``out`` is not given).  The kernel's waits are bounded; that none ran out is seen by
+    :func:`qmoe_b200.sub1.check_tile_status` where the caller synchronises."""
     _need(q, "q", (torch.bfloat16, torch.float16), 3, packed=False)
     dev = q.device
     for name, t in (("k", k), ("v", v)):

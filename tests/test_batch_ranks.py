@@ -7,7 +7,7 @@ import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
 
-from qmoe_b200.decoder import common_uniform
+from qmoe_b200.decoder import common_uniform, worst_of_ranks
 
 
 def _free_port():
@@ -70,3 +70,19 @@ def test_generate_batch_takes_the_common_numbers(monkeypatch):
     with pytest.raises(Seen) as seen:
         model.generate_batch([torch.zeros(2, dtype=torch.int64)] * 3, 6, temperature=1.0)
     assert seen.value.args == (None, 6, 3, 4, "a group")
+
+
+def _count_worker(rank, world, port, result_dir):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        torch.save(worst_of_ranks([rank, 0, 5 - rank], "cpu", world), os.path.join(result_dir, f"r{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_every_rank_learns_of_a_failure_on_one(tmp_path):
+    mp.spawn(_count_worker, args=(2, _free_port(), str(tmp_path)), nprocs=2, join=True)
+    for r in range(2):
+        assert torch.load(tmp_path / f"r{r}.pt") == [1, 0, 5]
+    assert worst_of_ranks([3, 0], "cpu") == [3, 0]

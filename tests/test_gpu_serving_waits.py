@@ -63,3 +63,18 @@ def test_rows_computed_again_take_longer_than_a_wait():
         got = serving.prompt_attention(q, k, v, cu_q, cu_k, out=torch.zeros_like(q))
     assert sub1.tile_timeouts(DEV, reset=True) == 0
     assert bool((got == float("inf")).all())
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_generation_does_not_return_tokens_behind_a_wait_that_ran_out(use_graph):
+    from qmoe_b200.decoder import SwitchDecoderLM
+    model = SwitchDecoderLM(d_model=128, d_ff=256, n_experts=4, n_layers=1, n_heads=2, vocab=64, max_len=64, device=DEV, seed=1,
+                            drop_reference_layout=False)
+    prompts = [torch.arange(20) % 64, torch.arange(3)]
+    want = model.generate_batch(prompts, 8, use_graph=use_graph)
+    assert sub1.tile_timeouts(DEV, reset=True) == 0
+    with wait_limit(1), pytest.raises(RuntimeError, match="gave up"):
+        model.generate_batch(prompts, 8, use_graph=use_graph)
+    # an earlier call's count is that caller's to clear: it does not make this one fail
+    assert torch.equal(model.generate_batch(prompts, 8, use_graph=use_graph), want)
+    assert sub1.tile_timeouts(DEV, reset=True) > 0
