@@ -405,6 +405,8 @@ __device__ __forceinline__ long long paged_quota(long long total, int warps) {
 __device__ __forceinline__ int paged_seen(const PagedArgs &a, int seq) {
   return (int)max(0LL, min((long long)a.lengths[seq], (long long)a.c.max_pages << a.c.page_shift));
 }
+// Tiles of that many positions, which may be 2^31 - 1.
+__device__ __forceinline__ int paged_tiles(int seen) { return (int)(((uint32_t)seen + 15u) / 16u); }
 
 __device__ __forceinline__ float paged_log2(float b) {  // a bias in units of log 2; the lowest values stay finite
   return b == -INFINITY ? b : fmaxf(b * 1.4426950408889634f, -FLT_MAX);
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
     const int s = s0 + tid;
     const int seen = s < a.n_seqs ? paged_seen(a, s) : 0;
     if (s < a.n_seqs) s_seen[s] = seen;
-    long long upto = (long long)((seen + 15) / 16) * per_seq;
+    long long upto = (long long)paged_tiles(seen) * per_seq;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
       if (s_prefix[mid] <= x) lo = mid;
       else hi = mid - 1;
     }
-    const int seq = lo, seen = s_seen[seq], n_tiles = (seen + 15) / 16;
+    const int seq = lo, seen = s_seen[seq], n_tiles = paged_tiles(seen);
     const long long in_seq = x - s_prefix[seq];
     const int which = in_seq <= 0x7fffffff ? (int)((uint32_t)in_seq / (uint32_t)n_tiles) : (int)(in_seq / n_tiles);
     const int tile0 = (int)(in_seq - (long long)which * n_tiles);
@@ -717,7 +719,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas(NB)) k_decode_paged(
             s[i] = b == -INFINITY ? b : s[i] + b;  // chosen, not added: a masked key may hold anything
           }
         }
-        if (pos0 + 16 > seen) {
+        if (seen - pos0 < 16) {
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (pos0 + 8 * (i >> 1) + g >= seen) s[i] = -INFINITY;
@@ -868,7 +870,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_decode_join(const PagedArgs a)
   const int seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads, d = a.c.head_dim, row_floats = shape.width + 2;
   const int kv = head / shape.group, block = head % shape.group / 16, row = head % shape.group % 16;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seen = paged_seen(a, seq), n_tiles = (seen + 15) / 16;
+  const int seen = paged_seen(a, seq), n_tiles = paged_tiles(seen);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first kernel ends
   if (tid == 0 && head % shape.group == 0 && a.lengths[seq] > seen) atomicAdd(a.c.status, 1);
   auto store = [&](int col, float v) {

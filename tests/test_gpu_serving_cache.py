@@ -425,3 +425,21 @@ def test_cache_offsets_outside_the_rows_are_clamped():
     for a, b in zip(*(serving.cache_read(caches[1], cu, start, table, 20) for cu in (bad, good))):
         assert torch.equal(a, b)
     assert caches[1].refused() == 0
+
+
+def test_decode_of_as_many_positions_as_a_length_can_say():
+    """2^31 - 1 positions in a table that has room for them, all but 2047 without a page, next to a short sequence."""
+    most, page = 2 ** 31 - 1, 1024
+    cache = serving.QuantCache(3, page, 1, 16, DEV)
+    table = torch.full((2, 2 ** 21), -1, dtype=torch.int32, device=DEV)
+    table[0, 0], table[0, -1], table[1, 0] = 0, 1, 2
+    k, v = (torch.randn(2052, 1, 16, device=DEV).bfloat16() for _ in range(2))
+    serving.cache_append(cache, k[:1024], v[:1024], _cu([1024]), _ints([0]), table[:1])
+    serving.cache_append(cache, k[1024:2047], v[1024:2047], _cu([1023]), _ints([most - 1023]), table[:1])   # the last page but its last place
+    serving.cache_append(cache, k[2047:2052], v[2047:2052], _cu([5]), _ints([0]), table[1:])
+    assert cache.refused() == 0
+    q = torch.randn(2, 1, 16, device=DEV).bfloat16()
+    got = serving.decode_attention_paged(q, cache, table, _ints([most, 5]))
+    assert cache.refused(reset=True) == 2 ** 27 - 2 * 64                    # tiles of 16 positions without a page
+    kq, vq = (value * scale.double()[..., None] for value, scale in (ref.quantise(t, "e4m3") for t in (k, v)))
+    _check_decode(got, q, kq, vq, [2047, 5], 0.25)
