@@ -27,10 +27,6 @@ __device__ __forceinline__ long long cache_slot(const CacheView &c, int seq, lon
   return (((long long)page * c.kv_heads) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
 }
 
-__device__ __forceinline__ float from_e4m3(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-}
-
 // Four codes to two pairs of fp16: (bytes 0, 1) and (bytes 2, 3).  int8: 0x6400 + (code + 128) is 1024 +
 // code + 128 in fp16.
 template <int FMT>
@@ -88,11 +84,6 @@ __device__ __forceinline__ uint32_t quantise4(const float (&x)[4], const RowScal
   for (int i = 0; i < 4; i++) n[i] = __float_as_uint(q[i] + 12582912.f);
   return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
 }
-template <int FMT>
-__device__ __forceinline__ float code_value(uint8_t c) {
-  return FMT == QMOE_CACHE_E4M3 ? from_e4m3(c) : (float)(int8_t)c;
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack_values(float lo, float hi);
 template <>

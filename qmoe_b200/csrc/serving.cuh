@@ -2,7 +2,6 @@
 #pragma once
 
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <float.h>
 
 #include "common.cuh"
