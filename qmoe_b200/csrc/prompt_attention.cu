@@ -109,8 +109,12 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // sum are taken relative to the older maximum, which is exact up to rounding since both are scaled alike.
 // P is rounded to the type of the inputs for the second product (half a step of it relative to every
 // weight); the sum is taken from the unrounded fp32 weights.
-// A value row that is not finite would spoil queries that give it weight 0 (0 * inf): a query row whose
-// result is not finite is computed again key by key.
+// A query that sees a score of NaN or +inf has a sum of NaN, or one that no finite scores reach (pair_exp2 turns NaN
+// into a huge number): its output is NaN, as the formula has it.  A value row that is not finite would spoil queries
+// that give it weight 0 (0 * inf): a query row whose sum is in order and whose result is not finite is computed again
+// key by key, a warp a row, at some hundred times the time of the tiles: 4096 tokens, 32 heads of 128, take 120 us, with
+// an infinite first value row, which every query sees, 270 ms; with NaN in its key instead 120 us (had they been
+// computed again, as long).
 // All waits are bounded (kPromptWait); when one runs out the CTA counts itself in d_prompt_timeouts, waits for its
 // copies and products in flight, frees its tensor memory and returns.
 constexpr int kPromptThreads = 512;
@@ -121,6 +125,7 @@ constexpr int kItems = 4;         // decided ahead
 constexpr int kItemReaders = 10;  // arrivals that give an item back: eight softmax warps, one for products, one for copies
 constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
 constexpr int kPolyPairs = 2;
+constexpr float kLargestSum = 0x1p100f;  // of finite scores: 2^25 weights of at most 2^8 are far below
 constexpr int kWave = 148;      // CTAs at a time
 constexpr int kMaxParts = 32;   // a warp's lanes look after one each when they are joined
 constexpr unsigned long long kPromptWait = 4000000000ull;  // ns without progress
@@ -743,7 +748,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       }
       // Rows go through shared memory, 64 columns at a time, so that a warp writes them one after another instead
       // of one piece of 32 rows at a time.
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const bool lost = !(sum <= kLargestSum);  // a score was NaN or +inf
+      const float inv = lost ? __int_as_float(0x7fffffff) : (sum == 0.f ? 0.f : 1.f / sum);
       uint8_t *stage = stage_out + warp * 4096;
       const int t0 = t & ~31, rows = min(32, n - (tile0 + t0));  // of this warp
       T *out = reinterpret_cast<T *>(a.out) + (item.q_row + (long long)(tile0 + t0)) * a.s.out_row + head * a.s.out_head;
@@ -790,7 +796,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         __syncwarp();
       }
       tc_fence_before();
-      unsigned again = __ballot_sync(0xffffffffu, live && !finite);
+      unsigned again = __ballot_sync(0xffffffffu, live && !finite && !lost);
       while (again != 0) {
         const int l = __ffs(again) - 1;
         again &= again - 1;
@@ -816,7 +822,7 @@ __global__ void __launch_bounds__(kPartsThreads) k_prompt_join(const PromptArgs 
   const int seq = packed_seq(a.cu_q, a.s.n_seqs, row);
   if (seq < 0) return;
   const int2 rq = packed_rows(a.cu_q, seq, a.s.total_q), rk = packed_rows(a.cu_k, seq, a.s.total_k);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the parts are worked on
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched as the last CTAs of the first kernel end
   const float2 stat = lane < a.n_parts ? a.part_stat[item * a.n_parts + lane] : make_float2(-INFINITY, 0.f);
   float top = stat.x;
 #pragma unroll
@@ -839,7 +845,8 @@ __global__ void __launch_bounds__(kPartsThreads) k_prompt_join(const PromptArgs 
   }
   bool finite = true;
   T *out = reinterpret_cast<T *>(a.out) + row * a.s.out_row + head * a.s.out_head + 4 * lane;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const bool lost = __any_sync(0xffffffffu, !(stat.y <= kLargestSum));  // a score was NaN or +inf
+  const float inv = lost ? __int_as_float(0x7fffffff) : (sum == 0.f ? 0.f : 1.f / sum);
   __align__(8) T v[4];
 #pragma unroll
   for (int x = 0; x < 4; x++) {
@@ -847,7 +854,7 @@ __global__ void __launch_bounds__(kPartsThreads) k_prompt_join(const PromptArgs 
     finite = finite && (4 * lane + x >= d || fabsf(o) <= FLT_MAX);
     v[x] = from_f32<T>(o);
   }
-  if (!__all_sync(0xffffffffu, finite)) {
+  if (!lost && !__all_sync(0xffffffffu, finite)) {
     attend_row<T, 4>(a, head, row, rq, rk);
   } else if (4 * lane + 4 <= d && (reinterpret_cast<uintptr_t>(out) & 7u) == 0) {
     *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(v);

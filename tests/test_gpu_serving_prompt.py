@@ -346,3 +346,51 @@ def test_keys_that_a_bias_masks_may_hold_anything(d, n, m, heads, n_dist, value)
     for i in some.tolist():
         _check(got[i:i + 1], q[reach + i:reach + i + 1], k[:m - n + reach + i + 1], v[:m - n + reach + i + 1], [1],
                [m - n + reach + i + 1], d ** -0.5, bias)
+
+
+def _time(call):
+    call()
+    events = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    events[0].record()
+    call()
+    events[1].record()
+    torch.cuda.synchronize()
+    return events[0].elapsed_time(events[1])
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("heads,n,m", [(32, 4096, 4096), (8, 256, 8192)])
+def test_scores_that_are_not_finite_cost_no_time(heads, n, m, value):
+    """A key that every query sees and whose scores are NaN, or +inf for some queries: NaN where a score is, at the
+    speed of finite inputs (computed key by key, these calls would take hundreds of times as long)."""
+    q, k, v = _case([n], [m], heads, heads // 4, 128, torch.bfloat16, seed=24)
+    cu_q, cu_k = _cu([n]), _cu([m])
+    call = lambda: serving.prompt_attention(q, k, v, cu_q, cu_k)  # noqa: E731
+    clean, finite = call(), _time(call)
+    k[0, :, 0] = value                                          # infinite scores of both signs
+    got, spoiled = call(), _time(call)
+    if math.isnan(value):
+        bad = torch.ones(n, heads, dtype=torch.bool, device=DEV)
+    else:
+        bad = q[:, :, 0] > 0
+        k[0] = 0
+        k = k[1:].contiguous()                                  # -inf: as if the key were not there
+        some = torch.nonzero(~bad & (torch.arange(n, device=DEV) % 97 == 40)[:, None])[:40]
+        for i, a in some.tolist():
+            seen = m - n + i
+            _check(got[i:i + 1, a:a + 1], q[i:i + 1, a:a + 1], k[:seen, a // 4:a // 4 + 1], v[1:seen + 1, a // 4:a // 4 + 1], [1], [seen], 128 ** -0.5)
+    assert bool(got[bad].isnan().all()) and not bool(got[~bad].isnan().any()) and bool(clean.isfinite().all())
+    assert spoiled < 5 * finite + 0.5
+
+
+@pytest.mark.parametrize("column", range(16))
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_nan_key_in_every_column_of_a_tile(column, d):
+    """Whichever way a key's weight is computed, and however many of them there are."""
+    n = 400
+    q, k, v = _case([n], [n], 2, 2, d, torch.bfloat16, seed=25)
+    clean = serving.prompt_attention(q, k, v, _cu([n]))
+    k[column, 0] = math.nan
+    k[column::16, 1] = math.nan
+    got = serving.prompt_attention(q, k, v, _cu([n]))
+    assert torch.equal(got[:column], clean[:column]) and bool(got[column:].isnan().all())
