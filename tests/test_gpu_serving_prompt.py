@@ -394,3 +394,25 @@ def test_a_nan_key_in_every_column_of_a_tile(column, d):
     k[column::16, 1] = math.nan
     got = serving.prompt_attention(q, k, v, _cu([n]))
     assert torch.equal(got[:column], clean[:column]) and bool(got[column:].isnan().all())
+
+
+def test_rows_computed_again_stay_within_reason():
+    """An infinite value that every query sees, a key that half of them see, and a masked one: every row is computed
+    again.  (One key at a time this call takes 70 ms.)"""
+    n, heads = 2048, 32
+    q, k, v = _case([n], [n], heads, 8, 128, torch.bfloat16, seed=26)
+    v[0, :, 5] = math.inf
+    v[n // 2, :, 7] = -math.inf
+    v[n - 1, :, 9] = math.nan
+    cu = _cu([n])
+    got = serving.prompt_attention(q, k, v, cu)
+    assert _time(lambda: serving.prompt_attention(q, k, v, cu)) < 35
+    finite = torch.ones_like(got, dtype=torch.bool)
+    finite[:, :, 5] = finite[n // 2:, :, 7] = finite[n - 1:, :, 9] = False
+    assert torch.equal(got.isfinite(), finite)
+    assert bool((got[:, :, 5] == math.inf).all()) and bool((got[n // 2:, :, 7] == -math.inf).all()) and bool(got[n - 1, :, 9].isnan().all())
+    v[~v.isfinite()] = 0
+    clean = serving.prompt_attention(q, k, v, cu)
+    # two computations of the same row, each within the bound of the tests above
+    size = v.abs().max().double()
+    assert float((got.double() - clean.double())[finite].abs().max()) <= 2.0 ** -7 * float(size) * 2
