@@ -443,7 +443,8 @@ typedef struct qmoe_prompt_args {
  * with bias = rel_bias_dev[h * n_dist + min(distance, n_dist - 1)] (fp32, may be NULL), the distance
  * being i + m - n - j: the one-directional relative bias of T5 / Switch (scale 1).  A key whose bias is -inf is
  * masked, whatever it holds.  Statistics and
- * sums are fp32.  At most 262140 query rows, 2^25 key rows and 32768 sequences a call.  Every wait of the
+ * sums are fp32.  At most 2^25 query rows (262140 with head_dim above 128), 2^25 key rows and 32768
+ * sequences a call.  Every wait of the
  * tensor-core kernel is bounded (4 s without progress); a CTA whose wait runs out leaves the output rows that it has not
  * finished as they were (of split keys: anything) and is counted by qmoe_moe_tile_timeouts.  qmoe_prompt_set_wait_limit(ns)
  * lowers the bound (1: give up without polling; 0: back to the default), so that a test can make a wait run out.

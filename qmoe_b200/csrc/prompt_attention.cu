@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       // ---- copies: Q, then K 0, V 0, K 1, V 1, ... of one item after another
       const int t = tid - 384;
       bool ok = true;
-      int copied = 0, first = 0, q_item = -1;  // buffers filled so far, at the beginning of the item; last item whose queries came
+      unsigned long long copied = 0, first = 0;  // buffers filled so far, at the beginning of the item
+      int q_item = -1;                           // last item whose queries came
       for (int x = 0;; x++) {
         PromptItem item;
         // one decision for all, thread 0's: how often the threads meet below depends on the item, which must not have
@@ -391,7 +392,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         }
         if (t == 0) {
           for (int c = 0; ok && c < n_tma; c++) {
-            const int at = first + c, stage = at % kStages;
+            const unsigned long long at = first + c;
+            const int stage = at % kStages;
             if (at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, s_fail);
             if (!ok) break;
             const uint32_t full = bar(s_bar.kv_full[stage]);
@@ -405,7 +407,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         __syncwarp();
         bool gave_up = false;
         for (int c = n_tma; c < 2 * n_steps; c++) {
-          const int at = first + c, stage = at % kStages;
+          const unsigned long long at = first + c;
+          const int stage = at % kStages;
           if (t == 0) {
             if (ok && at >= kStages) ok = wait_or_fail(bar(s_bar.kv_empty[stage]), (at / kStages - 1) & 1, s_fail);
             s_stop[c & 1] = !ok;
@@ -436,7 +439,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       // Copies in flight land before the block ends, whoever gave up and whenever; of every buffer its last filling.
       if (t == 0) {
         if (q_item >= 0) mbar_wait(bar(s_bar.q_full), q_item & 1);
-        for (int c = max(0, copied - kStages); c < copied; c++) mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
+        for (unsigned long long c = copied > kStages ? copied - kStages : 0; c < copied; c++)
+          mbar_wait(bar(s_bar.kv_full[c % kStages]), (c / kStages) & 1);
       }
     } else if (warp == 9) {
       // ---- what to work on.  Of 32 sequences at a time, the tiles with the most key tiles first, every tile for all
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       const bool bf16 = a.s.dtype == QMOE_BF16;
       const uint32_t idesc_s = make_instr_desc(kTileRows, kTileRows, bf16);
       const uint32_t idesc_o = make_instr_desc(kTileRows, 8 * chunks, bf16, true);
-      int first = 0, done[2] = {0, 0};  // buffers used and products of each tile before this item
+      uint32_t first = 0, done[2] = {0, 0};  // buffers used and products of each tile before this item; may wrap round
       auto tile_addr = [&](int c) { return smem_u32(ring) + ((first + c) % kStages) * tile_bytes; };
       auto wait_tile = [&](int c) {
         return __all_sync(0xffffffffu, wait_or_fail(bar(s_bar.kv_full[(first + c) % kStages]), ((first + c) / kStages) & 1, s_fail));
@@ -592,7 +596,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
     const uint32_t t_s = lane_base + i * kTileRows, t_o = lane_base + 256 + i * kTileRows;
     const int o_cols = 8 * chunks;
     const float sl2 = a.s.scale * kLog2e;
-    int done = 0;  // key tiles before this item
+    uint32_t done = 0;  // key tiles before this item; may wrap round
     bool ok = true;
     for (int x = 0;; x++) {
       PromptItem item;
@@ -1071,8 +1075,10 @@ extern "C" int qmoe_prompt_attention(const qmoe_prompt_args *args, int device, v
   QMOE_REQUIRE(isfinite(a.s.scale), "scale is not finite");
   if (a.s.n_seqs == 0 || a.s.total_q == 0) return QMOE_OK;
   QMOE_REQUIRE(a.q && a.out && (a.s.total_k == 0 || (a.k && a.v)), "null device pointer");
-  if (a.s.head_dim > 256 || a.s.total_q > (1 << 18) - 4 || a.s.total_k > (1 << 25) || a.s.n_seqs > 32768) {
-    set_error("%s: head_dim <= 256, 262140 query rows, 2^25 key rows and 32768 sequences are supported", __func__);
+  // Keys: an item's 2^18 tiles take about half a second, far less than a wait's bound.  Queries of wide heads: the rows
+  // kernel's grid.
+  if (a.s.head_dim > 256 || a.s.total_q > (a.s.head_dim > kTileRows ? (1 << 18) - 4 : 1 << 25) || a.s.total_k > (1 << 25) || a.s.n_seqs > 32768) {
+    set_error("%s: head_dim <= 256, 2^25 query rows (262140 of more than 128 values), 2^25 key rows and 32768 sequences are supported", __func__);
     return QMOE_ERR_UNSUPPORTED;
   }
   QMOE_REQUIRE(qmoe_prompt_work_bytes(args) == 0 || (args->work_dev != nullptr && (reinterpret_cast<uintptr_t>(args->work_dev) & 255u) == 0),

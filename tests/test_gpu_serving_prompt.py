@@ -416,3 +416,16 @@ def test_rows_computed_again_stay_within_reason():
     # two computations of the same row, each within the bound of the tests above
     size = v.abs().max().double()
     assert float((got.double() - clean.double())[finite].abs().max()) <= 2.0 ** -7 * float(size) * 2
+
+
+def test_more_query_rows_than_a_grid_axis():
+    """270000 rows; heads of more than 128 values are refused beyond 262140."""
+    lens = [900] * 300
+    q, k, v = _case(lens, lens, 2, 1, 16, torch.bfloat16, seed=27)
+    got = serving.prompt_attention(q, k, v, _cu(lens))
+    for i in (0, 150, 291, 299):
+        rows = slice(900 * i, 900 * i + 900)
+        _check(got[rows], q[rows], k[rows], v[rows], [900], [900], 0.25)
+    wide = torch.zeros(1, 1, 136, dtype=torch.bfloat16, device=DEV).expand(270000, 1, 136)
+    with pytest.raises(RuntimeError, match="262140"):
+        serving.prompt_attention(wide, wide, wide, _cu([270000]))

@@ -217,3 +217,8 @@ def test_waits_for_tensor_memory_name_the_values_they_guard():
 def test_wait_limit_is_not_negative():
     assert _lib.load().qmoe_prompt_set_wait_limit(-1) == _lib.ERR_INVALID_ARG
     assert _lib.load().qmoe_prompt_set_wait_limit(0) == _lib.OK
+
+
+@pytest.mark.parametrize("rows,head_dim,status", [((1 << 25) + 1, 64, _lib.ERR_UNSUPPORTED), ((1 << 18) - 3, 129, _lib.ERR_UNSUPPORTED)])
+def test_too_many_query_rows(rows, head_dim, status):
+    assert _prompt(_shape(total_q=rows, head_dim=head_dim, q_row=2 * 136, q_head=136, k_row=136, k_head=136, v_row=136, v_head=136)) == status
