@@ -551,7 +551,8 @@ int qmoe_sub1_release(int device);
  * counterpart in the reference, which reads `dec` directly in its kernel (sub1_cuda_kernel.cu:188). */
 int qmoe_sub1_forget(const int32_t *dec_dev, int device);
 
-/* Status of the tensor-core tile kernels inside qmoe_moe_grouped_ffn.  Each of their waits on an
+/* Status of the tensor-core tile kernels inside qmoe_moe_grouped_ffn (and of qmoe_prompt_attention, whose CTAs
+ * are counted with them).  Each of their waits on an
  * MMA-completion barrier is bounded; a CTA whose wait runs out stops, writes zeros for the output
  * rows it did not finish and adds one to a per-device word that no later call clears.
  * qmoe_moe_tile_timeouts synchronises the device, stores that word in *count_out and clears it when

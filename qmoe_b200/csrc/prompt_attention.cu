@@ -123,12 +123,14 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // Few items with many keys are split along the keys (key_parts): every part leaves its unfinished rows, maximum and
 // sum in the workspace, and a second kernel joins them.
 //
-// Bound by the chain scores -> softmax -> product of each tile: a step of 2 x 128 queries by 128 keys takes 3200
-// to 3600 clocks, of which the tensor core works 2048 at head_dim 128.  The exponentials are the softmax's
+// Bound by the chain scores -> softmax -> product of each tile: a step of 2 x 128 queries by 128 keys takes 3200 clocks
+// over one long prompt and 3700 over uneven ones, of which the tensor core works 2048 at head_dim 128 (in 900 to 1000
+// of them a softmax warp waits for its scores).  The same warps rescale O, and write an item's output in another 4600
+// clocks, in which the tensor core has nothing to do: a quarter of the time of 16 uneven prompts.  The exponentials are the softmax's
 // largest part (a special function unit gives 16 results a clock and SM: 2048 clocks a step), so two pairs of
 // eight are polynomials on the FMA units (1165 instead of 1143 TFLOP/s over one prompt of 8192 tokens).
-// One prompt of 16384 tokens, 32 heads of 128: 1.88 to 1.98 ms, 1.11 to 1.17 PFLOP/s; 16 uneven prompts of 8192 tokens
-// together 93 us.
+// One prompt of 16384 tokens, 32 heads of 128: 1.96 to 2.01 ms, 1.10 to 1.12 PFLOP/s; 16 uneven prompts of 8192 tokens
+// together 91 to 94 us.
 //
 // Every tile lies in shared memory as rows of 64 columns (128 bytes) under the 128-byte swizzle, one block
 // of 128 rows per 64 columns: K-major for Q and K, and the same bytes with the head axis contiguous for V.

@@ -118,8 +118,9 @@ struct RowsArgs {
 // Where the 16-bit tensors' rows do not begin on 16-byte boundaries (VEC false) they are read in words of 4 bytes
 // (7680 tokens of 32 heads of 65: 52 us, value by value 93) and written value by value, neighbouring lanes neighbouring values, through shared memory:
 // [row of the warp][16 * LANES values].
-// 16384 tokens of 8 heads of 128 in bf16 enter an e4m3 cache in 33 us (3.1 TB/s: the rounding, some twenty
-// instructions a value, takes as long as the memory); 65536 of them come back in 75 us (5.4 TB/s).
+// 16384 tokens of 8 heads of 128 in bf16 enter an e4m3 cache in 33 us (3.1 TB/s): 15.5 us of memory at the copy rate and
+// some 19 of issue (the rounding is about twenty instructions a value) that follow one another, as nothing is
+// requested while a pair of pieces is rounded; 65536 of them come back in 75 us (5.4 TB/s).
 constexpr int kRowsThreads = 256;
 constexpr int kRowsPieces = 8;  // of a thread, at most
 constexpr int kRowsTokens = 64;
@@ -351,15 +352,17 @@ __global__ void __launch_bounds__(kRowsThreads) k_cache_read(const RowsArgs a) {
 // positions along g and heads along c and is turned by movmatrix.
 // Weights: p = exp2(s - m), w = p * value scale / r in fp16, r being 2^-7 of the largest p * value scale so far, so
 // that rows of small and large scale keep their accuracy: half a step of fp16, and where w is subnormal 2^-32 of that
-// largest one.  m only moves when p grew by more than 2^8, and r moves with it: p and r are relative to the same m, so
+// largest one (the sums are fp32, of which a product loses what lies 2^-24 below them).  m only moves when p grew by more than 2^8, and r moves with it: p and r are relative to the same m, so
 // the sums stay as they are.  r grows, and the sums are taken down, when w would pass 2^15.  (r left behind when m
 // moves would belong to weights that have just become small: a later row that has all the weight but a scale
 // 2^-20 of an earlier one's would be rounded to a few bits, or to nothing.)
 //
-// Measured: 64 sequences, 32 query and 8 key heads of 128, 554 MB of e4m3 codes and scales in 130 us (4.3
-// TB/s; int8 codes, which take fewer conversion instructions, 121 us).  Bound by the turning of codes into fp16
-// (four instructions an e4m3 pair) and by the warps' uneven speeds: they end between 53 and 114 us, the
-// median at 96.  One sequence of 1000 positions takes 10 us on the GPU, two launches and one trip to memory each.
+// Measured: 64 sequences, 32 query and 8 key heads of 128, 554 MB of e4m3 codes and scales in 130 us a call (4.3
+// TB/s), 121 of them on the GPU (int8 codes, which take fewer conversion instructions, 115).  Bound by the warps' uneven
+// speeds, a tenth of them ending before 83 us, half before 87 and the last at 111, and the join behind that; the
+// conversions are the 6 us between the formats.  One sequence of 1000 positions takes 11 us on the GPU, two launches and
+// one trip to memory each.  More than 16 query heads a key head read the cache once per 16 (32 heads on one: 76 us,
+// 16 on one: 58).
 struct PagedArgs {
   CacheView c;
   const void *q;

@@ -95,11 +95,13 @@ __device__ __forceinline__ V block_total(V v, V *scratch) {
 // The bins only select, so their rounding does not matter; everything that decides is done on the logits'
 // order and on integer masses.  A bin that holds more than kList tokens (a row of almost equal logits) sends
 // the row to sample_by_radix, which reads it again from global memory.
-// What bounds it: the 64-bit exponentials where the whole row is kept (eleven operations a logit at 64 a clock
-// and SM), exchanges between the CTAs (a microsecond each) for few rows.
-// 256 rows of 131072 fp32 logits (134 MB): 85 us for the largest alone, 157 with the masses of the whole row, 164 with a
-// top_k of 50, 353 with a top_p of 0.9; of that about 11 us go to the start and end of each wave of clusters.  Four
-// rows of 32128: 8 us.
+// What bounds it: the passes over a slice and the exchanges between them (a barrier of the cluster and a trip through
+// distributed shared memory, a microsecond and more each), during which a CTA requests nothing: a cluster has one
+// row, and only the SM's second CTA works meanwhile.  With a top_p, of a row's 43 us loading takes 6.5, the masses and
+// counts 8.4, selecting and gathering 9.  The 64-bit exponentials (eleven operations a logit at 64 a clock and SM)
+// are 20 us of the times below.
+// 256 rows of 131072 fp32 logits (134 MB): 84 us for the largest alone, 155 with the masses of the whole row, 164 with a
+// top_k of 50, 354 with a top_p of 0.9 (bf16: 77, 149, 162, 363).  Four rows of 32128: 8 us.
 constexpr int kRowThreads = 512;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kBins = 1024;
