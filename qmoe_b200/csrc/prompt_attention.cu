@@ -140,11 +140,12 @@ __global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
 // sum are taken relative to the older maximum, which is exact up to rounding since both are scaled alike.
 // P is rounded to the type of the inputs for the second product (half a step of it relative to every
 // weight); the sum is taken from the unrounded fp32 weights.
-// A query that sees a score of NaN or +inf has a sum of NaN, or one that no finite scores reach (pair_exp2 turns NaN
-// into a huge number): its output is NaN, as the formula has it.  A value row that is not finite would spoil queries
-// that give it weight 0 (0 * inf): a query row whose sum is in order and whose result is not finite is computed again
-// by a warp of its own, some hundred times slower than the tiles: 4096 tokens, 32 heads of 128, take 120 us, and 42 ms
-// with an infinite first value row, which every query sees.
+// A query that sees a score of NaN or +inf, which the tiles' maxima show, gets NaN, as the formula has it.
+// A query row is computed again by a warp of its own where its result is not finite, as a value row that is not finite
+// spoils queries that give it weight 0 too (0 * inf), and where its scores are so large (2^27 and more) that the rounded
+// maximum lies some units of log 2 beside the largest score, by which all weights could underflow or overflow.
+// That is some hundred times slower than the tiles: 4096 tokens, 32 heads of 128, take 120 us, and 42 ms with an
+// infinite first value row, which every query sees.
 // All waits are bounded (kPromptWait); when one runs out the CTA counts itself in d_prompt_timeouts, waits for its
 // copies and products in flight, frees its tensor memory and returns.
 constexpr int kPromptThreads = 512;
@@ -155,7 +156,6 @@ constexpr int kItems = 4;         // decided ahead
 constexpr int kItemReaders = 10;  // arrivals that give an item back: eight softmax warps, one for products, one for copies
 constexpr int kBlockBytes = kTileRows * 128;  // 64 columns of a tile
 constexpr int kPolyPairs = 2;
-constexpr float kLargestSum = 0x1p100f;  // of finite scores: 2^25 weights of at most 2^8 are far below
 constexpr int kWave = 148;      // CTAs at a time
 constexpr int kMaxParts = 32;   // a warp's lanes look after one each when they are joined
 constexpr unsigned long long kPromptWait = 4000000000ull;  // ns without progress
@@ -206,9 +206,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float in_log2(float b) { return b == -INFINITY ? b : fmaxf(b * kLog2e, -FLT_MAX); }
 
+// NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 
@@ -612,6 +618,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       const int last = live ? row + shift : -1;  // last key that the query sees
       const float *bias = BIAS ? a.bias + (size_t)head * a.s.n_dist : nullptr;
       float top = -INFINITY, sum = 0.f;  // maximum that O and the sum are relative to, in units of log 2
+      bool lost = false;                 // a score was NaN or +inf
+      bool rough = false;                // `top` is not near the largest score any more
       float *near_bias = reinterpret_cast<float *>(stage_out + warp * 4096);
       const float far_bias = BIAS ? in_log2(bias[a.s.n_dist - 1]) : 0.f;
       for (int j = 0; j < steps; j++) {
@@ -681,12 +689,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         }
         m0 = max3(m0, s[kTileRows - 4], s[kTileRows - 3]);
         m1 = max3(m1, s[kTileRows - 2], s[kTileRows - 1]);
-        float tile_top = fmaxf(max3(m0, m1, m2), m3);
+        float tile_top = max2(max3(m0, m1, m2), m3);
+        lost = lost || !(tile_top < INFINITY);
+        const float raw_top = tile_top;
         if (!BIAS) tile_top *= sl2;
         const bool grow = tile_top > top + 8.f || (top == -INFINITY && tile_top > top);
         if (__any_sync(0xffffffffu, grow)) {
           const float next = grow ? tile_top : top;
           const float keep = grow ? exp2_approx(top - next) : 1.f;
+          if (!BIAS) rough = rough || (grow && fabsf(fmaf(raw_top, sl2, -next)) > 4.f);
           top = next;
           sum *= keep;
           if (j > 0) {
@@ -754,7 +765,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       done += steps;
       if (SPLIT) {
         const long long at = ((item.q_row + (long long)row) * a.s.heads + head) * a.n_parts + item.part;
-        if (live) a.part_stat[at] = make_float2(top, sum);
+        if (live) a.part_stat[at] = make_float2(lost ? __int_as_float(0x7fffffff) : top, rough ? __int_as_float(0x7fffffff) : sum);
         // rows through shared memory, 32 columns at a time (stores by the thread that owns the row took 20 us more
         // for 1024 queries of 32 heads in two parts)
         uint8_t *stage = stage_out + warp * 4096;
@@ -782,7 +793,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
       }
       // Rows go through shared memory, 64 columns at a time, so that a warp writes them one after another instead
       // of one piece of 32 rows at a time.
-      const bool lost = !(sum <= kLargestSum);  // a score was NaN or +inf
       const float inv = lost ? __int_as_float(0x7fffffff) : (sum == 0.f ? 0.f : 1.f / sum);
       uint8_t *stage = stage_out + warp * 4096;
       const int t0 = t & ~31, rows = min(32, n - (tile0 + t0));  // of this warp
@@ -830,7 +840,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_prompt_tiles(const Prompt
         __syncwarp();
       }
       tc_fence_before();
-      unsigned again = __ballot_sync(0xffffffffu, live && !finite && !lost);
+      unsigned again = __ballot_sync(0xffffffffu, live && (!finite || rough) && !lost);
       while (again != 0) {
         const int l = __ffs(again) - 1;
         again &= again - 1;
@@ -879,7 +889,7 @@ __global__ void __launch_bounds__(kPartsThreads) k_prompt_join(const PromptArgs 
   }
   bool finite = true;
   T *out = reinterpret_cast<T *>(a.out) + row * a.s.out_row + head * a.s.out_head + 4 * lane;
-  const bool lost = __any_sync(0xffffffffu, !(stat.y <= kLargestSum));  // a score was NaN or +inf
+  const bool lost = __any_sync(0xffffffffu, isnan(stat.x));  // a score was NaN or +inf
   const float inv = lost ? __int_as_float(0x7fffffff) : (sum == 0.f ? 0.f : 1.f / sum);
   __align__(8) T v[4];
 #pragma unroll

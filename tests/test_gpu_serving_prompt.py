@@ -429,3 +429,20 @@ def test_more_query_rows_than_a_grid_axis():
     wide = torch.zeros(1, 1, 136, dtype=torch.bfloat16, device=DEV).expand(270000, 1, 136)
     with pytest.raises(RuntimeError, match="262140"):
         serving.prompt_attention(wide, wide, wide, _cu([270000]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,m,heads", [(300, 300, 2), (300, 300, 160), (60, 3000, 2)])
+@pytest.mark.parametrize("power", [0, 13, 20, 30])
+def test_scores_of_any_finite_size(power, n, m, heads, dtype):
+    """Products that are whole numbers times 2^power: exact in 32 bits, far apart, some of them equal."""
+    d = 64
+    g = torch.Generator(device=DEV).manual_seed(28)
+    q, k = (torch.randint(-8, 9, (rows, h, d), generator=g, device=DEV).to(dtype) for rows, h in ((n, heads), (m, 1)))
+    q, k = q * 2.0 ** (power // 2 - 3), k * 2.0 ** (power - power // 2)      # fp16: 8 * 2^15 does not fit
+    if not bool(q.isfinite().all() and k.isfinite().all()):
+        pytest.skip("fp16 does not hold such values")
+    v = torch.randn(m, 1, d, generator=g, device=DEV).to(dtype)
+    got = serving.prompt_attention(q, k, v, _cu([n]), _cu([m]), scale=1.0)
+    some = torch.linspace(0, heads - 1, 2).long().tolist()
+    _check(got[:, some], q[:, some], k, v, [n], [m], 1.0)
